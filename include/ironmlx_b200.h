@@ -155,6 +155,19 @@ IMX_API int imx_moe_forward_residual(const imx_moe_config* cfg, const imx_moe_we
 IMX_API int imx_rms_norm(const void* x, int n_rows, int hidden, const void* weight, float eps, void* y,
                  void* stream);
 
+/* The residual's addition, the norm that follows it, and the rows of the next projection in 8 bits, in one pass
+ * (mlx/src/model/qwen35.rs:262-273 around fast::rms_norm):
+ *   v = x + residual (fp32), h = bf16(v), u = v * rsqrt(mean(v^2) + eps) * weight (fp32)
+ *   y = bf16(u);  y_q, y_scales = u as mxfp8 rows (imx_quantize's layout and rule), which imx_mxfp8_matmul reads
+ * Sums and products stay in fp32 and every output is rounded once: y may differ from imx_rms_norm's of h, which
+ * rounds in between, by a step of bf16.
+ * x, residual, h, y: bf16 [n_rows, hidden]; residual may be NULL (v = x); weight: bf16 [hidden] or NULL; y_q: e4m3
+ * [n_rows, hidden], y_scales: ue8m0 [n_rows, hidden / 32].  h, y and the pair y_q, y_scales may each be NULL, not all.
+ * hidden: a multiple of 8 (of 32 with y_q), at most 32768; arrays 16-byte aligned (y_scales: any).  h or y may be x's or
+ * residual's own buffer; any other overlap of an output with another array is refused. */
+IMX_API int imx_add_rms_norm(const void* x, const void* residual, int n_rows, int hidden, const void* weight, float eps,
+                     void* h, void* y, void* y_q, void* y_scales, void* stream);
+
 /* imx_moe_forward with CUDA events recorded on the stream between its stages;
  * synchronises and returns the five stage durations in milliseconds:
  * router, dispatch sort, first expert product (gate/up + SwiGLU), second
@@ -365,6 +378,39 @@ IMX_API int imx_expert_forward(const imx_moe_config* cfg, const imx_qtensor* gat
  * dense `Linear::forward_with_stream` (mlx/src/nn/linear.rs:170-177); bias may be NULL. */
 IMX_API int imx_linear(const void* x, int m, int in, const void* w, int n_out, const void* bias, void* y,
                void* stream);
+
+/* y[m, n_out] = dequantize(x_q)[m, in] @ dequantize(w[n_out, in])^T, both operands mxfp8 (e4m3, one ue8m0 scale per 32
+ * values), fp32 accumulation, y bf16: what `QuantizedLinear::forward_with_stream` (mlx/src/nn/linear.rs:51-63) computes
+ * for an mxfp8 weight, on rows that imx_add_rms_norm (or imx_quantize) left in 8 bits.  w->biases is NULL, w->global_scale
+ * is not read.  in: a multiple of 32; x_q and w->w 16-byte aligned, scales at any byte, y at any bf16 value (rows that
+ * start on 16 bytes are written fastest).  y overlaps no input.  scratch: imx_mxfp8_matmul_scratch_bytes bytes, 256-byte
+ * aligned, zero-filled once; it holds the status word that imx_moe_status() reads and nothing that a call leaves for
+ * another, so that calls on several streams may share it.  Should a bounded wait run out, the outputs concerned are NaN. */
+IMX_API int imx_mxfp8_matmul_scratch_bytes(int m, int n_out, int in, size_t* bytes);
+IMX_API int imx_mxfp8_matmul(const void* x_q, const void* x_scales, int m, const imx_qtensor* w, int n_out, int in, void* y,
+                     void* scratch, size_t scratch_bytes, void* stream);
+
+/* Low-rank adapters, `count` of them, of one projection: a[j] is [rank, in], b[j] is [n_out, rank], both bf16. */
+typedef struct imx_adapters {
+    const void* a;           /* bf16 [count, rank, in]                       */
+    const void* b;           /* bf16 [count, n_out, rank]                    */
+    const float* scale;      /* fp32 [count] (alpha / rank), or NULL (= 1)   */
+    int count;
+    int rank;                /* a multiple of 8, at most 256; adapters of a smaller rank are padded with zeros */
+} imx_adapters;
+
+/* The adapters of many requests beside a shared projection (no counterpart in the reference): row t of the batch has
+ * the adapter j = ids[t],
+ *   out[t] = bf16( y[t] + scale[j] * (x[t] . a[j]^T) . b[j]^T )
+ * with y[t] the projection's row, x[t] its input, sums in fp32.  A row whose id is outside [0, count) -- -1 by convention --
+ * has no adapter: out[t] = y[t].  Ids may come in any order.
+ * x: bf16 [n_rows, in], in a multiple of 8; y, out: bf16 [n_rows, n_out]; out may be y itself, any other overlap is refused.
+ * x, a and b 16-byte aligned; y and out at any bf16 value (16 bytes and n_out a multiple of 8 are fastest).
+ * scratch: imx_low_rank_scratch_bytes bytes, 256-byte aligned, its contents do not matter; calls that may run at the same
+ * time need a scratch each. */
+IMX_API int imx_low_rank_scratch_bytes(int n_rows, int in, int n_out, int count, int rank, size_t* bytes);
+IMX_API int imx_low_rank_add(const void* y, const void* x, int n_rows, int in, const imx_adapters* adapters,
+                     const int32_t* ids, int n_out, void* out, void* scratch, size_t scratch_bytes, void* stream);
 
 /* Quantize w[rows, in] (fp32) into packed values, scales and biases
  * (absent from the reference's wrappers, which only consume checkpoints that

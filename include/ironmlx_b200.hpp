@@ -139,7 +139,40 @@ inline void dequantize(const Array& w, const Array& scales, const Array* biases,
                          stream));
 }
 
+// Rows in mxfp8 (packed [M, in/4], scales [M, in/32]) times an mxfp8 weight.  The scratch is zero-filled when it is made and
+// only ever holds the status word.
+inline void mxfp8_matmul(const Array& rows, const Array& row_scales, const Array& w, const Array& scales, Array& y,
+                         cudaStream_t stream = nullptr) {
+    imx_qtensor q{w.ptr, scales.ptr, nullptr, 1.f};
+    const int in = (int)row_scales.dim(-1) * 32, m = (int)(row_scales.size() / row_scales.dim(-1)), n_out = (int)y.dim(-1);
+    size_t need = 0;
+    check(imx_mxfp8_matmul_scratch_bytes(m, n_out, in, &need));
+    Scratch& sc = Scratch::local();
+    void* ws = sc.get(need);
+    check(imx_mxfp8_matmul(rows.ptr, row_scales.ptr, m, &q, n_out, in, y.ptr, ws, sc.bytes(), stream));
+}
+
 }  // namespace ops
+
+// The low-rank adapters of one projection: a [count, rank, in], b [count, out, rank] bf16, scale fp32 [count].
+struct LowRankAdapters {
+    Array a, b;
+    std::optional<Array> scale;
+    // y += scale[j] * (x a[j]^T) b[j]^T with j = ids[t] for each row t (none where it is negative)
+    void add(Array& y, const Array& x, const Array& ids, cudaStream_t stream = nullptr) const {
+        const imx_adapters ad{a.ptr, b.ptr, scale ? (const float*)scale->ptr : nullptr, (int)a.dim(0), (int)a.dim(1)};
+        const int in = (int)a.dim(2), n_out = (int)b.dim(1), rows = (int)(x.size() / in);
+        if (x.dim(-1) != in || y.dim(-1) != n_out || ids.size() != rows)
+            throw Error(IMX_ERR_INVALID, "LowRankAdapters: shapes do not match the adapters");
+        size_t need = 0;
+        check(imx_low_rank_scratch_bytes(rows, in, n_out, ad.count, ad.rank, &need));
+        void* ws = scratch_.get(need);
+        check(imx_low_rank_add(y.ptr, x.ptr, rows, in, &ad, (const int32_t*)ids.ptr, n_out, y.ptr, ws, scratch_.bytes(), stream));
+    }
+
+private:
+    mutable Scratch scratch_;
+};
 
 // Dense bf16 projection x . W^T (+ b) (mlx/src/nn/linear.rs:129-177); inside the block it is only a holder of
 // its weight (router, shared-expert gate).
@@ -187,6 +220,11 @@ struct QuantizedLinear {
         ops::quantized_matmul(x, weight, scales, biases ? &*biases : nullptr, true, group_size, bits, mode, y, stream,
                               global_scale);
     }
+    // The projection of rows that RMSNorm::forward_residual left in 8 bits (mxfp8 weights only).
+    void forward_rows(const Array& rows, const Array& row_scales, Array& y, cudaStream_t stream = nullptr) const {
+        if (mode != "mxfp8") throw Error(IMX_ERR_INVALID, "forward_rows: 8-bit rows need an mxfp8 weight, not " + mode);
+        ops::mxfp8_matmul(rows, row_scales, weight, scales, y, stream);
+    }
     imx_qtensor qtensor() const {
         return imx_qtensor{weight.ptr, scales.ptr, biases ? biases->ptr : nullptr, global_scale};
     }
@@ -199,6 +237,13 @@ struct RMSNorm {
     void forward_with_stream(const Array& x, Array& y, cudaStream_t stream = nullptr) const {
         const int h = (int)x.dim(-1);
         check(imx_rms_norm(x.ptr, (int)(x.size() / h), h, weight.ptr, eps, y.ptr, stream));
+    }
+    // h = x + residual and its norm in one pass: y bf16 and / or rows in mxfp8 (rows and row_scales), whichever is given
+    void forward_residual(const Array& x, const Array* residual, Array* h, Array* y, Array* rows, Array* row_scales,
+                          cudaStream_t stream = nullptr) const {
+        const int n = (int)x.dim(-1);
+        check(imx_add_rms_norm(x.ptr, residual ? residual->ptr : nullptr, (int)(x.size() / n), n, weight.ptr, eps, h ? h->ptr : nullptr,
+                               y ? y->ptr : nullptr, rows ? rows->ptr : nullptr, row_scales ? row_scales->ptr : nullptr, stream));
     }
 };
 

@@ -25,6 +25,10 @@ class QTensor(C.Structure):
                 ("global_scale", C.c_float)]
 
 
+class Adapters(C.Structure):
+    _fields_ = [("a", C.c_void_p), ("b", C.c_void_p), ("scale", C.c_void_p), ("count", C.c_int), ("rank", C.c_int)]
+
+
 class MoEConfig(C.Structure):
     _fields_ = [(n, C.c_int) for n in (
         "hidden", "num_experts", "top_k", "intermediate", "shared_intermediate", "norm_topk_prob",
@@ -63,6 +67,7 @@ SIGNATURES = {
     "imx_moe_forward_residual": (_i, [C.POINTER(MoEConfig), C.POINTER(MoEWeights), _vp, _vp, _f, _i, _vp, _vp, _sz, _vp,
                                       C.POINTER(MoETrace)]),
     "imx_rms_norm": (_i, [_vp, _i, _i, _vp, _f, _vp, _vp]),
+    "imx_add_rms_norm": (_i, [_vp, _vp, _i, _i, _vp, _f, _vp, _vp, _vp, _vp, _vp]),
     "imx_moe_forward_timed": (_i, [C.POINTER(MoEConfig), C.POINTER(MoEWeights), _vp, _i, _vp, _vp, _sz, _vp,
                                    C.POINTER(C.c_float)]),
     "imx_moe_forward_host": (_i, [C.POINTER(MoEConfig), C.POINTER(MoEWeights), _vp, _i, _vp, _vp, _sz, _vp]),
@@ -99,6 +104,10 @@ SIGNATURES = {
     "imx_expert_scratch_bytes": (_i, [C.POINTER(MoEConfig), _i, C.POINTER(_sz)]),
     "imx_expert_forward": (_i, [C.POINTER(MoEConfig), C.POINTER(QTensor), C.POINTER(QTensor), _vp, _i, _vp, _vp, _sz, _vp]),
     "imx_linear": (_i, [_vp, _i, _i, _vp, _i, _vp, _vp, _vp]),
+    "imx_mxfp8_matmul_scratch_bytes": (_i, [_i, _i, _i, C.POINTER(_sz)]),
+    "imx_mxfp8_matmul": (_i, [_vp, _vp, _i, C.POINTER(QTensor), _i, _i, _vp, _vp, _sz, _vp]),
+    "imx_low_rank_scratch_bytes": (_i, [_i, _i, _i, _i, _i, C.POINTER(_sz)]),
+    "imx_low_rank_add": (_i, [_vp, _vp, _i, _i, C.POINTER(Adapters), _vp, _i, _vp, _vp, _sz, _vp]),
     "imx_quantize": (_i, [_vp, _i, _i, _i, _i, _i, _f, _vp, _vp, _vp, _vp]),
     "imx_gather_qmm": (_i, [_vp, _vp, C.POINTER(QTensor), _vp, _i, _i, _i, _i, _i, _i, _vp, _vp]),
 }

@@ -1,0 +1,187 @@
+// The residual's addition, RMSNorm and the next projection's rows in 8 bits (mlx/src/model/qwen35.rs:262-273 around
+// fast::rms_norm, mlx/src/fast.rs:37-49), one pass over the data:
+//   v = x + residual              fp32; h = bf16(v)
+//   u = v * inv * w               fp32, inv = rsqrt(mean(v^2) + eps); y = bf16(u)
+//   q = e4m3(u / 2^e)             e per 32 values: the smallest power of two with amax / 2^e <= 448 (imx_quantize's rule)
+//
+// Bound by memory for many rows, by latency for few.  A row's values stay in the registers of its threads between the
+// sum of squares and the outputs (NV pieces of eight values a thread), so that everything is read and written once.
+// Four neighbouring lanes hold the 32 values of a scale: two shuffles give the maximum.  Dividing by a power of two is
+// exact, so that the 8-bit conversion is the only rounding there.
+#include <cuda_fp8.h>
+
+#include "internal.h"
+
+namespace imx {
+
+namespace {
+
+constexpr int kMaxRow = 32768;
+// Threads a CTA may have with NV pieces a thread: what leaves a thread the registers to hold them.
+constexpr int max_threads(int nv) { return nv <= 2 ? 1024 : 512; }
+
+struct NormOut {
+    __nv_bfloat16* h;
+    __nv_bfloat16* y;
+    uint8_t* q;
+    uint8_t* scales;
+};
+
+// Biased exponent of the scale of 32 values: e + 127, e the smallest integer in [-127, 127] with amax / 448 <= 2^e.
+__device__ __forceinline__ uint32_t scale_code(float amax) {
+    const uint32_t b = __float_as_uint(__fdiv_rn(amax, 448.f));
+    const uint32_t exp = b >> 23, man = b & 0x7fffffu;
+    if (exp == 0) return man <= 0x400000u ? 0u : 1u;             // up to 2^-127, up to 2^-126
+    return exp + (man != 0 ? 1u : 0u);
+}
+
+// T threads a row (a multiple of 32), blockDim.x / T rows a CTA.
+template <int NV>
+__global__ void __launch_bounds__(max_threads(NV))
+add_rms_norm_kernel(const __nv_bfloat16* x, const __nv_bfloat16* residual, int n, int H, const __nv_bfloat16* w, float eps,
+                    const NormOut out, int T) {
+    __shared__ float s_part[32];
+    const int row_in = threadIdx.x / T, t = threadIdx.x - row_in * T;
+    const int row = blockIdx.x * (blockDim.x / T) + row_in;
+    const int pieces = row < n ? H / 8 : 0;
+    const size_t base = (size_t)row * H;
+    float v[NV][8];
+    float ss = 0.f;
+    uint4 a[NV], b[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int p = t + i * T;
+        if (p < pieces) {
+            a[i] = *reinterpret_cast<const uint4*>(x + base + (size_t)p * 8);
+            if (residual != nullptr) b[i] = *reinterpret_cast<const uint4*>(residual + base + (size_t)p * 8);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        if (t + i * T < pieces) {
+            const __nv_bfloat162* pa = reinterpret_cast<const __nv_bfloat162*>(&a[i]);
+            const __nv_bfloat162* pb = reinterpret_cast<const __nv_bfloat162*>(&b[i]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float2 f = __bfloat1622float2(pa[j]);
+                if (residual != nullptr) {
+                    const float2 g = __bfloat1622float2(pb[j]);
+                    f.x += g.x;
+                    f.y += g.y;
+                }
+                v[i][2 * j] = f.x;
+                v[i][2 * j + 1] = f.y;
+                ss = fmaf(f.x, f.x, ss);
+                ss = fmaf(f.y, f.y, ss);
+            }
+        }
+    }
+    ss = warp_sum(ss);
+    if (T > 32) {
+        if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5] = ss;
+        __syncthreads();
+        ss = 0.f;
+        for (int i = 0; i < T / 32; ++i) ss += s_part[row_in * (T / 32) + i];
+    }
+    const float inv = rsqrtf(ss / (float)H + eps);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int p = t + i * T;
+        // whole quads of lanes are in or out where a scale is wanted (H a multiple of 32)
+        const unsigned active = __ballot_sync(0xffffffffu, p < pieces);
+        if (p >= pieces) continue;
+        const size_t at = base + (size_t)p * 8;
+        if (out.h != nullptr) {
+            __nv_bfloat162 o[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = __floats2bfloat162_rn(v[i][2 * j], v[i][2 * j + 1]);
+            *reinterpret_cast<uint4*>(out.h + at) = *reinterpret_cast<const uint4*>(o);
+        }
+        float u[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[j] = v[i][j] * inv;
+        if (w != nullptr) {
+            const uint4 wv = __ldg(reinterpret_cast<const uint4*>(w + (size_t)p * 8));
+            const __nv_bfloat162* pw = reinterpret_cast<const __nv_bfloat162*>(&wv);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 f = __bfloat1622float2(pw[j]);
+                u[2 * j] *= f.x;
+                u[2 * j + 1] *= f.y;
+            }
+        }
+        if (out.y != nullptr) {
+            __nv_bfloat162 o[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = __floats2bfloat162_rn(u[2 * j], u[2 * j + 1]);
+            *reinterpret_cast<uint4*>(out.y + at) = *reinterpret_cast<const uint4*>(o);
+        }
+        if (out.q != nullptr) {
+            float amax = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(u[j]));
+            amax = fmaxf(amax, __shfl_xor_sync(active, amax, 1));
+            amax = fmaxf(amax, __shfl_xor_sync(active, amax, 2));
+            const uint32_t code = scale_code(amax);
+            const float up = __uint_as_float((254u - code) << 23);         // 2^-e
+            uint16_t c[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)                                    // NaN stays NaN
+                c[j] = __nv_cvt_float2_to_fp8x2(make_float2(u[2 * j] * up, u[2 * j + 1] * up), __NV_SATFINITE, __NV_E4M3);
+            *reinterpret_cast<uint2*>(out.q + at) = make_uint2(c[0] | (uint32_t)c[1] << 16, c[2] | (uint32_t)c[3] << 16);
+            if ((p & 3) == 0) out.scales[at / 32] = (uint8_t)code;
+        }
+    }
+}
+
+int launch_add_rms_norm(const void* x, const void* residual, int n, int H, const void* w, float eps, const NormOut& out, cudaStream_t stream) {
+    const int pieces = H / 8;
+    // As few threads a row as hold it in eight pieces each while there are rows enough to fill the GPU; one piece a
+    // thread, the shortest way, for a few rows.
+    DeviceInfo di;
+    IMX_TRY(current_device(&di));
+    int T = 32;
+    while (T < 512 && T * 4 < pieces) T *= 2;
+    const int most = pieces <= 2 * 1024 ? 1024 : 512;
+    while (T < most && T < pieces && (long)n * T < 1024L * di.sms) T *= 2;
+    const int block = T > 256 ? T : 256;
+    const int grid = ceil_div(n, block / T);
+    const int nv = ceil_div(pieces, T);
+    auto kernel = nv <= 1 ? add_rms_norm_kernel<1> : (nv <= 2 ? add_rms_norm_kernel<2> : (nv <= 4 ? add_rms_norm_kernel<4> : add_rms_norm_kernel<8>));
+    kernel<<<grid, block, 0, stream>>>((const __nv_bfloat16*)x, (const __nv_bfloat16*)residual, n, H, (const __nv_bfloat16*)w, eps,
+                                       out, T); IMX_LAUNCHED();
+    IMX_CHECK_CUDA(cudaGetLastError());
+    return IMX_OK;
+}
+
+}  // namespace
+
+}  // namespace imx
+
+using namespace imx;
+
+extern "C" int imx_add_rms_norm(const void* x, const void* residual, int n_rows, int hidden, const void* weight, float eps,
+                                void* h, void* y, void* y_q, void* y_scales, void* stream) {
+    IMX_REQUIRE(n_rows >= 0, "add_rms_norm: negative row count");
+    IMX_REQUIRE(hidden > 0 && hidden % 8 == 0 && hidden <= kMaxRow,
+                "add_rms_norm: the row length (%d) must be a positive multiple of 8, at most %d", hidden, kMaxRow);
+    if (n_rows == 0) return IMX_OK;
+    IMX_REQUIRE((y_q == nullptr) == (y_scales == nullptr), "add_rms_norm: y_q and y_scales go together");
+    IMX_REQUIRE(y_q == nullptr || hidden % 32 == 0, "add_rms_norm: 8-bit rows need a row length (%d) that is a multiple of 32", hidden);
+    IMX_REQUIRE(x != nullptr && (h != nullptr || y != nullptr || y_q != nullptr), "add_rms_norm: x and an output are required");
+    IMX_REQUIRE((((uintptr_t)x | (uintptr_t)residual | (uintptr_t)weight | (uintptr_t)h | (uintptr_t)y | (uintptr_t)y_q) % 16) == 0,
+                "add_rms_norm: arrays must be 16-byte aligned");
+    const size_t values = (size_t)n_rows * hidden;
+    const void* outs[4] = {h, y, y_q, y_scales};
+    const size_t sizes[4] = {values * 2, values * 2, values, values / 32};
+    for (int i = 0; i < 4; ++i) {
+        for (int j = i + 1; j < 4; ++j)
+            IMX_REQUIRE(!overlap(outs[i], sizes[i], outs[j], sizes[j]), "add_rms_norm: two outputs overlap");
+        IMX_REQUIRE(!overlap(outs[i], sizes[i], weight, (size_t)hidden * 2), "add_rms_norm: an output overlaps the weight");
+        for (const void* in : {x, residual})
+            IMX_REQUIRE(!overlap(outs[i], sizes[i], in, values * 2) || (i < 2 && outs[i] == in),
+                        "add_rms_norm: an output overlaps an input without being it");
+    }
+    return launch_add_rms_norm(x, residual, n_rows, hidden, weight, eps,
+                               NormOut{(__nv_bfloat16*)h, (__nv_bfloat16*)y, (uint8_t*)y_q, (uint8_t*)y_scales}, (cudaStream_t)stream);
+}

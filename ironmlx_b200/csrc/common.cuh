@@ -47,6 +47,10 @@ void count_launch();
 #define IMX_LAUNCHED() ::imx::count_launch()
 
 inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
+// Whether two arrays of na and nb bytes share any (NULL shares none).
+inline bool overlap(const void* a, size_t na, const void* b, size_t nb) {
+    return a != nullptr && b != nullptr && (uintptr_t)a < (uintptr_t)b + nb && (uintptr_t)b < (uintptr_t)a + na;
+}
 inline size_t align_up(size_t v, size_t a) { return (v + a - 1) / a * a; }
 
 // ── format description shared by all kernels ────────────────────────────────

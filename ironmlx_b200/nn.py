@@ -23,7 +23,29 @@ from ._lib import IronMLXError, MoEConfig, MoETrace, MoEWeights, QTensor, check,
 
 
 @dataclass
-class Linear:
+class LowRankAdapters:
+    """The low-rank adapters of one projection, for batches whose rows belong to requests with different ones: a
+    [count, rank, in] and b [count, out, rank] bf16, scale fp32 [count] (alpha / rank; None: 1).  Adapters of a smaller
+    rank are padded with zeros."""
+    a: torch.Tensor
+    b: torch.Tensor
+    scale: Optional[torch.Tensor] = None
+
+    def add(self, y: torch.Tensor, x: torch.Tensor, ids: torch.Tensor, stream=None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """y + scale * (x a^T) b^T with the adapter ids[t] of each row (none where it is negative)."""
+        return ops.low_rank_add(y, x, self.a, self.b, ids, self.scale, out, stream)
+
+
+class _WithAdapters:
+    def forward_with_adapters(self, x: torch.Tensor, adapters: LowRankAdapters, ids: torch.Tensor, stream=None) -> torch.Tensor:
+        """The shared projection of all rows and the low-rank adapter ids[t] of each (int32, negative: none)."""
+        with ops._on(x, stream):
+            y = self.forward_with_stream(x)
+            return adapters.add(y, x, ids, out=y)
+
+
+@dataclass
+class Linear(_WithAdapters):
     """Dense `x @ W^T (+ b)` (mlx/src/nn/linear.rs:129-177).  On the MoE path
     only the router and the shared-expert gate are dense, and both are consumed
     inside the fused block; called on its own it is one bf16 tensor-core GEMM."""
@@ -47,9 +69,14 @@ class RMSNorm:
     def forward_with_stream(self, x: torch.Tensor, stream=None) -> torch.Tensor:
         return ops.rms_norm(x, self.weight, self.eps, stream)
 
+    def forward_residual(self, x: torch.Tensor, residual: Optional[torch.Tensor], out: str = "bf16", stream=None):
+        """h = x + residual and its norm in one pass: (h, y, rows) as `ops.add_rms_norm` returns them; out: "bf16", "mxfp8"
+        (8-bit rows for `QuantizedLinear.forward_rows`) or "both"."""
+        return ops.add_rms_norm(x, residual, self.weight, self.eps, out, stream)
+
 
 @dataclass
-class QuantizedLinear:
+class QuantizedLinear(_WithAdapters):
     """mlx/src/nn/linear.rs:13-63: packed weight + per-group scales/biases,
     forward = `quantized_matmul(x, w, scales, biases, transpose=true, ...)`."""
     weight: torch.Tensor
@@ -72,6 +99,12 @@ class QuantizedLinear:
     def forward_with_stream(self, x: torch.Tensor, stream=None) -> torch.Tensor:
         return ops.quantized_matmul(x, self.weight, self.scales, self.biases, True, self.group_size,
                                     self.bits, self.mode, stream, self.global_scale)
+
+    def forward_rows(self, rows: ops.Mxfp8Rows, stream=None) -> torch.Tensor:
+        """The projection of rows that `RMSNorm.forward_residual` left in 8 bits (mxfp8 weights only)."""
+        if self.mode != "mxfp8" or self.biases is not None:
+            raise IronMLXError(_lib.ERR_INVALID, f"forward_rows: 8-bit rows need an mxfp8 weight, not {self.mode}")
+        return ops.mxfp8_matmul(rows, self.weight, self.scales, stream)
 
     def qtensor(self) -> QTensor:
         return ops.qtensor(self.weight, self.scales, self.biases, self.global_scale)

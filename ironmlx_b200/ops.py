@@ -10,8 +10,9 @@ scales/biases bf16, mxfp8/nvfp4 scales uint8.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -199,3 +200,145 @@ def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor], eps: float, stream
     check(lib().imx_rms_norm(x.data_ptr(), x.numel() // h, h, None if weight is None else weight.data_ptr(),
                              float(eps), y.data_ptr(), stream_ptr(stream)))
     return y
+
+
+class Mxfp8Rows(NamedTuple):
+    """Activation rows in mxfp8, laid out as `quantize(..., mode="mxfp8")` lays out weights: e4m3 codes as int32 words
+    [.., in/4] and ue8m0 scales uint8 [.., in/32]."""
+    packed: torch.Tensor
+    scales: torch.Tensor
+
+
+def _on(x: torch.Tensor, stream):
+    """The device of x, and the given stream, made current: what is allocated within belongs to that stream, and the
+    launches go to that device."""
+    if stream is not None:
+        return torch.cuda.stream(stream)
+    if x.device.index != torch.cuda.current_device():
+        return torch.cuda.device(x.device)
+    return contextlib.nullcontext()
+
+
+def _require_same_device(name, first, *tensors):
+    _require_cuda(first, *tensors)
+    for t in tensors:
+        if t is not None and t.device != first.device:
+            raise IronMLXError(_lib.ERR_INVALID, f"{name}: tensors on {first.device} and {t.device}")
+
+
+def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: Optional[torch.Tensor], eps: float,
+                 out: str = "bf16", stream=None):
+    """`h = x + residual` and `rms_norm(h)` in one pass, sums in fp32, each output rounded once.
+
+    Returns (h, y, rows): y bf16 for out="bf16" or "both" (None otherwise), rows an `Mxfp8Rows` that `mxfp8_matmul` reads
+    for out="mxfp8" or "both" (None otherwise).  Without a residual h is x itself."""
+    _require_same_device("add_rms_norm", x, residual, weight)
+    if out not in ("bf16", "mxfp8", "both"):
+        raise IronMLXError(_lib.ERR_INVALID, f"add_rms_norm: out must be bf16, mxfp8 or both, not {out!r}")
+    for t in (x, residual, weight):
+        if t is not None and t.dtype != torch.bfloat16:
+            raise IronMLXError(_lib.ERR_INVALID, "add_rms_norm: x, residual and weight must be bfloat16")
+    if x.dim() == 0 or x.shape[-1] == 0:
+        raise IronMLXError(_lib.ERR_INVALID, "add_rms_norm: x has no last dimension")
+    hidden = x.shape[-1]
+    if residual is not None and residual.shape != x.shape:
+        raise IronMLXError(_lib.ERR_INVALID, f"add_rms_norm: residual {tuple(residual.shape)} and x {tuple(x.shape)} differ")
+    if weight is not None and weight.numel() != hidden:
+        raise IronMLXError(_lib.ERR_INVALID, f"add_rms_norm: weight has {weight.numel()} elements, rows have {hidden}")
+    if out != "bf16" and hidden % 32:
+        raise IronMLXError(_lib.ERR_INVALID, f"add_rms_norm: 8-bit rows need a row length ({hidden}) that is a multiple of 32")
+    with _on(x, stream):
+        h = x if residual is None else torch.empty_like(x)
+        y = torch.empty_like(x) if out != "mxfp8" else None
+        rows = None
+        if out != "bf16":
+            rows = Mxfp8Rows(torch.empty(*x.shape[:-1], hidden // 4, dtype=torch.int32, device=x.device),
+                             torch.empty(*x.shape[:-1], hidden // 32, dtype=torch.uint8, device=x.device))
+        check(lib().imx_add_rms_norm(x.data_ptr(), _ptr(residual), x.numel() // hidden, hidden, _ptr(weight), float(eps),
+                                     None if residual is None else h.data_ptr(), _ptr(y),
+                                     None if rows is None else rows[0].data_ptr(), None if rows is None else rows[1].data_ptr(),
+                                     torch.cuda.current_stream().cuda_stream))
+    return h, y, rows
+
+
+_STATUS = {}
+
+
+def _status_block(device) -> torch.Tensor:
+    """The status block of a device's `mxfp8_matmul` calls: zero-filled once, kernels only ever set its first word."""
+    buf = _STATUS.get(device)
+    if buf is None:
+        buf = torch.zeros(256, dtype=torch.uint8, device=device)
+        if not torch.cuda.is_current_stream_capturing():             # in a capture: one for this call
+            torch.cuda.current_stream(device).synchronize()          # other streams see the zeros
+            _STATUS[device] = buf
+    return buf
+
+
+def check_status(device, stream=None) -> None:
+    """Raises if a bounded wait ran out in an `mxfp8_matmul` call on the device since the last check; synchronises the stream."""
+    buf = _STATUS.get(torch.device(device))
+    if buf is not None:
+        with _on(buf, stream):
+            check(lib().imx_moe_status(buf.data_ptr(), torch.cuda.current_stream().cuda_stream))
+
+
+def mxfp8_matmul(rows, w: torch.Tensor, scales: torch.Tensor, stream=None) -> torch.Tensor:
+    """`dequantize(rows) @ dequantize(w)^T` with both operands in mxfp8, bf16 out: rows as `add_rms_norm` or `quantize`
+    left them ((packed, scales), an `Mxfp8Rows`), w [out, in/4] int32 and scales [out, in/32] uint8."""
+    x, xs = rows[0], rows[1]
+    _require_same_device("mxfp8_matmul", x, xs, w, scales)
+    if x.dtype != torch.int32 or w.dtype != torch.int32 or xs.dtype != torch.uint8 or scales.dtype != torch.uint8:
+        raise IronMLXError(_lib.ERR_INVALID, "mxfp8_matmul: packed values must be int32 words, scales uint8")
+    if w.dim() != 2 or scales.dim() != 2 or x.dim() == 0 or xs.dim() == 0 or w.shape[1] % 8 or w.numel() == 0:
+        raise IronMLXError(_lib.ERR_INVALID, "mxfp8_matmul: w must be [out, in/4] and scales [out, in/32], in a multiple of 32")
+    n_out, in_dim = w.shape[0], w.shape[1] * 4
+    if x.shape[-1] != w.shape[1]:
+        raise IronMLXError(_lib.ERR_INVALID, f"mxfp8_matmul: rows have {x.shape[-1] * 4} values, the weight takes {in_dim}")
+    if tuple(scales.shape) != (n_out, in_dim // 32) or tuple(xs.shape) != tuple(x.shape[:-1]) + (in_dim // 32,):
+        raise IronMLXError(_lib.ERR_INVALID, "mxfp8_matmul: one scale per 32 values is needed for the rows and the weight")
+    with _on(x, stream):
+        y = torch.empty(*x.shape[:-1], n_out, dtype=torch.bfloat16, device=x.device)
+        qt = QTensor(w.data_ptr(), scales.data_ptr(), None, 1.0)
+        check(lib().imx_mxfp8_matmul(x.data_ptr(), xs.data_ptr(), x.numel() // x.shape[-1], C.byref(qt), n_out, in_dim,
+                                     y.data_ptr(), _status_block(x.device).data_ptr(), 256,
+                                     torch.cuda.current_stream().cuda_stream))
+    return y
+
+
+def low_rank_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Tensor, ids: torch.Tensor,
+                 scale: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None, stream=None) -> torch.Tensor:
+    """`y[t] + scale[j] * (x[t] @ a[j]^T) @ b[j]^T` with j = ids[t], the adapter of row t (none where it is outside
+    [0, count): the row is y's): the adapters of many requests beside a shared projection y = W x.
+
+    y [.., out_dim], x [.., in], a [count, rank, in], b [count, out_dim, rank] bf16; ids int32, one per row; scale fp32
+    [count].  `out` may be y itself; a new tensor by default."""
+    _require_same_device("low_rank_add", y, x, a, b, ids, scale, out)
+    for t in (y, x, a, b):
+        if t.dtype != torch.bfloat16:
+            raise IronMLXError(_lib.ERR_INVALID, "low_rank_add: y, x, a and b must be bfloat16")
+    if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2] or a.numel() == 0 or b.numel() == 0:
+        raise IronMLXError(_lib.ERR_INVALID, "low_rank_add: a must be [count, rank, in] and b [count, out, rank]")
+    count, rank, in_dim = a.shape
+    n_out = b.shape[1]
+    if x.dim() == 0 or y.dim() == 0 or x.shape[-1] != in_dim or y.shape[-1] != n_out or x.shape[:-1] != y.shape[:-1]:
+        raise IronMLXError(_lib.ERR_INVALID,
+                           f"low_rank_add: x {tuple(x.shape)} and y {tuple(y.shape)} do not match adapters {in_dim} -> {n_out}")
+    rows = x.numel() // in_dim
+    if ids.dtype != torch.int32 or ids.numel() != rows:
+        raise IronMLXError(_lib.ERR_INVALID, f"low_rank_add: ids must be int32, one for each of the {rows} rows")
+    if scale is not None and (scale.dtype != torch.float32 or scale.numel() != count):
+        raise IronMLXError(_lib.ERR_INVALID, f"low_rank_add: scale must be float32, one for each of the {count} adapters")
+    if out is not None and (out.shape != y.shape or out.dtype != y.dtype):
+        raise IronMLXError(_lib.ERR_INVALID, "low_rank_add: out must have y's shape and type")
+    with _on(x, stream):
+        if out is None:
+            out = torch.empty_like(y)
+        ad = _lib.Adapters(a.data_ptr(), b.data_ptr(), _ptr(scale), count, rank)
+        nb = C.c_size_t(0)
+        check(lib().imx_low_rank_scratch_bytes(rows, in_dim, n_out, count, rank, C.byref(nb)))
+        # a scratch of its own for every call: calls on several streams, and captured ones, do not share it
+        ws = torch.empty(nb.value, dtype=torch.uint8, device=x.device)
+        check(lib().imx_low_rank_add(y.data_ptr(), x.data_ptr(), rows, in_dim, C.byref(ad), ids.data_ptr(), n_out,
+                                     out.data_ptr(), ws.data_ptr(), nb.value, torch.cuda.current_stream().cuda_stream))
+    return out

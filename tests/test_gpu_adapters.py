@@ -1,0 +1,192 @@
+"""`low_rank_add`, the low-rank adapters of many requests beside a shared projection, against a restatement in 64 bits, and
+the three operators of a projection run together.
+
+Tolerances: one rounding to bf16 is 2^-8 of the value; the low-rank row and the sum over it are kept to 16 bits or more and
+their sums in fp32: 2^-15 of the sum of magnitudes |scale| (|x| |a|^T) |b|^T covers 2^-16 for the low-rank row's rounding and
+fp32 sums of up to 8192 and 256 terms in 32 or more parts (2^-17)."""
+import ctypes as C
+
+import pytest
+import torch
+
+from ironmlx_b200 import _lib, nn, ops
+from test_gpu_rows8 import bf16, check_product, check_rows, gen, mx, norm64
+
+pytestmark = pytest.mark.gpu
+
+
+def make(g, t, k, n, count, rank, scale=True):
+    return dict(y=bf16(g, t, n), x=bf16(g, t, k), a=bf16(g, count, rank, k, std=k ** -0.5), b=bf16(g, count, n, rank, std=0.1),
+                scale=torch.rand(count, generator=g, device="cuda") * 1.5 + 0.5 if scale else None)
+
+
+def check(out, p, ids):
+    y, x = p["y"].double(), p["x"].double()
+    mag = torch.zeros_like(y)
+    for j in range(p["a"].shape[0]):
+        at = torch.nonzero(ids == j).flatten()
+        s = 1.0 if p["scale"] is None else p["scale"][j].double()
+        y[at] += s * (x[at] @ p["a"][j].double().T) @ p["b"][j].double().T
+        mag[at] += s * (x[at].abs() @ p["a"][j].double().abs().T) @ p["b"][j].double().abs().T
+    assert ((out.double() - y).abs() <= y.abs() * 2.0 ** -8 + mag * 2.0 ** -15 + 1e-38).all()
+    none = (ids < 0) | (ids >= p["a"].shape[0])
+    assert torch.equal(out[none], p["y"][none])
+
+
+def run(p, ids, **kw):
+    return ops.low_rank_add(p["y"], p["x"], p["a"], p["b"], ids, p["scale"], **kw)
+
+
+@pytest.mark.parametrize("t,k,n,count,rank", [
+    (1, 2048, 8192, 1, 16), (1, 8, 1, 1, 8), (2, 64, 7, 3, 8), (5, 4096, 2048, 4, 64), (16, 2048, 512, 40, 32), (48, 4096, 2048, 40, 32),
+    (31, 1000, 1001, 2, 24), (64, 512, 264, 64, 256), (100, 2048, 1024, 3, 128), (130, 96, 200, 5, 16), (300, 2048, 2048, 1, 16),
+    (777, 2056, 1032, 5, 40), (1100, 512, 513, 12, 64), (2050, 256, 384, 200, 8), (600, 4096, 136, 2, 256), (5000, 64, 96, 3, 16)])
+@pytest.mark.parametrize("order", ["mixed", "runs"])
+def test_low_rank_add(cuda, t, k, n, count, rank, order):
+    g = gen(t + k + n + rank)
+    p = make(g, t, k, n, count, rank, scale=order == "mixed")
+    ids = torch.randint(-1, count, (t,), generator=g, device="cuda", dtype=torch.int32)
+    if order == "runs":
+        ids = ids[torch.arange(t, device="cuda") // max(1, t // 7) * max(1, t // 7)].contiguous()
+        ids[t - t // 9:] = -1                                           # padding
+    out = run(p, ids)
+    check(out, p, ids)
+    assert torch.equal(out, run(p, ids))
+    y = p["y"].clone()
+    assert ops.low_rank_add(y, p["x"], p["a"], p["b"], ids, p["scale"], out=y) is y and torch.equal(y, out)
+
+
+@pytest.mark.parametrize("t", [3, 70, 700])
+def test_ids_without_an_adapter(cuda, t):
+    """No row has one; ids far outside; every row the last adapter.  What a row without an adapter holds is left bit for bit,
+    NaN and infinities among it, whatever its x."""
+    g = gen(t)
+    p = make(g, t, 256, 320, 5, 16)
+    p["y"][0, 5], p["y"][1, 6] = float("nan"), float("-inf")
+    p["x"][0] = float("nan")
+    none = torch.full((t,), -1, dtype=torch.int32, device=cuda)
+    assert torch.equal(run(p, none).view(torch.int16), p["y"].view(torch.int16))
+    wild = torch.tensor([-2 ** 31, 2 ** 31 - 1, 5], device=cuda).int().repeat(t)[:t].contiguous()
+    assert torch.equal(run(p, wild).view(torch.int16), p["y"].view(torch.int16))
+    last = torch.full((t,), 4, dtype=torch.int32, device=cuda)
+    last[:2] = -1
+    out = run(p, last)
+    assert torch.equal(out[:2].view(torch.int16), p["y"][:2].view(torch.int16))
+    check(out[2:], {**p, "y": p["y"][2:], "x": p["x"][2:]}, last[2:])
+
+
+@pytest.mark.parametrize("t", [2, 40, 400])
+def test_rows_that_are_not_finite_stay_alone(cuda, t):
+    """A NaN or an infinity in one row's x or y, or in one adapter, changes no row beside it, also of the same adapter."""
+    g = gen(t + 1)
+    p = make(g, t, 512, 264, 3, 16)
+    ids = (torch.arange(t, device="cuda") % 2).int()
+    clean = run(p, ids)
+    p["x"][1, 9] = float("nan")
+    p["a"][2, 3, 4] = float("nan")                                       # an adapter of no row
+    p["b"][2, 3, 4] = float("inf")
+    out = run(p, ids)
+    assert out[1].isnan().all()
+    keep = torch.arange(t, device="cuda") != 1
+    assert torch.equal(out[keep], clean[keep])
+
+
+@pytest.mark.parametrize("t,n", [(3, 40), (3, 41), (200, 136), (200, 77), (1200, 264)])
+@pytest.mark.parametrize("at", [1, 4])
+def test_low_rank_add_at_any_place(cuda, t, n, at):
+    g = gen(n)
+    p = make(g, t, 128, n, 4, 16)
+    ids = torch.randint(-1, 4, (t,), generator=g, device="cuda", dtype=torch.int32)
+    want = run(p, ids)
+    src = torch.full((t * n + 16,), 3.0, dtype=torch.bfloat16, device=cuda)
+    src[at:at + t * n] = p["y"].flatten()
+    buf = torch.full((t * n + 16,), 7.0, dtype=torch.bfloat16, device=cuda)
+    lib, nb = _lib.lib(), C.c_size_t(0)
+    ad = _lib.Adapters(p["a"].data_ptr(), p["b"].data_ptr(), p["scale"].data_ptr(), 4, 16)
+    _lib.check(lib.imx_low_rank_scratch_bytes(t, 128, n, 4, 16, C.byref(nb)))
+    scratch = torch.full((nb.value + 256,), 0xff, dtype=torch.uint8, device=cuda)
+    for dst in (buf, src):
+        _lib.check(lib.imx_low_rank_add(src.data_ptr() + 2 * at, p["x"].data_ptr(), t, 128, C.byref(ad), ids.data_ptr(), n, dst.data_ptr() + 2 * at,
+                                        scratch.data_ptr(), nb.value, torch.cuda.current_stream().cuda_stream))
+        assert torch.equal(dst[at:at + t * n].view(t, n), want)
+        assert (dst[:at] == dst[0]).all() and (dst[at + t * n:] == dst[0]).all()
+    assert (scratch[nb.value:] == 0xff).all()
+
+
+def test_adapters_on_streams(cuda):
+    g = gen(20)
+    p, q = make(g, 300, 512, 512, 6, 16), make(g, 24, 512, 512, 6, 16)
+    ip, iq = (torch.randint(-1, 6, (t,), generator=g, device="cuda", dtype=torch.int32) for t in (300, 24))
+    want = run(p, ip), run(q, iq)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [run((p, q)[i % 2], (ip, iq)[i % 2], stream=streams[i // 2 % 2]) for i in range(24)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i % 2]) for i, y in enumerate(got))
+    assert ops.low_rank_add(p["y"][:0], p["x"][:0], p["a"], p["b"], ip[:0]).shape == (0, 512)
+
+
+@pytest.mark.parametrize("kind", ["dense", "affine", "mxfp8"])
+def test_projection_with_adapters(cuda, kind):
+    g = gen(21)
+    p = make(g, 30, 512, 256, 3, 16)
+    w = torch.randn(256, 512, generator=g, device="cuda") * 0.05
+    layer = nn.Linear(w.bfloat16()) if kind == "dense" else (
+        nn.QuantizedLinear.new(*ops.quantize(w), 64, 4) if kind == "affine" else
+        nn.QuantizedLinear.new_with_mode(*ops.quantize(w, mode="mxfp8"), 32, 8, "mxfp8"))
+    ids = torch.randint(-1, 3, (30,), generator=g, device="cuda", dtype=torch.int32)
+    out = layer.forward_with_adapters(p["x"], nn.LowRankAdapters(p["a"], p["b"], p["scale"]), ids)
+    check(out, {**p, "y": layer.forward_with_stream(p["x"])}, ids)
+
+
+@pytest.mark.parametrize("t", [1, 24, 200])
+def test_norm_product_and_adapters_together(cuda, t):
+    """The three as a decoder layer runs them -- residual and norm, the projection of the 8-bit rows, the adapters of the bf16
+    rows -- eagerly, then captured and replayed with other inputs in the same buffers while another captured run of its own
+    is replayed on another stream."""
+    g = gen(22)
+    hidden, n = 512, 768
+    norm = nn.RMSNorm.new(bf16(g, hidden, std=0.1) + 1, 1e-6)
+    layer = nn.QuantizedLinear.new_with_mode(*mx(g, n, hidden, 0.02), None, 32, 8, "mxfp8")
+    p = make(g, t, hidden, n, 4, 16)
+    adapters = nn.LowRankAdapters(p["a"], p["b"], p["scale"])
+
+    def inputs():
+        return [bf16(g, t, hidden), bf16(g, t, hidden, std=2.0), torch.randint(-1, 4, (t,), generator=g, device="cuda", dtype=torch.int32)]
+
+    def step(x, r, ids):
+        h, y, rows = norm.forward_residual(x, r, "both")
+        base = layer.forward_rows(rows)
+        return h, y, rows.packed, rows.scales, base, adapters.add(base, y, ids)
+
+    first = inputs()
+    h, y, packed, scales, base, out = step(*first)
+    v, u = norm64(first[0], first[1], norm.weight)
+    check_rows((packed, scales), u)
+    check_product(base, (packed, scales), (layer.weight, layer.scales))
+    check(out, {**p, "y": base, "x": y}, first[2])
+
+    graphs, bufs, outs = [], [], []
+    for _ in range(2):
+        buf = [b.clone() for b in first]
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            got = step(*buf)
+        graphs.append((graph, side))
+        bufs.append(buf)
+        outs.append(got)
+    torch.cuda.synchronize()
+    for _ in range(3):
+        fresh = [inputs(), inputs()]
+        for buf, new in zip(bufs, fresh):
+            for b, v in zip(buf, new):
+                b.copy_(v)
+        torch.cuda.synchronize()
+        for graph, side in graphs:
+            with torch.cuda.stream(side):
+                graph.replay()
+        torch.cuda.synchronize()
+        for got, new in zip(outs, fresh):
+            assert all(torch.equal(a, b) for a, b in zip(got, step(*new)))
