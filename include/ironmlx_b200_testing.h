@@ -35,4 +35,10 @@ extern "C"
 #endif
 __attribute__((visibility("default"))) void imx_testing_prefill_give_up(int on);
 
+/* The same for imx_mxfp8_matmul: its outputs are NaN, status 4 is recorded. */
+#ifdef __cplusplus
+extern "C"
+#endif
+__attribute__((visibility("default"))) void imx_testing_mxfp8_give_up(int on);
+
 #endif /* IRONMLX_B200_TESTING_H */

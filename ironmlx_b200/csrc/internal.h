@@ -197,7 +197,7 @@ unsigned long long launch_count();   // kernels this library has launched (or re
 // One-time set-up per (device, kernel family): attributes such as the dynamic shared-memory limit are per
 // device, so a process that drives several GPUs sets them on each.  The first call on a device should come
 // before any stream capture.
-enum { kSetupDecodeTmap = 0, kSetupRouteTc = 1, kSetupPrefillTc = 2 /* + the weight format: 11 of them */ };
+enum { kSetupDecodeTmap = 0, kSetupRouteTc = 1, kSetupPrefillTc = 2 /* + the weight format: 11 of them */, kSetupMxfp8 = 16 };
 bool device_needs_setup(int ordinal, int family);
 void device_mark_setup(int ordinal, int family);
 // Tiled TMA descriptor of a 2-D row-major matrix [rows, cols] of `esize`-byte elements, `ld_bytes` between
@@ -205,6 +205,9 @@ void device_mark_setup(int ordinal, int family);
 int make_tensor_map_2d(const void* base, CUtensorMapDataType dt, size_t esize, size_t rows, size_t cols,
                        size_t ld_bytes, int box_cols, int box_rows, bool swizzle128, CUtensorMap* out,
                        bool promote256 = false, int swizzle_bytes = 0);   // swizzle_bytes: 32 / 64 when swizzle128 is false
+// The same without the cache of encodings (swizzle: 0, 32, 64 or 128 bytes).
+int encode_tensor_map_2d(const void* base, CUtensorMapDataType dt, size_t esize, size_t rows, size_t cols, size_t ld_bytes,
+                         int box_cols, int box_rows, int swizzle, bool promote256, CUtensorMap* out);
 int launch_generic_grouped(const GroupedArgs& a, cudaStream_t stream, cudaEvent_t mid = nullptr);
 
 // `residual` (bf16 [n, H] or nullptr) is added to the fp32 sums before the one rounding.

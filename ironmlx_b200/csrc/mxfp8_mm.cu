@@ -1,47 +1,695 @@
 // y = dequantize(x_q) . dequantize(w)^T with both operands in mxfp8 (e4m3 codes, one power of two for 32 values):
 //   y[m, n] = bf16( sum over the blocks g of 2^(sx + sw - 254) * sum over k in g of qx * qw )
-// One thread an output, fp32 sums.
-#include <cuda_fp8.h>
+// That is what tcgen05.mma.kind::mxf8f6f4.block_scale computes, K = 32 a step with one scale a row and step, sums in fp32:
+// nothing is dequantized, the codes go from memory to the tensor cores by TMA alone.
+//
+// Both operands have the same form, so that one kernel serves both orientations: P (128 rows, the lanes of the accumulator) and
+// Q (NT rows, its columns), both K-major with 128-byte swizzle, 128 codes a stage.
+//   few rows of x   P = weight, Q = the rows (SWAP): the weight's bytes bound it, its tiles are spread over the SMs
+//   many rows       P = the rows, Q = weight: the tensor cores bound it
+// Few tiles for the GPU: the K range of a tile is cut over the CTAs of a cluster; each leaves its fp32 sums in shared memory
+// and adds one part of the tile over all of them, in rank order.
+//
+// Scales lie in memory as the format has them, [rows, in / 32] bytes.  The MMA reads them from tensor memory, four K steps in
+// a word, row r in lane r mod 32 of column r / 32: four warps fetch them as 16-byte pieces a row (four stages at a time, one
+// fetch ahead), write them into that order beside the stage, and tcgen05.cp takes them over, ordered before the MMAs that
+// follow it.  A stage's slot in tensor memory is written again no sooner than its shared memory, whose release waits for the
+// MMAs that read both.  Rows and blocks past the end get the scale 1 and, from TMA, codes of zero.
+//
+// Ten warps: 0..3 epilogue, 4..7 scales, 8 MMA and tensor memory, 9 loads.  Two accumulators alternate, so that the next
+// tile's MMAs run beside the epilogue; 2 x 256 columns leave no room for the scales: at NT = 256 the two share 48 columns,
+// which the epilogue takes out first.  Every wait is bounded; on expiry what is in flight is waited for, tensor memory is
+// freed, the status word is set and the tiles concerned are NaN.
+#include <atomic>
 
-#include "internal.h"
+#include "tcgen05.cuh"
+#include "../../include/ironmlx_b200_testing.h"
 
 namespace imx {
 
 namespace {
 
+using namespace tc;
+
 constexpr size_t kStatusBytes = 256;
+constexpr int kMxThreads = 352;
+constexpr int kMxK = 128;                          // codes of a row in a stage
+constexpr int kMxMaxStages = 10;
+constexpr int kMxGroups = 2;                       // groups of four K steps whose scales are in shared memory
+constexpr int kMxMaxSplits = 8;
+std::atomic<int> g_mx_spin_limit{kSpin};
 
-// NaN (0x7f, 0xff; 255) stays NaN
-__device__ __forceinline__ float e4m3_value(uint32_t c) { return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)c, __NV_E4M3))); }
-__device__ __forceinline__ float scale_value(uint32_t s) { return s == 255u ? __uint_as_float(0x7fc00000u) : ue8m0_to_f32(s); }
+template <int NT, bool SWAP, bool PAIR>
+struct Plan {
+    static constexpr int kQParts = NT > 128 ? 2 : 1;                     // 128-row parts of Q's scales
+    static constexpr int kQRows = PAIR ? NT / 2 : NT;                    // rows of Q that a CTA brings
+    static constexpr int kTile = (128 + kQRows) * kMxK;
+    static constexpr int kSf = 512 * (1 + kQParts);                      // scales of a K step
+    static constexpr int kGroup = 4 * kSf;                               // ... of the four that a row's 16 bytes hold
+    // epilogue: 32 rows x 64 outputs for each of its warps; SWAP: the tile's fp32 sums, a part from each CTA of the cluster
+    static constexpr int kOut = SWAP ? 128 * NT * 4 : 4 * 4096;
+    static constexpr int kFit = (int)((227 * 1024 - 4096 - kMxGroups * kGroup - kOut) / kTile);
+    static constexpr int kStages = kFit < kMxMaxStages ? kFit : kMxMaxStages;
+    static constexpr int kSfCols = 4 * (1 + kQParts);
+    static constexpr int kSf0 = NT == 256 ? 512 - kStages * kSfCols : 256;   // columns of the scales, a place for every stage, ...
+    static constexpr int kAcc1 = NT == 256 ? kSf0 - 256 : NT;            // ... of the second accumulator
+    static constexpr int kLag = NT == 256 ? 1 : 2;                       // a tile's MMAs wait for the drain of the kLag-th before
+    static constexpr size_t kSmem = (size_t)kStages * kTile + kMxGroups * kGroup + kOut + 2048;
+    static_assert(kSf0 + kStages * kSfCols <= 512 && (NT < 256 || kAcc1 >= 128), "tensor memory");
+};
 
-__global__ void __launch_bounds__(256)
-mxfp8_mm_kernel(const uint8_t* __restrict__ xq, const uint8_t* __restrict__ xs, int m, const uint8_t* __restrict__ wq,
-                const uint8_t* __restrict__ ws, int n_out, int in, __nv_bfloat16* __restrict__ y) {
-    const int n = blockIdx.x * 32 + (threadIdx.x & 31), row = blockIdx.y * 8 + (threadIdx.x >> 5);
-    if (n >= n_out || row >= m) return;
-    const uint8_t* a = xq + (size_t)row * in;
-    const uint8_t* b = wq + (size_t)n * in;
-    float acc = 0.f;
-    for (int g = 0; g < in / 32; ++g) {
-        float part = 0.f;
-        for (int k = 0; k < 32; k += 4) {
-            const uint32_t ca = *reinterpret_cast<const uint32_t*>(a + g * 32 + k), cb = *reinterpret_cast<const uint32_t*>(b + g * 32 + k);
+struct MxBars {
+    uint64_t full[kMxMaxStages];        // the stage's codes
+    uint64_t both[kMxMaxStages];        // pairs, in CTA 0: both CTAs have their codes and scales
+    uint64_t empty[kMxMaxStages];
+    uint64_t scales[kMxGroups];
+    uint64_t used[kMxGroups];           // the MMAs of the group have read its scales
+    uint64_t acc_full[2];
+    uint64_t drained[2];                // by accumulator, so that no wait can be two phases behind
+    uint64_t sums;                      // the parts of this CTA's columns have arrived from the cluster
+    uint64_t retired;                   // after an expired wait: the MMAs issued before it
+    uint32_t tmem_base;
+    int abort;
+};
+
+struct MxArgs {
+    const uint8_t* ps;
+    const uint8_t* qs;
+    int p_rows, q_rows, in;
+    __nv_bfloat16* y;
+    int n_out;
+    int tiles, tiles_q;
+    int stage_bytes;                    // that the loads of a stage bring
+    int y_map;                          // y leaves by TMA (rows that start on 16 bytes)
+    int piece_p, piece_q;               // bytes of scales that one load may fetch: 16, 4 or 1
+    int spin_limit;
+    int32_t* status;
+};
+struct MxMaps {
+    CUtensorMap p, q, y;
+};
+
+// kind::mxf8f6f4, e4m3 x e4m3, ue8m0 scales, M = m, N = n; K step kk of the four that share a word of scales
+__device__ __forceinline__ uint32_t mx_idesc(int m, int n, int kk) {
+    return (1u << 23) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 7) << 27) | ((uint32_t)kk << 4) | ((uint32_t)kk << 29);
+}
+template <bool PAIR>
+__device__ __forceinline__ void umma_mx(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t accumulate) {
+    if (PAIR)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "setp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+            : "memory");
+}
+// 32 x 16 bytes of shared memory -> four columns of all four 32-lane parts (of both CTAs of a pair, each from its own)
+template <bool PAIR>
+__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint32_t smem) {
+    const uint64_t desc = (uint64_t)((smem >> 4) & 0x3fffu) | (8ull << 16) | (8ull << 32) | (1ull << 46);     // no swizzle, 8 rows of 16 bytes together
+    if (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+    else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void st_shared(uint32_t addr, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+__device__ __forceinline__ void st_shared4(uint32_t addr, uint4 v) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int x, int y) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"((uint64_t)map), "r"(src), "r"(x), "r"(y) : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// The stores' source may be written again; ... and they are done.
+__device__ __forceinline__ void tma_store_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void tma_store_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+// Shared memory of this CTA into that of CTA `rank` of the cluster, counted there by the barrier at this CTA's offset `bar`.
+__device__ __forceinline__ void copy_to_peer(uint32_t dst, uint32_t src, uint32_t bytes, uint32_t bar, uint32_t rank) {
+    asm volatile(
+        "{\n\t.reg .b32 ra, rb;\n\t"
+        "mapa.shared::cluster.u32 ra, %0, %4;\n\t"
+        "mapa.shared::cluster.u32 rb, %3, %4;\n\t"
+        "cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [ra], [%1], %2, [rb];\n\t}"
+        ::"r"(dst), "r"(src), "r"(bytes), "r"(bar), "r"(rank)
+        : "memory");
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+__device__ __forceinline__ int ld_cluster_int(uint32_t addr, uint32_t rank) {
+    int v;
+    asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %1, %2;\n\tld.shared::cluster.s32 %0, [ra];\n\t}" : "=r"(v) : "r"(addr), "r"(rank) : "memory");
+    return v;
+}
+
+// Scales of a row for the four K steps of a group (16 blocks), 1 (127) past the end.
+__device__ __forceinline__ uint4 row_scales(const uint8_t* row, int group, int blocks, int piece) {
+    const int b0 = group * 16;
+    if (piece == 16) return __ldg(reinterpret_cast<const uint4*>(row + b0));
+    uint32_t v[4];
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) part = fmaf(e4m3_value((ca >> i) & 255u), e4m3_value((cb >> i) & 255u), part);
-        }
-        acc += part * (scale_value(xs[(size_t)row * (in / 32) + g]) * scale_value(ws[(size_t)n * (in / 32) + g]));
+    for (int i = 0; i < 4; ++i) {
+        const int b = b0 + 4 * i;
+        v[i] = 0x7f7f7f7fu;
+        if (b + 4 <= blocks && piece == 4) v[i] = __ldg(reinterpret_cast<const uint32_t*>(row + b));
+        else
+            for (int j = 0; j < 4 && b + j < blocks; ++j) v[i] = (v[i] & ~(255u << (8 * j))) | ((uint32_t)__ldg(row + b + j) << (8 * j));
     }
-    y[(size_t)row * n_out + n] = __float2bfloat16_rn(acc);
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+// Wait of the warp that issues the MMAs.  Its outcome must not steer the code: the compiler would take all that follows for
+// divergent and move the operands of every MMA to uniform registers, 50 cycles each.  So an expired wait sets the abort flag,
+// the later ones return at once, and what is then multiplied is never used.
+__device__ __forceinline__ void mbar_wait_on(uint32_t bar, uint32_t parity, uint32_t abort_flag, int limit) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .u32 n, f;\n\t"
+        "mov.u32 n, %3;\n"
+        "try_again:\n\t"
+        "setp.eq.u32 p, n, 0;\n\t"
+        "@p bra expired;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%0], %1;\n\t"
+        "@p bra arrived;\n\t"
+        "sub.u32 n, n, 1;\n\t"
+        "ld.volatile.shared.u32 f, [%2];\n\t"
+        "setp.eq.u32 p, f, 0;\n\t"
+        "@p bra try_again;\n"
+        "expired:\n\t"
+        "st.volatile.shared.u32 [%2], 1;\n"
+        "arrived:\n\t}"
+        ::"r"(bar), "r"(parity), "r"(abort_flag), "r"(limit)
+        : "memory");
+}
+
+// Four values of an output row, whatever of them lies below n_out.
+__device__ __forceinline__ void store4(__nv_bfloat16* y, size_t row, int n, int n_out, float4 v, bool whole) {
+    __nv_bfloat16* at = y + row * n_out + n;
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v.x, v.y), b = __floats2bfloat162_rn(v.z, v.w);
+    if (whole && n + 4 <= n_out) {
+        uint2 o;
+        o.x = *reinterpret_cast<const uint32_t*>(&a);
+        o.y = *reinterpret_cast<const uint32_t*>(&b);
+        *reinterpret_cast<uint2*>(at) = o;
+        return;
+    }
+    if (n < n_out) at[0] = a.x;
+    if (n + 1 < n_out) at[1] = a.y;
+    if (n + 2 < n_out) at[2] = b.x;
+    if (n + 3 < n_out) at[3] = b.y;
+}
+
+template <int NT, bool SWAP, bool PAIR>
+__global__ void __launch_bounds__(kMxThreads, 1)
+mxfp8_mm_kernel(const MxArgs a, const int lg_splits, const __grid_constant__ MxMaps maps) {
+    using P = Plan<NT, SWAP, PAIR>;
+    static_assert(!PAIR || !SWAP, "pairs: tiles of many rows");
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ MxBars bars;
+    unsigned char* base = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    // 1024-byte aligned: the stages, then the epilogue's, then the scales
+    const uint32_t sbase = smem_u32(base), out_base = sbase + P::kStages * P::kTile, sf_base = out_base + P::kOut;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    volatile int* abort_flag = &bars.abort;
+    const int spin = a.spin_limit;
+
+    // Warp 9 prepares the barriers, tells the others so and goes on to the loads, of which a full ring takes microseconds to
+    // issue; it needs nothing of what the others prepare.
+    if (warp == 9) {
+        for (int s = lane; s < P::kStages; s += 32) {
+            mbar_init(smem_u32(&bars.full[s]), 1);
+            mbar_init(smem_u32(&bars.both[s]), 2);
+            mbar_init(smem_u32(&bars.empty[s]), 1);
+        }
+        if (lane < 2) {
+            mbar_init(smem_u32(&bars.scales[lane]), 4);
+            mbar_init(smem_u32(&bars.used[lane]), 1);
+            mbar_init(smem_u32(&bars.acc_full[lane]), 1);
+            mbar_init(smem_u32(&bars.drained[lane]), PAIR ? 8 : 4);
+        }
+        if (lane == 2) {
+            mbar_init(smem_u32(&bars.sums), 1);
+            mbar_init(smem_u32(&bars.retired), 1);
+            bars.abort = 0;
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 8) {
+        if (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem_base)), "r"(512u) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars.tmem_base)), "r"(512u) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    if (warp == 9) asm volatile("bar.arrive 2, %0;" ::"n"(kMxThreads) : "memory");
+    else asm volatile("bar.sync 2, %0;" ::"n"(kMxThreads) : "memory");
+    // the peers' barriers are there before anyone arrives on them
+    if (PAIR || (SWAP && lg_splits > 0)) cluster_arrive();
+    if (PAIR && warp != 9) cluster_wait();
+    tc_fence_after();
+    const uint32_t tmem = warp == 9 ? 0u : bars.tmem_base;
+
+    // a cluster a tile when the K range is cut, else every CTA (pair) takes every stride-th tile whole
+    const int splits = 1 << lg_splits, rank = PAIR || (SWAP && lg_splits > 0) ? (int)cluster_ctarank() : 0;
+    const int steps = (a.in + kMxK - 1) / kMxK, lg_cluster = PAIR ? 1 : lg_splits;
+    const int k0 = PAIR ? 0 : (steps * rank) >> lg_splits, k1 = PAIR ? steps : (steps * (rank + 1)) >> lg_splits;
+    const int first = (int)blockIdx.x >> lg_cluster, stride = (int)gridDim.x >> lg_cluster;
+    constexpr int kPRows = PAIR ? 256 : 128;                 // rows of P in a tile
+    const int p_own = PAIR ? rank * 128 : 0;                 // ... of which this CTA's start here
+    auto place = [&](int t, int& p0, int& q0) {              // of a tile (in P, this CTA's half)
+        const int p = a.tiles_q == 1 ? t : (int)((unsigned)t / (unsigned)a.tiles_q);
+        p0 = p * kPRows + p_own;
+        q0 = (t - p * a.tiles_q) * NT;
+    };
+    // K range cut: columns of the tile that CTA r of the cluster adds (none past the last row of Q)
+    const int lg_own = 31 - __clz(NT) - lg_splits;
+    int p_first, q_first;
+    place(first, p_first, q_first);
+    auto sum_cols = [&](int r) { return max(0, min(1 << lg_own, a.q_rows - q_first - (r << lg_own))); };
+    bool met = false;                                        // this warp has waited for the cluster's start
+    int copied = 0;                                          // stages the loader has started
+
+    if (warp == 9) {
+        int s = 0;
+        uint32_t ph = 0;
+        bool ok = true;
+        for (int t = first; t < a.tiles && ok; t += stride) {
+            int p0, q0;
+            place(t, p0, q0);
+            for (int k = k0; k < k1; ++k) {
+                if (!mbar_wait(smem_u32(&bars.empty[s]), ph ^ 1u, abort_flag, spin)) {
+                    ok = false;
+                    break;
+                }
+                if (lane == 0) {
+                    const uint32_t st = sbase + (uint32_t)s * P::kTile, bar = smem_u32(&bars.full[s]);
+                    mbar_expect_tx(bar, (uint32_t)a.stage_bytes);
+                    tma_load_2d(st, &maps.p, k * kMxK, p0, bar);
+                    tma_load_2d(st + 128 * kMxK, &maps.q, k * kMxK, q0 + (PAIR ? rank * P::kQRows : 0), bar);
+                }
+                __syncwarp();
+                ++copied;
+                if (++s == P::kStages) {
+                    s = 0;
+                    ph ^= 1u;
+                }
+            }
+        }
+        if (PAIR) cluster_wait();
+    } else if (warp == 10) {
+        // pairs: tells CTA 0, which issues the MMAs, what has arrived here
+        int s = 0, g = 0;
+        uint32_t ph = 0, g_ph = 0;
+        bool ok = true;
+        for (int t = PAIR ? first : a.tiles; t < a.tiles && ok; t += stride)
+            for (int k = k0; k < k1; ++k) {
+                if (!mbar_wait(smem_u32(&bars.full[s]), ph, abort_flag, spin) ||
+                    ((k == k0 || (k & 3) == 0) && !mbar_wait(smem_u32(&bars.scales[g]), g_ph, abort_flag, spin))) {
+                    ok = false;
+                    break;
+                }
+                if (lane == 0) mbar_arrive_cta0(smem_u32(&bars.both[s]));
+                __syncwarp();
+                if ((k & 3) == 3 || k == k1 - 1) {
+                    g_ph ^= (uint32_t)(g == kMxGroups - 1);
+                    g = g == kMxGroups - 1 ? 0 : g + 1;
+                }
+                if (++s == P::kStages) {
+                    s = 0;
+                    ph ^= 1u;
+                }
+            }
+    } else if (warp == 8 && (!PAIR || rank == 0)) {
+        const uint32_t flag = smem_u32(&bars.abort);
+        int s = 0, g = 0, done = 0;
+        uint32_t ph = 0, g_ph = 0;
+        for (int t = first; t < a.tiles; t += stride, ++done) {
+            const int before = done - P::kLag;               // the tile whose drain makes room for this one
+            if (before >= 0) mbar_wait_on(smem_u32(&bars.drained[before & 1]), (uint32_t)(before >> 1) & 1u, flag, spin);
+            tc_fence_after();
+            const uint32_t acc = tmem + ((done & 1) ? (uint32_t)P::kAcc1 : 0u);
+            for (int k = k0; k < k1; ++k) {
+                const bool last = (k & 3) == 3 || k == k1 - 1;           // of the group
+                if (PAIR) {
+                    mbar_wait_on(smem_u32(&bars.both[s]), ph, flag, spin);
+                } else {
+                    mbar_wait_on(smem_u32(&bars.full[s]), ph, flag, spin);
+                    if (k == k0 || (k & 3) == 0) mbar_wait_on(smem_u32(&bars.scales[g]), g_ph, flag, spin);
+                }
+                tc_fence_after();
+                const uint32_t st = sbase + (uint32_t)s * P::kTile, sf = sf_base + (uint32_t)(g * P::kGroup + (k & 3) * P::kSf);
+                const uint32_t sp = tmem + (uint32_t)(P::kSf0 + s * P::kSfCols), sq = sp + 4;
+                if (elect_one()) {
+                    tmem_copy_scales<PAIR>(sp, sf);
+#pragma unroll
+                    for (int h = 0; h < P::kQParts; ++h) tmem_copy_scales<PAIR>(sq + 4 * h, sf + 512 * (1 + h));
+#pragma unroll
+                    for (int kk = 0; kk < 4; ++kk)
+                        umma_mx<PAIR>(acc, smem_desc(st) + 2 * kk, smem_desc(st + 128 * kMxK) + 2 * kk, mx_idesc(kPRows, NT, kk), sp, sq,
+                                      (k > k0 || kk > 0) ? 1u : 0u);
+                    if (PAIR) umma_commit_pair(smem_u32(&bars.empty[s]));
+                    else umma_commit(smem_u32(&bars.empty[s]));
+                    if (last) {
+                        if (PAIR) umma_commit_pair(smem_u32(&bars.used[g]));
+                        else umma_commit(smem_u32(&bars.used[g]));
+                    }
+                    if (k == k1 - 1) {
+                        if (PAIR) umma_commit_pair(smem_u32(&bars.acc_full[done & 1]));
+                        else umma_commit(smem_u32(&bars.acc_full[done & 1]));
+                    }
+                }
+                __syncwarp();
+                if (++s == P::kStages) {
+                    s = 0;
+                    ph ^= 1u;
+                }
+                if (last) {
+                    g_ph ^= (uint32_t)(g == kMxGroups - 1);
+                    g = g == kMxGroups - 1 ? 0 : g + 1;
+                }
+            }
+        }
+    } else if (warp == 8) {
+    } else if (warp >= 4) {
+        // Scales: a row of P and one or two of Q per thread (rows to threads so that a warp's 32 words fill 128 bytes of the
+        // order above), a group of four K steps at a time, the next one on its way, a tile ahead into L2
+        const int sf_row = (lane >> 3) * 32 + (warp & 3) * 8 + (lane & 7), blocks = a.in / 32, g0 = k0 >> 2, groups = ((k1 - 1) >> 2) - g0 + 1;
+        const uint32_t at = sf_base + (uint32_t)((sf_row & 31) * 16 + (sf_row >> 5) * 4);
+        const uint8_t* row[1 + P::kQParts];
+        auto rows_of = [&](int t) {
+            int p0, q0;
+            place(t, p0, q0);
+            row[0] = p0 + sf_row < a.p_rows ? a.ps + (size_t)(p0 + sf_row) * blocks : nullptr;
+#pragma unroll
+            for (int h = 0; h < P::kQParts; ++h) {
+                const int r = h * 128 + sf_row;
+                row[1 + h] = r < NT && q0 + r < a.q_rows ? a.qs + (size_t)(q0 + r) * blocks : nullptr;
+            }
+        };
+        auto fetch = [&](int i, uint4 (&v)[1 + P::kQParts]) {
+#pragma unroll
+            for (int j = 0; j < 1 + P::kQParts; ++j)
+                v[j] = row[j] != nullptr ? row_scales(row[j], g0 + i, blocks, j == 0 ? a.piece_p : a.piece_q) : make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
+        };
+        auto prefetch = [&](int from) {
+            for (int b = from; b < min(k1 * 4, blocks); b += 32)
+#pragma unroll
+                for (int j = 0; j < 1 + P::kQParts; ++j)
+                    if (row[j] != nullptr) asm volatile("prefetch.global.L2 [%0];" ::"l"(row[j] + b));
+        };
+        uint4 v[1 + P::kQParts], next[1 + P::kQParts];
+        rows_of(first);
+        fetch(0, next);
+        prefetch(g0 * 16 + 32);
+        int g = 0;
+        uint32_t g_ph = 0;
+        bool ok = true;
+        for (int t = first; t < a.tiles && ok; t += stride) {
+            for (int i = 0; i < groups; ++i) {
+#pragma unroll
+                for (int j = 0; j < 1 + P::kQParts; ++j) v[j] = next[j];
+                if (i + 1 < groups) {
+                    fetch(i + 1, next);
+                } else if (t + stride < a.tiles) {
+                    rows_of(t + stride);
+                    fetch(0, next);
+                    prefetch(g0 * 16 + 32);
+                }
+                if (!mbar_wait(smem_u32(&bars.used[g]), g_ph ^ 1u, abort_flag, spin)) {
+                    ok = false;
+                    break;
+                }
+#pragma unroll
+                for (int j = 0; j < 1 + P::kQParts; ++j) {
+                    const uint32_t to = at + (uint32_t)(g * P::kGroup + j * 512);
+                    st_shared(to, v[j].x);
+                    st_shared(to + P::kSf, v[j].y);
+                    st_shared(to + 2 * P::kSf, v[j].z);
+                    st_shared(to + 3 * P::kSf, v[j].w);
+                }
+                fence_async_proxy();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(smem_u32(&bars.scales[g]));
+                if (++g == kMxGroups) {
+                    g = 0;
+                    g_ph ^= 1u;
+                }
+            }
+        }
+    } else {
+        const int l = warp * 32 + lane;                      // lane of the accumulator
+        const uint32_t quarter = (uint32_t)(warp * 32) << 16;
+        constexpr int kChunks = NT >= 32 ? NT / 32 : 1;
+        constexpr int kPairs = (kChunks + 1) / 2;
+        const uint32_t out_own = out_base + (uint32_t)(warp * 4096), out_row = out_own + (uint32_t)(lane * 128);
+        int done = 0;
+        for (int t = first; t < a.tiles; t += stride, ++done) {
+            int p0, q0;
+            place(t, p0, q0);
+            const int buf = done & 1;
+            if (!mbar_wait(smem_u32(&bars.acc_full[buf]), (uint32_t)(done >> 1) & 1u, abort_flag, spin)) break;
+            tc_fence_after();
+            const uint32_t acc = tmem + quarter + (buf ? (uint32_t)P::kAcc1 : 0u);
+            for (int pr = 0; pr < kPairs; ++pr) {
+                // the columns that the two accumulators share come first
+                const int c0 = NT == 256 && buf == 0 ? (2 * pr + 4) & 7 : 2 * pr;
+                uint32_t v[2][32];
+                tmem_ld32(acc + (uint32_t)(c0 * 32), v[0]);
+                if (kChunks > 1) tmem_ld32(acc + (uint32_t)(c0 * 32 + 32), v[1]);
+                if (pr == (NT == 256 ? 1 : kPairs - 1)) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (PAIR) mbar_arrive_cta0(smem_u32(&bars.drained[buf]));
+                        else mbar_arrive(smem_u32(&bars.drained[buf]));
+                    }
+                }
+#pragma unroll
+                for (int h = 0; h < (kChunks > 1 ? 2 : 1); ++h) {
+                    const int c = (c0 + h) * 32;
+                    if (SWAP && lg_splits > 0) {
+                        // into the stages' place, [column][lane]
+                        float* part = reinterpret_cast<float*>(base) + c * 128 + l;
+#pragma unroll
+                        for (int i = 0; i < (NT < 32 ? NT : 32); ++i)
+                            if (q0 + c + i < a.q_rows) part[i * 128] = __uint_as_float(v[h][i]);
+                    } else if (SWAP) {
+                        if (p0 + l < a.n_out) {
+                            __nv_bfloat16* at = a.y + (size_t)(q0 + c) * a.n_out + p0 + l;
+#pragma unroll
+                            for (int i = 0; i < (NT < 32 ? NT : 32); ++i)
+                                if (q0 + c + i < a.q_rows) at[(size_t)i * a.n_out] = __float2bfloat16_rn(__uint_as_float(v[h][i]));
+                        }
+                    } else if (a.y_map) {
+                        // 32 rows x 64 columns a warp, 128-byte swizzle
+                        if (h == 0) {
+                            if (lane == 0) tma_store_read();
+                            __syncwarp();
+                        }
+#pragma unroll
+                        for (int i = 0; i < 32; i += 8) {
+                            uint32_t o[4];
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) {
+                                const __nv_bfloat162 b = __floats2bfloat162_rn(__uint_as_float(v[h][i + 2 * j]), __uint_as_float(v[h][i + 2 * j + 1]));
+                                o[j] = *reinterpret_cast<const uint32_t*>(&b);
+                            }
+                            st_shared4(out_row + (uint32_t)((((h * 4 + i / 8) ^ lane) & 7) * 16), make_uint4(o[0], o[1], o[2], o[3]));
+                        }
+                        if (h == 1) {
+                            fence_async_proxy();
+                            __syncwarp();
+                            if (lane == 0 && p0 + warp * 32 < a.p_rows && q0 + c0 * 32 < a.n_out) tma_store_2d(&maps.y, out_own, q0 + c0 * 32, p0 + warp * 32);
+                        }
+                    } else if (p0 + l < a.p_rows) {
+                        __nv_bfloat16* at = a.y + (size_t)(p0 + l) * a.n_out;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i)
+                            if (q0 + c + i < a.n_out) at[q0 + c + i] = __float2bfloat16_rn(__uint_as_float(v[h][i]));
+                    }
+                }
+            }
+        }
+        if (!SWAP && lane == 0) tma_store_done();
+        if (SWAP && lg_splits > 0) {
+            // each CTA's columns to it, [sender][column][lane]; it adds them
+            fence_async_proxy();
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            cluster_wait();
+            met = true;
+            if (warp == 0 && elect_one()) {
+                mbar_expect_tx(smem_u32(&bars.sums), (uint32_t)((sum_cols(rank) * 512) << lg_splits));
+                for (int r = 0; r < splits && done > 0 && *abort_flag == 0; ++r)
+                    if (sum_cols(r) > 0)
+                        copy_to_peer(out_base + (uint32_t)(rank << lg_own) * 512u, sbase + (uint32_t)(r << lg_own) * 512u, (uint32_t)sum_cols(r) * 512u,
+                                     smem_u32(&bars.sums), (uint32_t)r);
+            }
+            __syncwarp();
+        }
+        if (SWAP && lg_splits > 0 && mbar_wait(smem_u32(&bars.sums), 0u, abort_flag, spin)) {
+            const int p0 = p_first, q0 = q_first + (rank << lg_own), cols = sum_cols(rank);
+            const float4* parts = reinterpret_cast<const float4*>(base + P::kStages * P::kTile);
+            const bool whole = ((uintptr_t)a.y % 8) == 0 && a.n_out % 4 == 0;
+            for (int i = tid; i < cols * 32; i += 128) {
+                const int col = i >> 5, n = (i & 31) * 4;
+                if (p0 + n >= a.n_out) continue;
+                float4 sum = parts[col * 32 + (i & 31)];
+                for (int c = 1; c < splits; ++c) {
+                    const float4 v = parts[((c << lg_own) + col) * 32 + (i & 31)];
+                    sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
+                }
+                store4(a.y, (size_t)(q0 + col), p0 + n, a.n_out, sum, whole);
+            }
+        }
+    }
+    __syncthreads();
+    const bool gave_up = bars.abort != 0;
+    if (gave_up) {
+        if (warp == 8 && (!PAIR || rank == 0)) {
+            if (elect_one()) {
+                if (PAIR) umma_commit_own_pair(smem_u32(&bars.retired));
+                else umma_commit(smem_u32(&bars.retired));
+            }
+            __syncwarp();
+            mbar_drain(smem_u32(&bars.retired), 0u);
+        } else if (warp == 9) {
+            for (int k = max(0, copied - P::kStages); k < copied; ++k)
+                mbar_drain(smem_u32(&bars.full[k % P::kStages]), (uint32_t)(k / P::kStages) & 1u);
+        }
+        __syncthreads();
+    }
+    if (PAIR) cluster_sync();                                // neither CTA's arrivals and MMAs outlive the other
+    if (warp == 8) {
+        if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    }
+    bool bad = gave_up;
+    if (PAIR) {
+        bad = bad || ld_cluster_int(smem_u32(&bars.abort), (uint32_t)(rank ^ 1)) != 0;
+        cluster_sync();
+    }
+    if (SWAP && lg_splits > 0) {
+        if (!met) cluster_wait();
+        // nobody leaves while another CTA may copy into its shared memory or out of it
+        asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+        cluster_wait();
+    }
+    if (bad) {
+        if (tid == 0) atomicExch(a.status, 4);
+        for (int t = first; t < a.tiles; t += stride) {
+            int p0, q0;
+            place(t, p0, q0);
+            for (int i = tid; i < 128 * NT; i += kMxThreads) {
+                const int p = p0 + i / NT, q = q0 + i % NT;
+                if (p < a.p_rows && q < a.q_rows) a.y[SWAP ? (size_t)q * a.n_out + p : (size_t)p * a.n_out + q] = __float2bfloat16_rn(__uint_as_float(0x7fc00000u));
+            }
+        }
+    }
+}
+
+template <int NT, bool SWAP, bool PAIR = false>
+int set_up() {
+    IMX_CHECK_CUDA(cudaFuncSetAttribute(mxfp8_mm_kernel<NT, SWAP, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Plan<NT, SWAP, PAIR>::kSmem));
+    return IMX_OK;
+}
+
+struct Call {
+    const uint8_t *x, *xs, *w, *ws;
+    int m, n_out, in;
+    __nv_bfloat16* y;
+    int32_t* status;
+    int sms;
+    cudaStream_t stream;
+};
+
+template <int NT, bool SWAP, bool PAIR = false>
+int launch(const Call& c, int lg_splits) {
+    const int splits = 1 << lg_splits;
+    MxArgs a = {};
+    a.ps = SWAP ? c.ws : c.xs;
+    a.qs = SWAP ? c.xs : c.ws;
+    a.p_rows = SWAP ? c.n_out : c.m;
+    a.q_rows = SWAP ? c.m : c.n_out;
+    a.in = c.in;
+    a.y = c.y;
+    a.n_out = c.n_out;
+    a.tiles_q = ceil_div(a.q_rows, NT);
+    const long tiles = (long)ceil_div(a.p_rows, PAIR ? 256 : 128) * a.tiles_q;
+    IMX_REQUIRE(tiles <= 0x7fffffffL / kMxMaxSplits, "mxfp8_matmul: too many outputs");
+    a.tiles = (int)tiles;
+    auto piece = [&](const uint8_t* s) { return (uintptr_t)s % 16 == 0 && c.in % 512 == 0 ? 16 : ((uintptr_t)s % 4 == 0 && c.in % 128 == 0 ? 4 : 1); };
+    a.piece_p = piece(a.ps);
+    a.piece_q = piece(a.qs);
+    a.spin_limit = g_mx_spin_limit.load();
+    a.status = c.status;
+    // rows of x that do not exist are not brought: what the lanes hold in their place reaches no output
+    const int p_box = !SWAP && c.m < 128 ? (c.m + 7) & ~7 : 128;
+    a.stage_bytes = (p_box + Plan<NT, SWAP, PAIR>::kQRows) * kMxK;
+    MxMaps maps;
+    IMX_TRY(encode_tensor_map_2d(SWAP ? c.w : c.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (size_t)a.p_rows, (size_t)c.in, (size_t)c.in, kMxK, p_box, 128, true, &maps.p));
+    IMX_TRY(encode_tensor_map_2d(SWAP ? c.x : c.w, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (size_t)a.q_rows, (size_t)c.in, (size_t)c.in, kMxK, Plan<NT, SWAP, PAIR>::kQRows, 128,
+                                 true, &maps.q));
+    a.y_map = !SWAP && (uintptr_t)c.y % 16 == 0 && c.n_out % 8 == 0;
+    if (a.y_map)
+        IMX_TRY(encode_tensor_map_2d(c.y, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (size_t)c.m, (size_t)c.n_out, (size_t)c.n_out * 2, 64, 32, 128, true, &maps.y));
+    cudaLaunchConfig_t cfg = {};
+    const int cluster = PAIR ? 2 : splits, most = c.sms / 2 * (PAIR ? 1 : 2);
+    cfg.gridDim = dim3((unsigned)(lg_splits > 0 ? a.tiles * splits : (a.tiles < most ? a.tiles : most) * cluster));
+    cfg.blockDim = dim3(kMxThreads);
+    cfg.dynamicSmemBytes = Plan<NT, SWAP, PAIR>::kSmem;
+    cfg.stream = c.stream;
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    IMX_CHECK_CUDA(cudaLaunchKernelEx(&cfg, mxfp8_mm_kernel<NT, SWAP, PAIR>, a, lg_splits, maps)); IMX_LAUNCHED();
+    return IMX_OK;
+}
+
+int run(const Call& c) {
+    const int steps = ceil_div(c.in, kMxK);
+    int nt = c.m <= 16 ? 16 : (c.m <= 32 ? 32 : (c.m <= 64 ? 64 : 128));
+    bool swap = c.m <= 128, pair = false;
+    if (!swap) nt = (long)ceil_div(c.m, 128) * ceil_div(c.n_out, 256) >= c.sms ? 256 : 128;
+    if (!swap && nt == 256) pair = true;
+    long tiles = swap ? (long)ceil_div(c.n_out, 128) * ceil_div(c.m, nt) : (long)ceil_div(c.m, 128) * ceil_div(c.n_out, nt);
+    int splits = 1;
+    while (swap && splits < kMxMaxSplits && tiles * splits * 2 <= c.sms && steps >= splits * 4) splits *= 2;
+    if (const char* e = getenv("IMX_MX")) {
+        int s = 0;
+        sscanf(e, "%d,%d,%d", &s, &nt, &splits);
+        swap = s == 1;
+        pair = s == 2;
+        if (!swap) splits = 1;
+    }
+    int lg = 0;
+    while (1 << lg < splits) ++lg;
+    if (pair) return nt == 256 ? launch<256, false, true>(c, 0) : launch<128, false, true>(c, 0);
+    if (swap) return nt == 16 ? launch<16, true>(c, lg) : (nt == 32 ? launch<32, true>(c, lg) : (nt == 64 ? launch<64, true>(c, lg) : launch<128, true>(c, lg)));
+    return nt == 256 ? launch<256, false>(c, 0) : (nt == 64 ? launch<64, false>(c, 0) : launch<128, false>(c, 0));
 }
 
 }  // namespace
+
+// Test hook (include/ironmlx_b200_testing.h).
+void testing_mxfp8_give_up(int on) { g_mx_spin_limit.store(on ? 0 : kSpin); }
 
 }  // namespace imx
 
 using namespace imx;
 
 extern "C" {
+
+void imx_testing_mxfp8_give_up(int on) { testing_mxfp8_give_up(on); }
 
 int imx_mxfp8_matmul_scratch_bytes(int m, int n_out, int in, size_t* bytes) {
     IMX_REQUIRE(bytes != nullptr && m >= 0 && n_out > 0 && in > 0 && in % 32 == 0, "mxfp8_matmul_scratch_bytes: bad arguments");
@@ -65,11 +713,22 @@ int imx_mxfp8_matmul(const void* x_q, const void* x_scales, int m, const imx_qte
     const size_t yb = (size_t)m * n_out * 2, xb = (size_t)m * in, wb = (size_t)n_out * in;
     IMX_REQUIRE(!overlap(y, yb, x_q, xb) && !overlap(y, yb, x_scales, xb / 32) && !overlap(y, yb, w->w, wb) &&
                 !overlap(y, yb, w->scales, wb / 32) && !overlap(y, yb, scratch, kStatusBytes), "mxfp8_matmul: y overlaps another array");
-    mxfp8_mm_kernel<<<dim3((unsigned)ceil_div(n_out, 32), (unsigned)ceil_div(m, 8)), 256, 0, (cudaStream_t)stream>>>(
-        (const uint8_t*)x_q, (const uint8_t*)x_scales, m, (const uint8_t*)w->w, (const uint8_t*)w->scales, n_out, in,
-        (__nv_bfloat16*)y); IMX_LAUNCHED();
-    IMX_CHECK_CUDA(cudaGetLastError());
-    return IMX_OK;
+    DeviceInfo di;
+    IMX_TRY(current_device(&di));
+    if (device_needs_setup(di.ordinal, kSetupMxfp8)) {       // once per device
+        IMX_TRY((set_up<16, true>()));
+        IMX_TRY((set_up<32, true>()));
+        IMX_TRY((set_up<64, true>()));
+        IMX_TRY((set_up<128, true>()));
+        IMX_TRY((set_up<64, false>()));
+        IMX_TRY((set_up<128, false>()));
+        IMX_TRY((set_up<256, false>()));
+        IMX_TRY((set_up<128, false, true>()));
+        IMX_TRY((set_up<256, false, true>()));
+        device_mark_setup(di.ordinal, kSetupMxfp8);
+    }
+    return run(Call{(const uint8_t*)x_q, (const uint8_t*)x_scales, (const uint8_t*)w->w, (const uint8_t*)w->scales, m, n_out, in,
+                    (__nv_bfloat16*)y, (int32_t*)scratch, di.sms, (cudaStream_t)stream});
 }
 
 }  // extern "C"

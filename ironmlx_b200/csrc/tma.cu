@@ -66,9 +66,8 @@ void device_mark_setup(int ordinal, int family) {
     g_setup[ordinal] |= 1u << family;
 }
 
-int make_tensor_map_2d(const void* base, CUtensorMapDataType dt, size_t esize, size_t rows, size_t cols,
-                       size_t ld_bytes, int box_cols, int box_rows, bool swizzle128, CUtensorMap* out,
-                       bool promote256, int swizzle_bytes) {
+int encode_tensor_map_2d(const void* base, CUtensorMapDataType dt, size_t esize, size_t rows, size_t cols, size_t ld_bytes,
+                         int box_cols, int box_rows, int swizzle, bool promote256, CUtensorMap* out) {
     static EncodeTiledFn fn = nullptr;
     static std::mutex fn_mu;
     {
@@ -83,6 +82,23 @@ int make_tensor_map_2d(const void* base, CUtensorMapDataType dt, size_t esize, s
     }
     IMX_REQUIRE(((uintptr_t)base % 16) == 0 && ld_bytes % 16 == 0 && (box_cols * esize) % 16 == 0,
                 "tensor map: a matrix is not 16-byte aligned (base %p, row pitch %zu)", base, ld_bytes);
+    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)ld_bytes};
+    const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
+    const cuuint32_t estr[2] = {1, 1};
+    const CUtensorMapSwizzle mode = swizzle == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
+                                    : (swizzle == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                     : (swizzle == 32 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_NONE));
+    const CUresult r = fn(out, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, mode,
+                          promote256 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    IMX_REQUIRE(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with %d", (int)r);
+    return IMX_OK;
+}
+
+int make_tensor_map_2d(const void* base, CUtensorMapDataType dt, size_t esize, size_t rows, size_t cols,
+                       size_t ld_bytes, int box_cols, int box_rows, bool swizzle128, CUtensorMap* out,
+                       bool promote256, int swizzle_bytes) {
     const int swz = swizzle128 ? 128 : swizzle_bytes;
     // A map depends on nothing but its arguments (it holds the address, not the contents): calls with the same
     // weights and workspace reuse the encoding instead of paying the driver call again.
@@ -98,17 +114,7 @@ int make_tensor_map_2d(const void* base, CUtensorMapDataType dt, size_t esize, s
             *out = cache[i].map;
             return IMX_OK;
         }
-    const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-    const cuuint64_t strides[1] = {(cuuint64_t)ld_bytes};
-    const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
-    const cuuint32_t estr[2] = {1, 1};
-    const CUtensorMapSwizzle mode = swz == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
-                                    : (swz == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
-                                                 : (swz == 32 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_NONE));
-    const CUresult r = fn(out, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, mode,
-                          promote256 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    IMX_REQUIRE(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with %d", (int)r);
+    IMX_TRY(encode_tensor_map_2d(base, dt, esize, rows, cols, ld_bytes, box_cols, box_rows, swz, promote256, out));
     MapEntry& e = cache[next];
     next = (next + 1) % kMapCache;
     e.key = key;

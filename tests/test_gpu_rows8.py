@@ -260,3 +260,25 @@ def test_layers(cuda):
     q4 = ops.quantize(torch.randn(256, 512, generator=g, device="cuda"))
     with pytest.raises(_lib.IronMLXError):
         nn.QuantizedLinear.new(*q4, 64, 4).forward_rows(rows)
+
+
+@pytest.mark.parametrize("m,n_in,n_out", [(8, 2048, 256), (600, 512, 1024), (128, 64, 40000)])
+def test_expired_wait_gives_nan_and_a_status(cuda, m, n_in, n_out):
+    """With every wait giving up at once nothing is copied or multiplied: outputs are NaN, the status is reported once, the
+    next call is right again."""
+    g = gen(14)
+    rows, w = mx(g, m, n_in), mx(g, n_out, n_in, 0.02)
+    want = ops.mxfp8_matmul(rows, *w)
+    ops.check_status(cuda)
+    _lib.lib().imx_testing_mxfp8_give_up(1)
+    try:
+        y = ops.mxfp8_matmul(rows, *w)
+        torch.cuda.synchronize()
+    finally:
+        _lib.lib().imx_testing_mxfp8_give_up(0)
+    assert y.isnan().all()
+    with pytest.raises(_lib.IronMLXError) as e:
+        ops.check_status(cuda)
+    assert e.value.code == _lib.ERR_DEVICE
+    ops.check_status(cuda)
+    assert torch.equal(ops.mxfp8_matmul(rows, *w), want)
