@@ -164,14 +164,8 @@ struct LowRankAdapters {
         const int in = (int)a.dim(2), n_out = (int)b.dim(1), rows = (int)(x.size() / in);
         if (x.dim(-1) != in || y.dim(-1) != n_out || ids.size() != rows)
             throw Error(IMX_ERR_INVALID, "LowRankAdapters: shapes do not match the adapters");
-        size_t need = 0;
-        check(imx_low_rank_scratch_bytes(rows, in, n_out, ad.count, ad.rank, &need));
-        void* ws = scratch_.get(need);
-        check(imx_low_rank_add(y.ptr, x.ptr, rows, in, &ad, (const int32_t*)ids.ptr, n_out, y.ptr, ws, scratch_.bytes(), stream));
+        check(imx_low_rank_add(y.ptr, x.ptr, rows, in, &ad, (const int32_t*)ids.ptr, n_out, y.ptr, stream));
     }
-
-private:
-    mutable Scratch scratch_;
 };
 
 // Dense bf16 projection x . W^T (+ b) (mlx/src/nn/linear.rs:129-177); inside the block it is only a holder of

@@ -107,8 +107,7 @@ SIGNATURES = {
     "imx_linear": (_i, [_vp, _i, _i, _vp, _i, _vp, _vp, _vp]),
     "imx_mxfp8_matmul_scratch_bytes": (_i, [_i, _i, _i, C.POINTER(_sz)]),
     "imx_mxfp8_matmul": (_i, [_vp, _vp, _i, C.POINTER(QTensor), _i, _i, _vp, _vp, _sz, _vp]),
-    "imx_low_rank_scratch_bytes": (_i, [_i, _i, _i, _i, _i, C.POINTER(_sz)]),
-    "imx_low_rank_add": (_i, [_vp, _vp, _i, _i, C.POINTER(Adapters), _vp, _i, _vp, _vp, _sz, _vp]),
+    "imx_low_rank_add": (_i, [_vp, _vp, _i, _i, C.POINTER(Adapters), _vp, _i, _vp, _vp]),
     "imx_quantize": (_i, [_vp, _i, _i, _i, _i, _i, _f, _vp, _vp, _vp, _vp]),
     "imx_gather_qmm": (_i, [_vp, _vp, C.POINTER(QTensor), _vp, _i, _i, _i, _i, _i, _i, _vp, _vp]),
 }

@@ -335,10 +335,6 @@ def low_rank_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
         if out is None:
             out = torch.empty_like(y)
         ad = _lib.Adapters(a.data_ptr(), b.data_ptr(), _ptr(scale), count, rank)
-        nb = C.c_size_t(0)
-        check(lib().imx_low_rank_scratch_bytes(rows, in_dim, n_out, count, rank, C.byref(nb)))
-        # a scratch of its own for every call: calls on several streams, and captured ones, do not share it
-        ws = torch.empty(nb.value, dtype=torch.uint8, device=x.device)
         check(lib().imx_low_rank_add(y.data_ptr(), x.data_ptr(), rows, in_dim, C.byref(ad), ids.data_ptr(), n_out,
-                                     out.data_ptr(), ws.data_ptr(), nb.value, torch.cuda.current_stream().cuda_stream))
+                                     out.data_ptr(), torch.cuda.current_stream().cuda_stream))
     return out

@@ -53,13 +53,9 @@ def test_mxfp8_matmul_refuses_scratch(kw):
     refused(product(**kw), b"scratch", _lib.ERR_WORKSPACE)
 
 
-def low_rank(y=A, x=B, n=4, n_in=64, a=D, b=D + 0x1000000, scale=None, count=3, rank=8, ids=E, n_out=64, out=F, scratch=G, nb=None):
-    lib = _lib.lib()
-    need = C.c_size_t(0)
-    if nb is None and n > 0 and n_in > 0 and n_out > 0 and count > 0 and 0 < rank <= 256:
-        assert lib.imx_low_rank_scratch_bytes(n, n_in, n_out, count, rank, C.byref(need)) == 0
+def low_rank(y=A, x=B, n=4, n_in=64, a=D, b=D + 0x1000000, scale=None, count=3, rank=8, ids=E, n_out=64, out=F):
     ad = _lib.Adapters(a, b, scale, count, rank)
-    return lib.imx_low_rank_add(y, x, n, n_in, C.byref(ad), ids, n_out, out, scratch, need.value if nb is None else nb, None)
+    return _lib.lib().imx_low_rank_add(y, x, n, n_in, C.byref(ad), ids, n_out, out, None)
 
 
 @pytest.mark.parametrize("kw,needle", [
@@ -76,11 +72,6 @@ def test_low_rank_add_refuses(kw, needle):
     refused(low_rank(**kw), needle)
 
 
-@pytest.mark.parametrize("kw", [dict(scratch=None), dict(scratch=G + 64), dict(nb=0)])
-def test_low_rank_add_refuses_scratch(kw):
-    refused(low_rank(**kw), b"scratch", _lib.ERR_WORKSPACE)
-
-
 def test_no_rows_are_no_work():
     """Nothing is read or launched for an empty batch, whose tensors have no address."""
     assert norm(n=0, x=None, residual=None, h=None, y=None, q=None, s=None) == 0
@@ -94,8 +85,6 @@ def test_scratch_sizes():
     assert lib.imx_mxfp8_matmul_scratch_bytes(5, 100, 64, C.byref(nb)) == 0 and nb.value >= 256
     refused(lib.imx_mxfp8_matmul_scratch_bytes(5, 100, 60, C.byref(nb)), b"bad arguments")
     refused(lib.imx_mxfp8_matmul_scratch_bytes(5, 100, 64, None), b"bad arguments")
-    refused(lib.imx_low_rank_scratch_bytes(5, 64, 64, 0, 8, C.byref(nb)), b"bad arguments")
-    refused(lib.imx_low_rank_scratch_bytes(5, 64, 64, 1, 512, C.byref(nb)), b"bad arguments")
 
 
 def test_python_layer_refuses_host_tensors_and_other_formats():
