@@ -70,7 +70,6 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&v)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ uint4 ldg16(const __nv_bfloat16* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
 // v = hi + lo to 16 bits (what is not finite stays in hi)
 __device__ __forceinline__ void split2(float v, __nv_bfloat16& hi, __nv_bfloat16& lo) {
     hi = __float2bfloat16_rn(v);
@@ -79,73 +78,109 @@ __device__ __forceinline__ void split2(float v, __nv_bfloat16& hi, __nv_bfloat16
 }
 __device__ __forceinline__ uint32_t pack2(__nv_bfloat16 a, __nv_bfloat16 b) { return (uint32_t)__bfloat16_as_ushort(a) | (uint32_t)__bfloat16_as_ushort(b) << 16; }
 
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
+    const int n = there ? 16 : 0;             // the rest is filled with zeros
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
 // ── few rows ────────────────────────────────────────────────────────────────
 constexpr int kFewRows = 128;                 // rows of a launch
 constexpr int kFewUnit = 16;
-constexpr int kFewCtas = 8;                   // CTAs of a cluster
+// Each lane has a ring of 16-byte pieces in shared memory for what it alone will read, filled by cp.async: in registers there
+// is room for two or three pieces on their way (2.6 TB/s).  RB: blocks of 32 values of the rank, 1, 2, 4 or 8.
+__host__ __device__ constexpr int ring_pieces(int rb) { return rb == 8 ? 18 : (rb == 4 ? 15 : 12); }
+// Dynamic shared memory: the rings, this CTA's sums [row][rank], and in one place the warps' parts of them, [k part][row][rank]
+// (8 parts of ranks up to 32, 4 up to 64, 2 up to 128), and afterwards the low-rank rows as hi and lo.
+struct FewPlan {
+    int pitch, sums_at, part_at, lo_at, bytes;       // pitch: values of a row of hi or lo
+    __host__ __device__ FewPlan(int rank, int rb) {
+        pitch = rb * 32 + 8;
+        sums_at = kThreads * ring_pieces(rb) * 16;
+        part_at = sums_at + kFewUnit * rank * 4;
+        lo_at = part_at + kFewUnit * pitch * 2;
+        const int parts = 8 / rb, a = parts > 1 ? parts * kFewUnit * rank * 4 : 0, b = 2 * kFewUnit * pitch * 2;
+        bytes = part_at + (a > b ? a : b);
+    }
+};
 
 struct FewShared {
     int32_t ids[kFewRows];
+    int32_t same[kFewRows];                   // rows before with the same id
+    uint32_t leads[kFewRows / 32];            // rows that lead a unit, a bit each
     int32_t rows[kFewUnit];
-    int32_t n_rows, id;
-    float part[2048];                         // [k part][row][rank] of the warps: 8 parts of up to 8, 4 of 24, 2 of 56
-    float sum[kFewUnit * kMaxRank];           // [row][rank] of this CTA's part of the input dimension
-    __align__(16) __nv_bfloat16 hi[kFewUnit][kMaxRank + 8], lo[kFewUnit][kMaxRank + 8];
 };
 
-__global__ void __launch_bounds__(kThreads)
-low_rank_few_kernel(const LowRankArgs p) {
-    __shared__ FewShared s;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
-    const int unit = blockIdx.x / kFewCtas, c = (int)cluster_rank();
-    // Row i leads a unit if a multiple of 16 rows before it have its id; units are numbered in the order of their leaders.
-    if (tid < kFewRows) {
-        const int id = tid < p.n ? p.ids[tid] : -1;
-        s.ids[tid] = id >= 0 && id < p.count ? id : -1;
+// The rows (in s.rows) and the adapter of a unit; returns how many, 0 where there is no such unit.  Row i leads a unit if a
+// multiple of 16 rows before it have its id; units are numbered in the order of their leaders.
+__device__ __forceinline__ int find_unit(const LowRankArgs& p, FewShared& s, int unit, int& id) {
+    const int i = threadIdx.x, lane = i & 31;
+    int own = -1;
+    if (i < kFewRows) {
+        own = i < p.n ? p.ids[i] : -1;
+        own = own >= 0 && own < p.count ? own : -1;
+        s.ids[i] = own;
     }
-    if (tid == 0) s.n_rows = 0;
     __syncthreads();
-    if (warp == 0) {
-        int before = 0;
-        bool found = false;
-        for (int base = 0; base < p.n && !found; base += 32) {
-            const int i = base + lane, id = s.ids[i];
-            int same = 0;
-            for (int j = 0; j < base; j += 4) {
-                const int4 v = *reinterpret_cast<const int4*>(&s.ids[j]);
-                same += (v.x == id) + (v.y == id) + (v.z == id) + (v.w == id);
-            }
-            const unsigned alike = __match_any_sync(0xffffffffu, i < p.n ? id : -2 - lane);
-            same += __popc(alike & ((1u << lane) - 1u));
-            const unsigned leads = __ballot_sync(0xffffffffu, i < p.n && same % kFewUnit == 0);
-            const int here = unit - before;
-            if (here < __popc(leads)) {
-                // the unit's leader is the here-th set bit; its rows are it and the next 15 with its id
-                unsigned m = leads;
-                for (int k = 0; k < here; ++k) m &= m - 1;
-                const int src = __ffs(m) - 1, leader = base + src, lead_id = __shfl_sync(0xffffffffu, id, src);
-                int n = 0;
-                for (int b2 = leader & ~31; b2 < p.n && n < kFewUnit; b2 += 32) {
-                    const int r = b2 + lane;
-                    const unsigned hit = __ballot_sync(0xffffffffu, r >= leader && r < p.n && s.ids[r] == lead_id);
-                    const int at = n + __popc(hit & ((1u << lane) - 1u));
-                    if ((hit >> lane & 1u) && at < kFewUnit) s.rows[at] = r;
-                    n += __popc(hit);
-                }
-                if (lane == 0) {
-                    s.n_rows = min(n, kFewUnit);
-                    s.id = lead_id;
-                }
-                found = true;
-            }
-            before += __popc(leads);
+    int same = 0;
+    if (i < kFewRows) {
+        for (int j = 0; j < (i & ~31) && i < p.n; j += 4) {
+            const int4 v = *reinterpret_cast<const int4*>(&s.ids[j]);
+            same += (v.x == own) + (v.y == own) + (v.z == own) + (v.w == own);
         }
+        const unsigned alike = __match_any_sync(0xffffffffu, i < p.n ? own : -2 - lane);
+        same += __popc(alike & ((1u << lane) - 1u));
+        const unsigned leads = __ballot_sync(0xffffffffu, i < p.n && same % kFewUnit == 0);
+        if (lane == 0) s.leads[i >> 5] = leads;
+        s.same[i] = same;
     }
     __syncthreads();
-    const int m = s.n_rows, id = s.id;
+    int leader = -1, here = unit;
+#pragma unroll
+    for (int b = 0; b < kFewRows / 32; ++b) {
+        unsigned m = s.leads[b];
+        if (leader < 0 && here < __popc(m)) {
+            for (; here > 0; --here) m &= m - 1;
+            leader = b * 32 + __ffs(m) - 1;
+        }
+        here -= __popc(m);
+    }
+    if (leader < 0) return 0;
+    id = s.ids[leader];
+    const int at = same - s.same[leader];
+    const bool mine = i < p.n && own == id && at >= 0 && at < kFewUnit;
+    if (mine) s.rows[at] = i;
+    return __syncthreads_count(mine);
+}
+
+// `clusters` clusters of `ctas` CTAs a unit: each cluster multiplies x . a^T for itself and takes a part of the columns.
+// TP: tiles of eight values of the rank that a warp multiplies (1, 2 or 4; RB > 1: 4).
+template <int RB, int TP>
+__global__ void __launch_bounds__(kThreads, RB <= 2 ? 3 : 2)
+low_rank_few_kernel(const LowRankArgs p, const int ctas, const int clusters) {
+    __shared__ __align__(16) FewShared s;
+    extern __shared__ __align__(16) unsigned char dyn[];
+    constexpr int kPiece = kThreads * 16;     // bytes between a lane's pieces
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
+    const int c = ctas > 1 ? (int)cluster_rank() : 0;
+    int id = -1;
+    const int cluster = blockIdx.x / ctas, unit = cluster / clusters;
+    const int m = find_unit(p, s, unit, id);
     if (m == 0) return;                       // fewer units than clusters: the whole cluster leaves
     // output columns of this CTA, in tiles of eight
-    const int tiles = (p.n_out + 7) / 8, t0 = tiles * c / kFewCtas, t1 = tiles * (c + 1) / kFewCtas;
+    const int tiles = (p.n_out + 7) / 8, part_of = (cluster - unit * clusters) * ctas + c;
+    const int t0 = (int)((long)tiles * part_of / (ctas * clusters)), t1 = (int)((long)tiles * (part_of + 1) / (ctas * clusters));
     if (id < 0) {
         if (p.out != p.y)
             for (int r = 0; r < m; ++r) {
@@ -154,38 +189,108 @@ low_rank_few_kernel(const LowRankArgs p) {
             }
         return;
     }
-    const int rank = p.rank, rt = rank / 8;   // rank in tiles of eight
+    // a lane multiplies the rows g and g + 8 of the unit
+    const int row0 = s.rows[min(g, m - 1)], row1 = s.rows[min(g + 8, m - 1)];
+    const bool has0 = g < m, has1 = g + 8 < m, more = m > 8;
+    const int rank = p.rank;
+    const FewPlan pl(rank, RB);
+    float* sums = reinterpret_cast<float*>(dyn + pl.sums_at);
+    float* parts = reinterpret_cast<float*>(dyn + pl.part_at);
+    __nv_bfloat16* hi = reinterpret_cast<__nv_bfloat16*>(dyn + pl.part_at);
+    __nv_bfloat16* lo = reinterpret_cast<__nv_bfloat16*>(dyn + pl.lo_at);
+    const uint32_t own = smem_addr(dyn) + (uint32_t)tid * 16u;
     const __nv_bfloat16* a = p.a + (size_t)id * rank * p.in;
     const __nv_bfloat16* b = p.b + (size_t)id * p.n_out * rank;
-    const uint4 zero = make_uint4(0, 0, 0, 0);
 
-    // x . a^T: warps over tiles of the rank (up to four each) and over k
-    const int lg_wr = rt >= 8 ? 3 : (rt >= 4 ? 2 : (rt >= 2 ? 1 : 0)), wr = warp & ((1 << lg_wr) - 1), wk = warp >> lg_wr, n_wk = 8 >> lg_wr;
-    const int blocks = (p.in + 31) / 32, b0 = blocks * c / kFewCtas, b1 = blocks * (c + 1) / kFewCtas;
-    float acc[4][4] = {};
+    // x . a^T: a warp takes TP tiles of the rank, every RB-th, and one of 8 / RB parts of the k blocks of 32
+    constexpr int kWk = 8 / RB;
+    const int wr = warp & (RB - 1), wk = warp / RB, rt = rank / 8;
+    float acc[TP][4] = {};
     {
-        const __nv_bfloat16* x0 = p.x + (size_t)s.rows[min(g, m - 1)] * p.in;
-        const __nv_bfloat16* x1 = p.x + (size_t)s.rows[min(g + 8, m - 1)] * p.in;
-#pragma unroll 2
-        for (int kb = b0 + wk; kb < b1; kb += n_wk) {
-            const int k = kb * 32 + q * 8;
-            const bool in = k < p.in;
-            const uint4 v0 = in && g < m ? ldg16(x0 + k) : zero, v1 = in && g + 8 < m ? ldg16(x1 + k) : zero;
+        constexpr int kPieces = TP + 2, kDepth = ring_pieces(RB) / kPieces;
+        const int blocks = (p.in + 31) / 32, b0 = blocks * c / ctas, b1 = blocks * (c + 1) / ctas;
+        const int n = (b1 - b0 - wk + kWk - 1) / kWk;                     // blocks of this warp
+        int k = (b0 + wk) * 32 + q * 8;                                   // of the next load
+        const __nv_bfloat16* x0 = p.x + (size_t)row0 * p.in + k;
+        const __nv_bfloat16* x1 = p.x + (size_t)row1 * p.in + k;
+        const __nv_bfloat16* aw = a + (size_t)(wr * 8 + g) * p.in + k;
+        const size_t tile = (size_t)(8 * RB) * p.in;
+        int left = n;
+        uint32_t to = own;
+        auto load = [&]() {
+            if (left > 0) {
+                const bool in = k < p.in;
+                copy16(to, in && has0 ? x0 : p.x, in && has0);
+                if (more) copy16(to + kPiece, in && has1 ? x1 : p.x, in && has1);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int t = wr + (i << lg_wr);
-                if (t >= rt) break;
-                const uint4 w = in ? ldg16(a + (size_t)(t * 8 + g) * p.in + k) : zero;
-                mma(acc[i], v0.x, v1.x, v0.y, v1.y, w.x, w.y);
-                mma(acc[i], v0.z, v1.z, v0.w, v1.w, w.z, w.w);
+                for (int i = 0; i < TP; ++i)
+                    if (wr + i * RB < rt) copy16(to + (2 + i) * kPiece, in ? aw + i * tile : a, in);
+            }
+            copies_commit();
+            --left;
+            k += kWk * 32;
+            x0 += kWk * 32;
+            x1 += kWk * 32;
+            aw += kWk * 32;
+            to += kPieces * kPiece;
+            if (to == own + kDepth * kPieces * kPiece) to = own;
+        };
+#pragma unroll
+        for (int i = 0; i < kDepth; ++i) load();
+        uint32_t from = own;
+        for (int i = 0; i < n; ++i) {
+            copies_wait<kDepth - 1>();
+            const uint4 v0 = ld_shared16(from), v1 = more ? ld_shared16(from + kPiece) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+            for (int t = 0; t < TP; ++t) {
+                if (wr + t * RB >= rt) break;
+                const uint4 w = ld_shared16(from + (2 + t) * kPiece);
+                mma(acc[t], v0.x, v1.x, v0.y, v1.y, w.x, w.y);
+                mma(acc[t], v0.z, v1.z, v0.w, v1.w, w.z, w.w);
+            }
+            load();
+            from += kPieces * kPiece;
+            if (from == own + kDepth * kPieces * kPiece) from = own;
+        }
+        copies_wait<0>();
+    }
+    // The second product's pieces, b and y of a tile of output columns each: the first are on their way while the cluster meets.
+    constexpr int kPieces = RB + 1, kDepth = ring_pieces(RB) / kPieces;
+    const bool pairs = p.n_out % 2 == 0 && (((uintptr_t)p.y | (uintptr_t)p.out) % 4) == 0;
+    const int n = (t1 - t0 - warp + 7) >> 3;                              // tiles of this warp, every eighth
+    int left = n, row = (t0 + warp) * 8 + g, col = (t0 + warp) * 8 + 2 * q;    // of the next load: row of b, column of y
+    const __nv_bfloat16* bw = b + (size_t)row * rank + q * 8;
+    const __nv_bfloat16* y0 = p.y + (size_t)row0 * p.n_out + col;
+    const __nv_bfloat16* y1 = p.y + (size_t)row1 * p.n_out + col;
+    uint32_t to = own;
+    auto load = [&]() {
+        if (left > 0) {
+#pragma unroll
+            for (int kb = 0; kb < RB; ++kb) {
+                const bool there = row < p.n_out && kb * 32 + q * 8 < rank;
+                copy16(to + (1 + kb) * kPiece, there ? bw + kb * 32 : b, there);
+            }
+            if (pairs && col < p.n_out) {
+                if (has0) copy4(to, y0);
+                if (more && has1) copy4(to + 4, y1);
             }
         }
-    }
-    const int pitch = n_wk > 1 ? rt * 8 : 0;  // (with one part the warps' tiles are the sums)
-    float* part = n_wk > 1 ? s.part + wk * kFewUnit * pitch : s.sum;
+        copies_commit();
+        --left;
+        row += 64;
+        col += 64;
+        bw += 64 * rank;
+        y0 += 64;
+        y1 += 64;
+        to += kPieces * kPiece;
+        if (to == own + kDepth * kPieces * kPiece) to = own;
+    };
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int t = wr + (i << lg_wr);
+    for (int i = 0; i < kDepth; ++i) load();
+    float* part = kWk > 1 ? parts + wk * kFewUnit * rank : sums;          // (with one part the warps' tiles are the sums)
+#pragma unroll
+    for (int i = 0; i < TP; ++i) {
+        const int t = wr + i * RB;
         if (t >= rt) break;
         float* d = part + t * 8 + 2 * q;
         d[g * rank] = acc[i][0];
@@ -193,70 +298,109 @@ low_rank_few_kernel(const LowRankArgs p) {
         d[(g + 8) * rank] = acc[i][2];
         d[(g + 8) * rank + 1] = acc[i][3];
     }
-    __syncthreads();
-    if (n_wk > 1) {
+    if (kWk > 1) {
+        __syncthreads();
         for (int i = tid; i < m * rank; i += kThreads) {
             float v = 0.f;
-            for (int k = 0; k < n_wk; ++k) v += s.part[k * kFewUnit * pitch + i];
-            s.sum[i] = v;
+#pragma unroll
+            for (int k = 0; k < kWk; ++k) v += parts[k * kFewUnit * rank + i];
+            sums[i] = v;
         }
     }
-    cluster_sync();
+    if (ctas > 1) cluster_sync();
+    else __syncthreads();
     const float sc = p.scale != nullptr ? p.scale[id] : 1.f;
-    const int blocks_r = (rank + 31) / 32;
-    for (int i = tid; i < kFewUnit * blocks_r * 32; i += kThreads) {
-        const int r = i / (blocks_r * 32), k = i - r * blocks_r * 32;
+    for (int i = tid; i < kFewUnit * RB * 32; i += kThreads) {
+        const int r = i / (RB * 32), k = i % (RB * 32);
         float v = 0.f;
         if (r < m && k < rank) {
-            const uint32_t at = smem_addr(&s.sum[r * rank + k]);
-#pragma unroll
-            for (int peer = 0; peer < kFewCtas; ++peer) v += ld_peer(peer_addr(at, peer));
+            const uint32_t at = smem_addr(&sums[r * rank + k]);
+            for (int peer = 0; peer < ctas; ++peer) v += ctas > 1 ? ld_peer(peer_addr(at, peer)) : sums[r * rank + k];
             v *= sc;
         }
-        split2(v, s.hi[r][k], s.lo[r][k]);
+        split2(v, hi[r * pl.pitch + k], lo[r * pl.pitch + k]);
     }
+    if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");     // this CTA has read the others' sums
     __syncthreads();
 
     // + t . b^T
-    const bool pairs = p.n_out % 2 == 0 && (((uintptr_t)p.y | (uintptr_t)p.out) % 4) == 0;
-    const size_t at0 = (size_t)s.rows[min(g, m - 1)] * p.n_out, at1 = (size_t)s.rows[min(g + 8, m - 1)] * p.n_out;
-    const uint4* h0 = reinterpret_cast<const uint4*>(&s.hi[g][q * 8]);
-    const uint4* h1 = reinterpret_cast<const uint4*>(&s.hi[g + 8][q * 8]);
-    const uint4* l0 = reinterpret_cast<const uint4*>(&s.lo[g][q * 8]);
-    const uint4* l1 = reinterpret_cast<const uint4*>(&s.lo[g + 8][q * 8]);
-#pragma unroll 4
-    for (int t = t0 + warp; t < t1; t += 8) {
-        float d[4] = {0.f, 0.f, 0.f, 0.f};
-        const __nv_bfloat16* br = b + (size_t)(t * 8 + g) * rank + q * 8;
-        for (int kb = 0; kb < blocks_r; ++kb) {
-            const uint4 w = t * 8 + g < p.n_out && kb * 32 + q * 8 < rank ? ldg16(br + kb * 32) : zero;
-            const uint4 vh0 = h0[kb * 4], vh1 = h1[kb * 4], vl0 = l0[kb * 4], vl1 = l1[kb * 4];
-            mma(d, vh0.x, vh1.x, vh0.y, vh1.y, w.x, w.y);
-            mma(d, vh0.z, vh1.z, vh0.w, vh1.w, w.z, w.w);
-            mma(d, vl0.x, vl1.x, vl0.y, vl1.y, w.x, w.y);
-            mma(d, vl0.z, vl1.z, vl0.w, vl1.w, w.z, w.w);
-        }
-        const int n = t * 8 + 2 * q;
+    const uint4* h0 = reinterpret_cast<const uint4*>(hi + g * pl.pitch + q * 8);
+    const uint4* h1 = reinterpret_cast<const uint4*>(hi + (g + 8) * pl.pitch + q * 8);
+    const uint4* l0 = reinterpret_cast<const uint4*>(lo + g * pl.pitch + q * 8);
+    const uint4* l1 = reinterpret_cast<const uint4*>(lo + (g + 8) * pl.pitch + q * 8);
+    constexpr int kKept = RB <= 2 ? RB : 1;   // up to a rank of 64 the low-rank rows stay in registers
+    uint4 vh0[kKept], vh1[kKept], vl0[kKept], vl1[kKept];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            if (g + 8 * h >= m || n >= p.n_out) continue;
-            const size_t at = (h ? at1 : at0) + n;
-            if (pairs) {
-                const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(p.y + at));
-                *reinterpret_cast<__nv_bfloat162*>(p.out + at) = __floats2bfloat162_rn(v.x + d[2 * h], v.y + d[2 * h + 1]);
-            } else {
-                p.out[at] = __float2bfloat16_rn(__bfloat162float(p.y[at]) + d[2 * h]);
-                if (n + 1 < p.n_out) p.out[at + 1] = __float2bfloat16_rn(__bfloat162float(p.y[at + 1]) + d[2 * h + 1]);
-            }
-        }
+    for (int kb = 0; kb < kKept; ++kb) {
+        vh0[kb] = h0[kb * 4];
+        vh1[kb] = h1[kb * 4];
+        vl0[kb] = l0[kb * 4];
+        vl1[kb] = l1[kb * 4];
     }
-    cluster_sync();                           // the others have read this CTA's sums
+    size_t at0 = (size_t)row0 * p.n_out + (t0 + warp) * 8 + 2 * q, at1 = (size_t)row1 * p.n_out + (t0 + warp) * 8 + 2 * q;
+    int out_col = (t0 + warp) * 8 + 2 * q;
+    uint32_t from = own;
+    auto write = [&](size_t at, uint32_t y, float d0, float d1) {
+        if (pairs) {
+            const float2 v = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&y));
+            *reinterpret_cast<__nv_bfloat162*>(p.out + at) = __floats2bfloat162_rn(v.x + d0, v.y + d1);
+        } else {
+            p.out[at] = __float2bfloat16_rn(__bfloat162float(p.y[at]) + d0);
+            if (out_col + 1 < p.n_out) p.out[at + 1] = __float2bfloat16_rn(__bfloat162float(p.y[at + 1]) + d1);
+        }
+    };
+    for (int i = 0; i < n; ++i) {
+        copies_wait<kDepth - 1>();
+        float d[4] = {0.f, 0.f, 0.f, 0.f}, e[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint4 yv = ld_shared16(from);
+#pragma unroll
+        for (int kb = 0; kb < RB; ++kb) {
+            const uint4 w = ld_shared16(from + (1 + kb) * kPiece);
+            const int i0 = RB <= 2 ? kb : 0;
+            if (RB > 2) {
+                vh0[0] = h0[kb * 4];
+                vh1[0] = h1[kb * 4];
+                vl0[0] = l0[kb * 4];
+                vl1[0] = l1[kb * 4];
+            }
+            mma(d, vh0[i0].x, vh1[i0].x, vh0[i0].y, vh1[i0].y, w.x, w.y);
+            mma(e, vl0[i0].x, vl1[i0].x, vl0[i0].y, vl1[i0].y, w.x, w.y);
+            mma(d, vh0[i0].z, vh1[i0].z, vh0[i0].w, vh1[i0].w, w.z, w.w);
+            mma(e, vl0[i0].z, vl1[i0].z, vl0[i0].w, vl1[i0].w, w.z, w.w);
+        }
+        if (out_col < p.n_out) {
+            if (has0) write(at0, yv.x, d[0] + e[0], d[1] + e[1]);
+            if (more && has1) write(at1, yv.y, d[2] + e[2], d[3] + e[3]);
+        }
+        load();
+        at0 += 64;
+        at1 += 64;
+        out_col += 64;
+        from += kPieces * kPiece;
+        if (from == own + kDepth * kPieces * kPiece) from = own;
+    }
+    copies_wait<0>();
+    if (ctas > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");       // ... and they this one's
+}
+
+struct FewKernel {
+    const void* kernel;
+    int rb;
+};
+FewKernel few_kernel(int rank) {
+    if (rank <= 8) return {(const void*)low_rank_few_kernel<1, 1>, 1};
+    if (rank <= 16) return {(const void*)low_rank_few_kernel<1, 2>, 1};
+    if (rank <= 32) return {(const void*)low_rank_few_kernel<1, 4>, 1};
+    if (rank <= 64) return {(const void*)low_rank_few_kernel<2, 4>, 2};
+    if (rank <= 128) return {(const void*)low_rank_few_kernel<4, 4>, 4};
+    return {(const void*)low_rank_few_kernel<8, 4>, 8};
 }
 
 // ── many rows ───────────────────────────────────────────────────────────────
 constexpr int kTileRows = 64;
 constexpr int kCols = 64;                     // columns of a stage, of the input first, then of the output
-__host__ __device__ constexpr int tile_stages(int rank) { return rank > 128 ? 2 : 4; }
+// Stages of columns in shared memory: what fits with two CTAs on an SM (one from a rank of 65 on).
+__host__ __device__ constexpr int tile_stages(int rank) { return rank > 128 ? 2 : (rank > 32 ? 4 : 6); }
 constexpr int kMaxBins = 2048;                // adapters + 1
 constexpr int kBlockRows = 8192;              // rows of a launch: each CTA looks through all their ids
 constexpr int kColPitch = (kCols / 8 + 1) * 16;   // bytes; an odd number of 16-byte pieces: eight rows meet no bank twice
@@ -270,27 +414,18 @@ struct TileShared {
 // Offsets in the dynamic shared memory.
 struct TilePlan {
     int r16, pitch;                           // rank rounded up to 16; bytes of a row of it
-    int stage, stages_at, sums_at, hi_at, lo_at, bytes;
+    int stage, sums_at, hi_at, lo_at, bytes;
     __host__ __device__ explicit TilePlan(int rank) {
         r16 = (rank + 15) & ~15;
         pitch = ((r16 / 8) | 1) * 16;
         const int first = (kTileRows + r16) * kColPitch, second = kTileRows * kColPitch + kCols * pitch;
         stage = first > second ? first : second;
-        stages_at = 0;
         sums_at = tile_stages(rank) * stage;
         hi_at = sums_at + kTileRows * r16 * 4;
         lo_at = hi_at + kTileRows * pitch;
         bytes = lo_at + kTileRows * pitch;
     }
 };
-
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
-    const int n = there ? 16 : 0;             // the rest is filled with zeros
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // NJ: tiles of 16 values of the rank that a warp multiplies (rank up to 32 NJ).
 template <int NJ>
@@ -302,20 +437,28 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas) {
     const TilePlan pl(p.rank);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int unit = blockIdx.x / ctas, c = ctas > 1 ? (int)cluster_rank() : 0;
-    // Units of this block of rows: adapter 0's rows in tiles of 64, adapter 1's, ..., at last the rows without one.
+    // Units of this block of rows: adapter 0's rows in tiles of 64, adapter 1's, ..., at last the rows without one.  A warp
+    // has an eighth of the ids, 32 at a time in batch order, all of them in registers: as loads of the loops below, one after
+    // the other, they took 22 us.
     int32_t* bins = reinterpret_cast<int32_t*>(smem);
     const int n_bins = p.count + 1;
+    constexpr int kIds = kBlockRows / kThreads;
+    const int groups = (p.n + kThreads - 1) / kThreads, from = warp * groups * 32;
+    int bin[kIds];
+#pragma unroll
+    for (int i = 0; i < kIds; ++i) {
+        const int r = from + i * 32 + lane;
+        bin[i] = i < groups && r < p.n ? p.ids[r] : -1;
+        if (i < groups && r < p.n && (bin[i] < 0 || bin[i] >= p.count)) bin[i] = p.count;
+    }
     for (int i = tid; i < n_bins; i += kThreads) bins[i] = 0;
     if (tid == 0) s.n_rows = 0;
     __syncthreads();
-    auto bin_of = [&](int i) {
-        const int id = p.ids[i];
-        return id >= 0 && id < p.count ? id : p.count;
-    };
-    for (int i = tid; i < ((p.n + 31) & ~31); i += kThreads) {
-        const int bin = i < p.n ? bin_of(i) : -1;
-        const unsigned alike = __match_any_sync(0xffffffffu, bin);
-        if (bin >= 0 && lane == __ffs(alike) - 1) atomicAdd(&bins[bin], __popc(alike));
+#pragma unroll
+    for (int i = 0; i < kIds; ++i) {
+        if (i >= groups) break;
+        const unsigned alike = __match_any_sync(0xffffffffu, bin[i]);
+        if (bin[i] >= 0 && lane == __ffs(alike) - 1) atomicAdd(&bins[bin[i]], __popc(alike));
     }
     __syncthreads();
     if (warp == 0) {
@@ -341,18 +484,19 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas) {
     const int m = s.n_rows, id = s.id, skip = s.first;
     if (m == 0) return;
     {
-        // the unit's rows: those of the bin from the skip-th on, in batch order; a warp looks through an eighth
-        const int per = ((p.n + 255) / 256) * 32, from = warp * per, to = min(from + per, p.n);
+        // the unit's rows: those of the bin from the skip-th on, in batch order
         int n = 0;
-        for (int base = from; base < to; base += 32) n += __popc(__ballot_sync(0xffffffffu, base + lane < to && bin_of(base + lane) == id));
+#pragma unroll
+        for (int i = 0; i < kIds; ++i) n += __popc(__ballot_sync(0xffffffffu, bin[i] == id));
         if (lane == 0) s.warp_count[warp] = n;
         __syncthreads();
         n = -skip;
         for (int w = 0; w < warp; ++w) n += s.warp_count[w];
-        for (int base = from; base < to && n < m; base += 32) {
-            const unsigned hit = __ballot_sync(0xffffffffu, base + lane < to && bin_of(base + lane) == id);
+#pragma unroll
+        for (int i = 0; i < kIds; ++i) {
+            const unsigned hit = __ballot_sync(0xffffffffu, bin[i] == id);
             const int at = n + __popc(hit & ((1u << lane) - 1u));
-            if ((hit >> lane & 1u) && at >= 0 && at < m) s.rows[at] = base + lane;
+            if ((hit >> lane & 1u) && at >= 0 && at < m) s.rows[at] = from + i * 32 + lane;
             n += __popc(hit);
         }
     }
@@ -376,53 +520,97 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas) {
     const __nv_bfloat16* a = p.a + (size_t)id * rank * p.in;
     const __nv_bfloat16* b = p.b + (size_t)id * p.n_out * rank;
     const uint32_t base = smem_addr(smem);
-    // a stage of the first product: 64 rows of x and the rank's rows of a, 64 columns each
-    auto load_in = [&](int k, int st) {
-        const uint32_t xs = base + pl.stages_at + st * pl.stage, as = xs + kTileRows * kColPitch;
-        for (int i = tid; i < kTileRows * 8; i += kThreads) {
-            const int r = i >> 3, col = k * kCols + (i & 7) * 8;
-            const bool there = r < m && col < p.in;
-            copy16(xs + r * kColPitch + (i & 7) * 16, there ? p.x + (size_t)s.rows[r] * p.in + col : p.x, there);
-        }
-        for (int i = tid; i < r16 * 8; i += kThreads) {
-            const int r = i >> 3, col = k * kCols + (i & 7) * 8;
-            const bool there = r < rank && col < p.in;
-            copy16(as + r * kColPitch + (i & 7) * 16, there ? a + (size_t)r * p.in + col : a, there);
-        }
+    // What a thread copies is the same in every stage but for the columns: of x and y a piece of two rows, of a and b NJ pieces.
+    const int cr = tid >> 3, cc = (tid & 7) * 8;
+    const __nv_bfloat16* xr[2];
+    const __nv_bfloat16* yr[2];
+    bool has[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        has[i] = cr + 32 * i < m;
+        const size_t row = s.rows[has[i] ? cr + 32 * i : 0];
+        xr[i] = p.x + row * p.in + cc;
+        yr[i] = p.y + row * p.n_out + cc;
+    }
+    const int pieces = r16 / 8;
+    int b_left[NJ], b_to[NJ];                 // rows of b up to the end (0: zeros, below: nothing), and where the piece goes
+    const __nv_bfloat16* b_from[NJ];
+#pragma unroll
+    for (int i = 0; i < NJ; ++i) {
+        const int e = tid + i * kThreads, r = e / pieces, j = e - r * pieces;
+        b_left[i] = r < kCols ? (j * 8 < rank ? p.n_out - n0 * kCols - r : 0) : -(1 << 30);
+        b_from[i] = b + (size_t)(n0 * kCols + r) * rank + j * 8;
+        b_to[i] = kTileRows * kColPitch + r * pl.pitch + j * 16;
+    }
+    const uint32_t own = base + cr * kColPitch + cc * 2;
+    int in_left = p.in - k0 * kCols - cc, out_left = p.n_out - n0 * kCols - cc;      // columns of x and of y up to the end
+    const __nv_bfloat16* a_from = a + (size_t)cr * p.in + k0 * kCols + cc;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        xr[i] += k0 * kCols;
+        yr[i] += n0 * kCols;
+    }
+    // the next stage of the first product: 64 rows of x and the rank's rows of a, 64 columns each
+    auto load_in = [&](uint32_t st) {
+        const bool in = in_left > 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) copy16(own + st + i * 32 * kColPitch, in && has[i] ? xr[i] : p.x, in && has[i]);
+#pragma unroll
+        for (int i = 0; i < NJ; ++i)
+            if (cr + 32 * i < r16) {
+                const bool there = in && cr + 32 * i < rank;
+                copy16(own + st + (kTileRows + 32 * i) * kColPitch, there ? a_from + (size_t)(32 * i) * p.in : a, there);
+            }
+        in_left -= kCols;
+        a_from += kCols;
+        xr[0] += kCols;
+        xr[1] += kCols;
     };
     // ... of the second: 64 rows of y (where they are whole pieces) and 64 of b
-    const int pieces = r16 / 8;
-    auto load_out = [&](int n, int st) {
-        const uint32_t ys = base + pl.stages_at + st * pl.stage, bs = ys + kTileRows * kColPitch;
-        if (p.wide)
-            for (int i = tid; i < kTileRows * 8; i += kThreads) {
-                const int r = i >> 3, col = n * kCols + (i & 7) * 8;
-                const bool there = r < m && col < p.n_out;
-                copy16(ys + r * kColPitch + (i & 7) * 16, there ? p.y + (size_t)s.rows[r] * p.n_out + col : p.y, there);
-            }
-        for (int i = tid; i < kCols * pieces; i += kThreads) {
-            const int r = i / pieces, j = i - r * pieces, row = n * kCols + r;
-            const bool there = row < p.n_out && j * 8 < rank;
-            copy16(bs + r * pl.pitch + j * 16, there ? b + (size_t)row * rank + j * 8 : b, there);
+    auto load_out = [&](uint32_t st) {
+        if (p.wide) {
+            const bool in = out_left > 0;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) copy16(own + st + i * 32 * kColPitch, in && has[i] ? yr[i] : p.y, in && has[i]);
         }
+#pragma unroll
+        for (int i = 0; i < NJ; ++i) {
+            if (b_left[i] > -(1 << 29)) copy16(base + st + b_to[i], b_left[i] > 0 ? b_from[i] : b, b_left[i] > 0);
+            b_left[i] -= kCols;
+            b_from[i] += kCols * rank;
+        }
+        out_left -= kCols;
+        yr[0] += kCols;
+        yr[1] += kCols;
     };
     const int rt = warp & 3, half = warp >> 2;     // the warp's 16 rows, and its half of the rank's or the columns' tiles
     // (ldmatrix: lanes 0..15 give the rows of the first eight columns, 16..31 those of the next)
     const int lr = lane & 15, lc = (lane >> 4) * 16;
     const int total = (k1 - k0) + (n1 - n0);       // both products' stages in one line
-    auto load = [&](int i) {
-        if (i < k1 - k0) load_in(k0 + i, i % kTileStages);
-        else if (i < total) load_out(n0 + i - (k1 - k0), i % kTileStages);
+    const uint32_t ring = (uint32_t)(kTileStages * pl.stage);
+    int loaded = 0;
+    uint32_t to_stage = 0, at_stage = 0;           // offsets of the stage to fill next and of the one to use next
+    auto load = [&]() {
+        if (loaded < k1 - k0) load_in(to_stage);
+        else if (loaded < total) load_out(to_stage);
         copies_commit();
+        ++loaded;
+        to_stage += pl.stage;
+        if (to_stage == ring) to_stage = 0;
     };
-    for (int i = 0; i < kTileStages - 1; ++i) load(i);
+    auto next_stage = [&]() {
+        at_stage += pl.stage;
+        if (at_stage == ring) at_stage = 0;
+    };
+    for (int i = 0; i < kTileStages - 1; ++i) load();
     float acc[NJ][8] = {};
     int it = 0;
     for (; it < k1 - k0; ++it) {
         copies_wait<kTileStages - 2>();
         __syncthreads();
-        load(it + kTileStages - 1);
-        const uint32_t xs = base + pl.stages_at + (it % kTileStages) * pl.stage, as = xs + kTileRows * kColPitch;
+        load();
+        const uint32_t xs = base + at_stage, as = xs + kTileRows * kColPitch;
+        next_stage();
 #pragma unroll
         for (int kk = 0; kk < kCols / 16; ++kk) {
             uint32_t va[4];
@@ -480,27 +668,56 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas) {
         }
     }
     if (ctas > 1) cluster_sync();
+    else __syncthreads();
+    // up to a rank of 64 the low-rank rows stay in registers
+    constexpr int kKept = NJ <= 2 ? 2 * NJ : 0;
+    uint32_t kh[kKept > 0 ? kKept : 1][4], kl[kKept > 0 ? kKept : 1][4];
+    const uint32_t hi_own = base + pl.hi_at + (rt * 16 + lr) * pl.pitch + lc, lo_own = hi_own + pl.lo_at - pl.hi_at;
+#pragma unroll
+    for (int kk = 0; kk < kKept; ++kk)
+        if (kk * 16 < r16) {
+            ldmatrix4(hi_own + kk * 32, kh[kk]);
+            ldmatrix4(lo_own + kk * 32, kl[kk]);
+        }
+    __nv_bfloat16* to_own[2];
+    bool has_own[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = rt * 16 + (lane >> 2) + 8 * i;
+        has_own[i] = r < m;
+        to_own[i] = p.out + (size_t)s.rows[has_own[i] ? r : 0] * p.n_out + n0 * kCols + half * 32 + (lane & 3) * 8;
+    }
+    int n = n0 * kCols;                            // first column of the stage
     for (; it < total; ++it) {
         copies_wait<kTileStages - 2>();
         __syncthreads();
-        load(it + kTileStages - 1);
-        const int n = n0 + it - (k1 - k0);
-        unsigned char* ys_p = smem + pl.stages_at + (it % kTileStages) * pl.stage;
-        const uint32_t ys = smem_addr(ys_p), bs = ys + kTileRows * kColPitch;
+        load();
+        unsigned char* ys_p = smem + at_stage;
+        next_stage();
+        const uint32_t bs = smem_addr(ys_p) + kTileRows * kColPitch + (half * 32 + lr) * pl.pitch + lc;
         float d[4][4] = {};                   // four tiles of eight columns of the warp's 32
-#pragma unroll 2
-        for (int kk = 0; kk < r16 / 16; ++kk) {
-            uint32_t vh[4], vl[4];
-            ldmatrix4(base + pl.hi_at + (rt * 16 + lr) * pl.pitch + kk * 32 + lc, vh);
-            ldmatrix4(base + pl.lo_at + (rt * 16 + lr) * pl.pitch + kk * 32 + lc, vl);
+        auto step = [&](const uint32_t (&vh)[4], const uint32_t (&vl)[4], int kk) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
                 uint32_t vb[4];
-                ldmatrix4(bs + (half * 32 + j * 16 + lr) * pl.pitch + kk * 32 + lc, vb);
+                ldmatrix4(bs + j * 16 * pl.pitch + kk * 32, vb);
                 mma(d[2 * j], vh[0], vh[1], vh[2], vh[3], vb[0], vb[2]);
                 mma(d[2 * j + 1], vh[0], vh[1], vh[2], vh[3], vb[1], vb[3]);
                 mma(d[2 * j], vl[0], vl[1], vl[2], vl[3], vb[0], vb[2]);
                 mma(d[2 * j + 1], vl[0], vl[1], vl[2], vl[3], vb[1], vb[3]);
+            }
+        };
+        if (kKept > 0) {
+#pragma unroll
+            for (int kk = 0; kk < kKept; ++kk)
+                if (kk * 16 < r16) step(kh[kk], kl[kk], kk);
+        } else {
+#pragma unroll 2
+            for (int kk = 0; kk < r16 / 16; ++kk) {
+                uint32_t vh[4], vl[4];
+                ldmatrix4(hi_own + kk * 32, vh);
+                ldmatrix4(lo_own + kk * 32, vl);
+                step(vh, vl, kk);
             }
         }
         if (p.wide) {
@@ -514,24 +731,26 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas) {
                     *at = __floats2bfloat162_rn(v.x + d[j][2 * h], v.y + d[j][2 * h + 1]);
                 }
             __syncwarp();
+            const int r0 = rt * 16 + (lane >> 2), col = half * 32 + (lane & 3) * 8;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int r = rt * 16 + (lane >> 2) + 8 * i, col = half * 32 + (lane & 3) * 8;
-                if (r < m && n * kCols + col < p.n_out)
-                    *reinterpret_cast<uint4*>(p.out + (size_t)s.rows[r] * p.n_out + n * kCols + col) = *reinterpret_cast<const uint4*>(ys_p + r * kColPitch + col * 2);
-            }
+            for (int i = 0; i < 2; ++i)
+                if (has_own[i] && n + col < p.n_out)
+                    *reinterpret_cast<uint4*>(to_own[i]) = *reinterpret_cast<const uint4*>(ys_p + (r0 + 8 * i) * kColPitch + col * 2);
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const int r = rt * 16 + g + 8 * (e >> 1), col = n * kCols + half * 32 + j * 8 + 2 * q + (e & 1);
+                    const int r = rt * 16 + g + 8 * (e >> 1), col = n + half * 32 + j * 8 + 2 * q + (e & 1);
                     if (r < m && col < p.n_out) {
                         const size_t at = (size_t)s.rows[r] * p.n_out + col;
                         p.out[at] = __float2bfloat16_rn(__bfloat162float(p.y[at]) + d[j][e]);
                     }
                 }
         }
+        n += kCols;
+        to_own[0] += kCols;
+        to_own[1] += kCols;
     }
     copies_wait<0>();
 }
@@ -561,16 +780,20 @@ int launch_low_rank(LowRankArgs p, int sms, cudaStream_t stream) {
         p.y = whole.y + (size_t)r0 * p.n_out;
         p.out = whole.out + (size_t)r0 * p.n_out;
         p.ids = whole.ids + r0;
-        void* args[] = {&p, nullptr};
+        int ctas = 1;
+        void* args[] = {&p, &ctas, nullptr};
         if (step == kFewRows) {
-            IMX_TRY(launch_clusters((const void*)low_rank_few_kernel, (unsigned)(p.n * kFewCtas), kFewCtas, 0, stream, args));
+            const FewKernel few = few_kernel(p.rank);
+            while (ctas < 8 && p.n * ctas * 2 <= (few.rb <= 2 ? 3 : 2) * sms) ctas *= 2;
+            int clusters = 1;
+            while (clusters < 16 && p.n * ctas * clusters * 2 <= sms && p.n_out >= 128 * ctas * clusters) clusters *= 2;
+            args[2] = &clusters;
+            IMX_TRY(launch_clusters(few.kernel, (unsigned)(p.n * ctas * clusters), ctas, (size_t)FewPlan(p.rank, few.rb).bytes, stream, args));
             continue;
         }
         // no more units than these; CTAs for two on every SM
         const int units = p.n / kTileRows + (p.count + 1 < p.n ? p.count + 1 : p.n);
-        int ctas = 1;
         while (ctas < 8 && units * ctas * 2 <= 2 * sms) ctas *= 2;
-        args[1] = &ctas;
         const void* kernel = p.rank <= 32 ? (const void*)low_rank_tile_kernel<1> : (p.rank <= 64 ? (const void*)low_rank_tile_kernel<2>
                                           : (p.rank <= 128 ? (const void*)low_rank_tile_kernel<4> : (const void*)low_rank_tile_kernel<8>));
         IMX_TRY(launch_clusters(kernel, (unsigned)(units * ctas), ctas, (size_t)TilePlan(p.rank).bytes, stream, args));
@@ -608,6 +831,10 @@ extern "C" int imx_low_rank_add(const void* y, const void* x, int n_rows, int in
         const void* kernels[4] = {(const void*)low_rank_tile_kernel<1>, (const void*)low_rank_tile_kernel<2>, (const void*)low_rank_tile_kernel<4>,
                                   (const void*)low_rank_tile_kernel<8>};
         for (int i = 0; i < 4; ++i) IMX_CHECK_CUDA(cudaFuncSetAttribute(kernels[i], cudaFuncAttributeMaxDynamicSharedMemorySize, TilePlan(32 << i).bytes));
+        for (int rank : {8, 16, 32, 64, 128, 256}) {
+            const FewKernel few = few_kernel(rank);
+            IMX_CHECK_CUDA(cudaFuncSetAttribute(few.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FewPlan(rank, few.rb).bytes));
+        }
         device_mark_setup(di.ordinal, kSetupLowRank);
     }
     const int wide = n_out % 8 == 0 && (((uintptr_t)y | (uintptr_t)out) % 16) == 0;

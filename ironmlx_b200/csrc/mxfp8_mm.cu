@@ -36,7 +36,7 @@ constexpr int kMxThreads = 352;
 constexpr int kMxK = 128;                          // codes of a row in a stage
 constexpr int kMxMaxStages = 10;
 constexpr int kMxGroups = 2;                       // groups of four K steps whose scales are in shared memory
-constexpr int kMxMaxSplits = 8;
+constexpr int kMxMaxSplits = 8;                  // CTAs of a cluster that cut the K range of a tile
 std::atomic<int> g_mx_spin_limit{kSpin};
 
 template <int NT, bool SWAP, bool PAIR>
@@ -655,27 +655,44 @@ int launch(const Call& c, int lg_splits) {
     return IMX_OK;
 }
 
+// Which kernel: the least of a model of their times in us, a part that does not shrink and a time for each K step of each wave
+// of tiles, fitted to the kernels alone on a B200 (2048 -> 8192 unless said; measured, in brackets the model):
+//   1 row     S16 8.9 (8.6), S16 cut in 2 7.7 (7.8), N64 9.4 (9.6);   2048 -> 512  S16 cut in 1, 2, 4, 8  8.2, 6.3, 5.4, 5.3
+//   64 rows   S64 11.4 (11.3), S64 cut in 2 10.9 (9.9), N64 9.7 (9.6);   4096 -> 2048  S64 cut in 4 9.6 (9.9), N64 14.0 (14.4)
+//   256 rows  N64 15.4 (14.4), N128 11.1 (10.9), P256 13.0 (11.7);   777 rows 4096 -> 2048  N128 16.4 (17.0), P256 17.9 (17.8)
+//   1024 rows N128 27.6 (23.0), P256 19.8 (18.0);   2048 -> 152064, 64 rows  S64 60.4, N64 91, N128 61, P256 70 (memory: 52)
+// Clusters of eight that fill the GPU find no place together: 4096 -> 2048, 1 row, cut in 8 (128 CTAs) 11.8, in 4 7.3.
 int run(const Call& c) {
     const int steps = ceil_div(c.in, kMxK);
-    int nt = c.m <= 16 ? 16 : (c.m <= 32 ? 32 : (c.m <= 64 ? 64 : 128));
-    bool swap = c.m <= 128, pair = false;
-    if (!swap) nt = (long)ceil_div(c.m, 128) * ceil_div(c.n_out, 256) >= c.sms ? 256 : 128;
-    if (!swap && nt == 256) pair = true;
-    long tiles = swap ? (long)ceil_div(c.n_out, 128) * ceil_div(c.m, nt) : (long)ceil_div(c.m, 128) * ceil_div(c.n_out, nt);
-    int splits = 1;
-    while (swap && splits < kMxMaxSplits && tiles * splits * 2 <= c.sms && steps >= splits * 4) splits *= 2;
-    if (const char* e = getenv("IMX_MX")) {
-        int s = 0;
-        sscanf(e, "%d,%d,%d", &s, &nt, &splits);
-        swap = s == 1;
-        pair = s == 2;
-        if (!swap) splits = 1;
+    enum { S16, S32, S64, N64, N128, P256 } best = P256;
+    int best_lg = 0;
+    float least = 1e30f;
+    auto offer = [&](decltype(best) kernel, int lg, float fixed, long tiles, int at_once, float step) {
+        const long waves = (tiles + at_once - 1) / at_once;
+        const float us = fixed + (float)waves * (float)ceil_div(steps, 1 << lg) * step;
+        if (us < least) {
+            least = us;
+            best = kernel;
+            best_lg = lg;
+        }
+    };
+    const int nt = c.m <= 16 ? 16 : (c.m <= 32 ? 32 : 64);
+    const long tiles = (long)ceil_div(c.n_out, 128) * ceil_div(c.m, nt);
+    for (int lg = 0; lg < 4 && (lg == 0 || (tiles << lg <= (lg == 3 ? 64 : c.sms) && steps >= 2 << lg)); ++lg)
+        offer(nt == 16 ? S16 : (nt == 32 ? S32 : S64), lg, 4.6f + 0.03f * nt + (lg > 0 ? 1.f : 0.f), tiles, lg > 0 ? (int)tiles : c.sms,
+              nt == 64 ? 0.30f : 0.22f);
+    const long rows128 = ceil_div(c.m, 128);
+    offer(N64, 0, 4.8f, rows128 * ceil_div(c.n_out, 64), c.sms, 0.30f);
+    offer(N128, 0, 4.8f, rows128 * ceil_div(c.n_out, 128), c.sms, 0.38f);
+    offer(P256, 0, 5.5f, (long)ceil_div(c.m, 256) * ceil_div(c.n_out, 256), c.sms / 2, 0.39f);
+    switch (best) {
+        case S16: return launch<16, true>(c, best_lg);
+        case S32: return launch<32, true>(c, best_lg);
+        case S64: return launch<64, true>(c, best_lg);
+        case N64: return launch<64, false>(c, 0);
+        case N128: return launch<128, false>(c, 0);
+        default: return launch<256, false, true>(c, 0);
     }
-    int lg = 0;
-    while (1 << lg < splits) ++lg;
-    if (pair) return nt == 256 ? launch<256, false, true>(c, 0) : launch<128, false, true>(c, 0);
-    if (swap) return nt == 16 ? launch<16, true>(c, lg) : (nt == 32 ? launch<32, true>(c, lg) : (nt == 64 ? launch<64, true>(c, lg) : launch<128, true>(c, lg)));
-    return nt == 256 ? launch<256, false>(c, 0) : (nt == 64 ? launch<64, false>(c, 0) : launch<128, false>(c, 0));
 }
 
 }  // namespace
@@ -719,11 +736,8 @@ int imx_mxfp8_matmul(const void* x_q, const void* x_scales, int m, const imx_qte
         IMX_TRY((set_up<16, true>()));
         IMX_TRY((set_up<32, true>()));
         IMX_TRY((set_up<64, true>()));
-        IMX_TRY((set_up<128, true>()));
         IMX_TRY((set_up<64, false>()));
         IMX_TRY((set_up<128, false>()));
-        IMX_TRY((set_up<256, false>()));
-        IMX_TRY((set_up<128, false, true>()));
         IMX_TRY((set_up<256, false, true>()));
         device_mark_setup(di.ordinal, kSetupMxfp8);
     }

@@ -39,9 +39,11 @@ class LowRankAdapters:
 class _WithAdapters:
     def forward_with_adapters(self, x: torch.Tensor, adapters: LowRankAdapters, ids: torch.Tensor, stream=None) -> torch.Tensor:
         """The shared projection of all rows and the low-rank adapter ids[t] of each (int32, negative: none)."""
-        with ops._on(x, stream):
-            y = self.forward_with_stream(x)
-            return adapters.add(y, x, ids, out=y)
+        if ops._elsewhere(x, stream):
+            with ops._on(x, stream):
+                return self.forward_with_adapters(x, adapters, ids)
+        y = self.forward_with_stream(x)
+        return adapters.add(y, x, ids, out=y)
 
 
 @dataclass

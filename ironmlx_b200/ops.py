@@ -10,7 +10,6 @@ scales/biases bf16, mxfp8/nvfp4 scales uint8.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes as C
 from typing import NamedTuple, Optional
 
@@ -212,17 +211,28 @@ class Mxfp8Rows(NamedTuple):
 def _on(x: torch.Tensor, stream):
     """The device of x, and the given stream, made current: what is allocated within belongs to that stream, and the
     launches go to that device."""
-    if stream is not None:
-        return torch.cuda.stream(stream)
-    if x.device.index != torch.cuda.current_device():
-        return torch.cuda.device(x.device)
-    return contextlib.nullcontext()
+    return torch.cuda.device(x.device) if stream is None else torch.cuda.stream(stream)
+
+
+def _elsewhere(x: torch.Tensor, stream) -> bool:
+    """Whether a call on x has to switch stream or device first (`_on`)."""
+    return stream is not None or x.get_device() != torch.cuda.current_device()
+
+
+# The current stream's handle: a call of a few microseconds would spend three on the Stream object.
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _require_same_device(name, first, *tensors):
-    _require_cuda(first, *tensors)
+    if not first.is_cuda or not first.is_contiguous():
+        raise IronMLXError(_lib.ERR_INVALID, f"{name}: tensors must be contiguous CUDA tensors")
+    device = first.get_device()
     for t in tensors:
-        if t is not None and t.device != first.device:
+        if t is None:
+            continue
+        if not t.is_cuda or not t.is_contiguous():
+            raise IronMLXError(_lib.ERR_INVALID, f"{name}: tensors must be contiguous CUDA tensors")
+        if t.get_device() != device:
             raise IronMLXError(_lib.ERR_INVALID, f"{name}: tensors on {first.device} and {t.device}")
 
 
@@ -235,52 +245,60 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: Opti
     _require_same_device("add_rms_norm", x, residual, weight)
     if out not in ("bf16", "mxfp8", "both"):
         raise IronMLXError(_lib.ERR_INVALID, f"add_rms_norm: out must be bf16, mxfp8 or both, not {out!r}")
-    for t in (x, residual, weight):
-        if t is not None and t.dtype != torch.bfloat16:
-            raise IronMLXError(_lib.ERR_INVALID, "add_rms_norm: x, residual and weight must be bfloat16")
-    if x.dim() == 0 or x.shape[-1] == 0:
+    shape = x.shape
+    if (x.dtype != torch.bfloat16 or (residual is not None and residual.dtype != torch.bfloat16)
+            or (weight is not None and weight.dtype != torch.bfloat16)):
+        raise IronMLXError(_lib.ERR_INVALID, "add_rms_norm: x, residual and weight must be bfloat16")
+    if len(shape) == 0 or shape[-1] == 0:
         raise IronMLXError(_lib.ERR_INVALID, "add_rms_norm: x has no last dimension")
-    hidden = x.shape[-1]
-    if residual is not None and residual.shape != x.shape:
-        raise IronMLXError(_lib.ERR_INVALID, f"add_rms_norm: residual {tuple(residual.shape)} and x {tuple(x.shape)} differ")
+    hidden = shape[-1]
+    if residual is not None and residual.shape != shape:
+        raise IronMLXError(_lib.ERR_INVALID, f"add_rms_norm: residual {tuple(residual.shape)} and x {tuple(shape)} differ")
     if weight is not None and weight.numel() != hidden:
         raise IronMLXError(_lib.ERR_INVALID, f"add_rms_norm: weight has {weight.numel()} elements, rows have {hidden}")
     if out != "bf16" and hidden % 32:
         raise IronMLXError(_lib.ERR_INVALID, f"add_rms_norm: 8-bit rows need a row length ({hidden}) that is a multiple of 32")
-    with _on(x, stream):
-        h = x if residual is None else torch.empty_like(x)
-        y = torch.empty_like(x) if out != "mxfp8" else None
-        rows = None
-        if out != "bf16":
-            rows = Mxfp8Rows(torch.empty(*x.shape[:-1], hidden // 4, dtype=torch.int32, device=x.device),
-                             torch.empty(*x.shape[:-1], hidden // 32, dtype=torch.uint8, device=x.device))
-        check(lib().imx_add_rms_norm(x.data_ptr(), _ptr(residual), x.numel() // hidden, hidden, _ptr(weight), float(eps),
-                                     None if residual is None else h.data_ptr(), _ptr(y),
-                                     None if rows is None else rows[0].data_ptr(), None if rows is None else rows[1].data_ptr(),
-                                     torch.cuda.current_stream().cuda_stream))
+    if _elsewhere(x, stream):
+        with _on(x, stream):
+            return add_rms_norm(x, residual, weight, eps, out)
+    device = x.device
+    h = x if residual is None else torch.empty_like(x)
+    y = rows = None
+    if out != "mxfp8":
+        y = torch.empty_like(x)
+    if out != "bf16":
+        lead = tuple(shape)[:-1]
+        rows = Mxfp8Rows(torch.empty(*lead, hidden // 4, dtype=torch.int32, device=device),
+                         torch.empty(*lead, hidden // 32, dtype=torch.uint8, device=device))
+    check(lib().imx_add_rms_norm(x.data_ptr(), None if residual is None else residual.data_ptr(), x.numel() // hidden, hidden,
+                                 None if weight is None else weight.data_ptr(), eps, None if residual is None else h.data_ptr(),
+                                 None if y is None else y.data_ptr(), None if rows is None else rows[0].data_ptr(),
+                                 None if rows is None else rows[1].data_ptr(), _raw_stream(x.get_device())))
     return h, y, rows
 
 
 _STATUS = {}
 
 
-def _status_block(device) -> torch.Tensor:
+def _status_block(index: int) -> torch.Tensor:
     """The status block of a device's `mxfp8_matmul` calls: zero-filled once, kernels only ever set its first word."""
-    buf = _STATUS.get(device)
+    buf = _STATUS.get(index)
     if buf is None:
-        buf = torch.zeros(256, dtype=torch.uint8, device=device)
+        buf = torch.zeros(256, dtype=torch.uint8, device=torch.device("cuda", index))
         if not torch.cuda.is_current_stream_capturing():             # in a capture: one for this call
-            torch.cuda.current_stream(device).synchronize()          # other streams see the zeros
-            _STATUS[device] = buf
+            torch.cuda.current_stream(index).synchronize()           # other streams see the zeros
+            _STATUS[index] = buf
     return buf
 
 
-def check_status(device, stream=None) -> None:
-    """Raises if a bounded wait ran out in an `mxfp8_matmul` call on the device since the last check; synchronises the stream."""
-    buf = _STATUS.get(torch.device(device))
+def check_status(device=None, stream=None) -> None:
+    """Raises if a bounded wait ran out in an `mxfp8_matmul` call on the device (default: the current one) since the last
+    check; synchronises the stream."""
+    index = torch.device("cuda" if device is None else device).index
+    buf = _STATUS.get(torch.cuda.current_device() if index is None else index)
     if buf is not None:
         with _on(buf, stream):
-            check(lib().imx_moe_status(buf.data_ptr(), torch.cuda.current_stream().cuda_stream))
+            check(lib().imx_moe_status(buf.data_ptr(), stream_ptr()))
 
 
 def mxfp8_matmul(rows, w: torch.Tensor, scales: torch.Tensor, stream=None) -> torch.Tensor:
@@ -290,19 +308,23 @@ def mxfp8_matmul(rows, w: torch.Tensor, scales: torch.Tensor, stream=None) -> to
     _require_same_device("mxfp8_matmul", x, xs, w, scales)
     if x.dtype != torch.int32 or w.dtype != torch.int32 or xs.dtype != torch.uint8 or scales.dtype != torch.uint8:
         raise IronMLXError(_lib.ERR_INVALID, "mxfp8_matmul: packed values must be int32 words, scales uint8")
-    if w.dim() != 2 or scales.dim() != 2 or x.dim() == 0 or xs.dim() == 0 or w.shape[1] % 8 or w.numel() == 0:
+    shape, wshape = x.shape, w.shape
+    if len(wshape) != 2 or len(shape) == 0 or wshape[1] % 8 or w.numel() == 0:
         raise IronMLXError(_lib.ERR_INVALID, "mxfp8_matmul: w must be [out, in/4] and scales [out, in/32], in a multiple of 32")
-    n_out, in_dim = w.shape[0], w.shape[1] * 4
-    if x.shape[-1] != w.shape[1]:
-        raise IronMLXError(_lib.ERR_INVALID, f"mxfp8_matmul: rows have {x.shape[-1] * 4} values, the weight takes {in_dim}")
-    if tuple(scales.shape) != (n_out, in_dim // 32) or tuple(xs.shape) != tuple(x.shape[:-1]) + (in_dim // 32,):
+    n_out, words = wshape
+    if shape[-1] != words:
+        raise IronMLXError(_lib.ERR_INVALID, f"mxfp8_matmul: rows have {shape[-1] * 4} values, the weight takes {words * 4}")
+    lead = tuple(shape)[:-1]
+    if scales.shape != (n_out, words // 8) or xs.shape != (*lead, words // 8):
         raise IronMLXError(_lib.ERR_INVALID, "mxfp8_matmul: one scale per 32 values is needed for the rows and the weight")
-    with _on(x, stream):
-        y = torch.empty(*x.shape[:-1], n_out, dtype=torch.bfloat16, device=x.device)
-        qt = QTensor(w.data_ptr(), scales.data_ptr(), None, 1.0)
-        check(lib().imx_mxfp8_matmul(x.data_ptr(), xs.data_ptr(), x.numel() // x.shape[-1], C.byref(qt), n_out, in_dim,
-                                     y.data_ptr(), _status_block(x.device).data_ptr(), 256,
-                                     torch.cuda.current_stream().cuda_stream))
+    if _elsewhere(x, stream):
+        with _on(x, stream):
+            return mxfp8_matmul(rows, w, scales)
+    index = x.get_device()
+    y = torch.empty(*lead, n_out, dtype=torch.bfloat16, device=x.device)
+    qt = QTensor(w.data_ptr(), scales.data_ptr(), None, 1.0)
+    check(lib().imx_mxfp8_matmul(x.data_ptr(), xs.data_ptr(), x.numel() // words, C.byref(qt), n_out, words * 4, y.data_ptr(),
+                                 _status_block(index).data_ptr(), 256, _raw_stream(index)))
     return y
 
 
@@ -314,27 +336,29 @@ def low_rank_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
     y [.., out_dim], x [.., in], a [count, rank, in], b [count, out_dim, rank] bf16; ids int32, one per row; scale fp32
     [count].  `out` may be y itself; a new tensor by default."""
     _require_same_device("low_rank_add", y, x, a, b, ids, scale, out)
-    for t in (y, x, a, b):
-        if t.dtype != torch.bfloat16:
-            raise IronMLXError(_lib.ERR_INVALID, "low_rank_add: y, x, a and b must be bfloat16")
-    if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2] or a.numel() == 0 or b.numel() == 0:
+    if y.dtype != torch.bfloat16 or x.dtype != torch.bfloat16 or a.dtype != torch.bfloat16 or b.dtype != torch.bfloat16:
+        raise IronMLXError(_lib.ERR_INVALID, "low_rank_add: y, x, a and b must be bfloat16")
+    ashape, bshape, xshape, yshape = a.shape, b.shape, x.shape, y.shape
+    if len(ashape) != 3 or len(bshape) != 3 or ashape[0] != bshape[0] or ashape[1] != bshape[2] or a.numel() == 0 or b.numel() == 0:
         raise IronMLXError(_lib.ERR_INVALID, "low_rank_add: a must be [count, rank, in] and b [count, out, rank]")
-    count, rank, in_dim = a.shape
-    n_out = b.shape[1]
-    if x.dim() == 0 or y.dim() == 0 or x.shape[-1] != in_dim or y.shape[-1] != n_out or x.shape[:-1] != y.shape[:-1]:
+    count, rank, in_dim = ashape
+    n_out = bshape[1]
+    if len(xshape) == 0 or len(yshape) == 0 or xshape[-1] != in_dim or yshape[-1] != n_out or xshape[:-1] != yshape[:-1]:
         raise IronMLXError(_lib.ERR_INVALID,
-                           f"low_rank_add: x {tuple(x.shape)} and y {tuple(y.shape)} do not match adapters {in_dim} -> {n_out}")
+                           f"low_rank_add: x {tuple(xshape)} and y {tuple(yshape)} do not match adapters {in_dim} -> {n_out}")
     rows = x.numel() // in_dim
     if ids.dtype != torch.int32 or ids.numel() != rows:
         raise IronMLXError(_lib.ERR_INVALID, f"low_rank_add: ids must be int32, one for each of the {rows} rows")
     if scale is not None and (scale.dtype != torch.float32 or scale.numel() != count):
         raise IronMLXError(_lib.ERR_INVALID, f"low_rank_add: scale must be float32, one for each of the {count} adapters")
-    if out is not None and (out.shape != y.shape or out.dtype != y.dtype):
+    if out is not None and (out.shape != yshape or out.dtype != torch.bfloat16):
         raise IronMLXError(_lib.ERR_INVALID, "low_rank_add: out must have y's shape and type")
-    with _on(x, stream):
-        if out is None:
-            out = torch.empty_like(y)
-        ad = _lib.Adapters(a.data_ptr(), b.data_ptr(), _ptr(scale), count, rank)
-        check(lib().imx_low_rank_add(y.data_ptr(), x.data_ptr(), rows, in_dim, C.byref(ad), ids.data_ptr(), n_out,
-                                     out.data_ptr(), torch.cuda.current_stream().cuda_stream))
+    if _elsewhere(x, stream):
+        with _on(x, stream):
+            return low_rank_add(y, x, a, b, ids, scale, out)
+    if out is None:
+        out = torch.empty_like(y)
+    ad = _lib.Adapters(a.data_ptr(), b.data_ptr(), None if scale is None else scale.data_ptr(), count, rank)
+    check(lib().imx_low_rank_add(y.data_ptr(), x.data_ptr(), rows, in_dim, C.byref(ad), ids.data_ptr(), n_out, out.data_ptr(),
+                                 _raw_stream(x.get_device())))
     return out
