@@ -405,10 +405,13 @@ typedef struct imx_adapters {
  * with y[t] the projection's row, x[t] its input, sums in fp32.  A row whose id is outside [0, count) -- -1 by convention --
  * has no adapter: out[t] = y[t].  Ids may come in any order.
  * x: bf16 [n_rows, in], in a multiple of 8; y, out: bf16 [n_rows, n_out]; out may be y itself, any other overlap is refused.
- * x, a and b 16-byte aligned; y and out at any bf16 value (16 bytes and n_out a multiple of 8 are fastest).  Needs no
- * scratch.  Where x, a or b are not finite the outputs that they reach are not either (NaN where the formula has an infinity). */
+ * x, a and b 16-byte aligned; y and out at any bf16 value (16 bytes and n_out a multiple of 8 are fastest).
+ * Where x, a or b are not finite the outputs that they reach are not either (NaN where the formula has an infinity).
+ * scratch: imx_low_rank_scratch_bytes bytes, as imx_mxfp8_matmul's: a status word that calls on several streams may share.
+ * Should a bounded wait run out, the outputs concerned are NaN. */
+IMX_API int imx_low_rank_scratch_bytes(int n_rows, int in, int n_out, int count, int rank, size_t* bytes);
 IMX_API int imx_low_rank_add(const void* y, const void* x, int n_rows, int in, const imx_adapters* adapters,
-                     const int32_t* ids, int n_out, void* out, void* stream);
+                     const int32_t* ids, int n_out, void* out, void* scratch, size_t scratch_bytes, void* stream);
 
 /* Quantize w[rows, in] (fp32) into packed values, scales and biases
  * (absent from the reference's wrappers, which only consume checkpoints that

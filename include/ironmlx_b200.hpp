@@ -164,7 +164,11 @@ struct LowRankAdapters {
         const int in = (int)a.dim(2), n_out = (int)b.dim(1), rows = (int)(x.size() / in);
         if (x.dim(-1) != in || y.dim(-1) != n_out || ids.size() != rows)
             throw Error(IMX_ERR_INVALID, "LowRankAdapters: shapes do not match the adapters");
-        check(imx_low_rank_add(y.ptr, x.ptr, rows, in, &ad, (const int32_t*)ids.ptr, n_out, y.ptr, stream));
+        size_t need = 0;
+        check(imx_low_rank_scratch_bytes(rows, in, n_out, ad.count, ad.rank, &need));
+        Scratch& sc = Scratch::local();
+        void* ws = sc.get(need);
+        check(imx_low_rank_add(y.ptr, x.ptr, rows, in, &ad, (const int32_t*)ids.ptr, n_out, y.ptr, ws, sc.bytes(), stream));
     }
 };
 

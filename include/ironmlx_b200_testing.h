@@ -41,4 +41,10 @@ extern "C"
 #endif
 __attribute__((visibility("default"))) void imx_testing_mxfp8_give_up(int on);
 
+/* ... and for imx_low_rank_add's kernel of many rows: status 5. */
+#ifdef __cplusplus
+extern "C"
+#endif
+__attribute__((visibility("default"))) void imx_testing_low_rank_give_up(int on);
+
 #endif /* IRONMLX_B200_TESTING_H */

@@ -76,6 +76,7 @@ SIGNATURES = {
     "imx_testing_route_give_up": (None, [_i]),
     "imx_testing_prefill_give_up": (None, [_i]),
     "imx_testing_mxfp8_give_up": (None, [_i]),
+    "imx_testing_low_rank_give_up": (None, [_i]),
     "imx_moe_saturations": (_i, [_vp, _vp, C.POINTER(C.c_longlong)]),
     "imx_moe_route": (_i, [_vp, _i, _i, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
     "imx_moe_route_scratch_bytes": (_i, [_i, _i, _i, C.POINTER(_sz)]),
@@ -107,7 +108,8 @@ SIGNATURES = {
     "imx_linear": (_i, [_vp, _i, _i, _vp, _i, _vp, _vp, _vp]),
     "imx_mxfp8_matmul_scratch_bytes": (_i, [_i, _i, _i, C.POINTER(_sz)]),
     "imx_mxfp8_matmul": (_i, [_vp, _vp, _i, C.POINTER(QTensor), _i, _i, _vp, _vp, _sz, _vp]),
-    "imx_low_rank_add": (_i, [_vp, _vp, _i, _i, C.POINTER(Adapters), _vp, _i, _vp, _vp]),
+    "imx_low_rank_scratch_bytes": (_i, [_i, _i, _i, _i, _i, C.POINTER(_sz)]),
+    "imx_low_rank_add": (_i, [_vp, _vp, _i, _i, C.POINTER(Adapters), _vp, _i, _vp, _vp, _sz, _vp]),
     "imx_quantize": (_i, [_vp, _i, _i, _i, _i, _i, _f, _vp, _vp, _vp, _vp]),
     "imx_gather_qmm": (_i, [_vp, _vp, C.POINTER(QTensor), _vp, _i, _i, _i, _i, _i, _i, _vp, _vp]),
 }

@@ -9,12 +9,18 @@
 // Which rows make up a unit every CTA finds out by itself from the ids: the units of an adapter are its rows in batch order,
 // so that the result does not depend on who runs when.  Rows without an adapter are units of their own that are copied.
 //
-// Two kernels, both bound by memory:
-//   few rows (at most 128 a launch): a and b are read once and go straight into the fragments of mma.sync, whose k order is
-//     permuted so that a lane's 16 bytes are four k pairs; latency counts, a cluster of eight spreads a unit's adapter.
-//   many rows: tiles of 64 rows; x with a, then y with b, come in stages of 64 columns by cp.async, four in flight; out
-//     leaves through y's place in shared memory in 16-byte pieces.
-#include "internal.h"
+// Two kernels:
+//   few rows (at most 128): a and b are read once and go straight into the fragments of mma.sync, whose k order is permuted so
+//     that a lane's 16 bytes are four k pairs.  Bound by latency: one row of rank 16, 2048 -> 2048, takes 5.5 us; 48 rows of 12
+//     adapters of rank 64, 4096 -> 4096 (12.6 MB: 1.9 us at the copy bandwidth), 11.8 us.
+//   many rows: tiles of 64 rows by tcgen05.mma, x and y gathered by cp.async, a and b brought by TMA.  Bound by how fast the
+//     warps move a stage through shared memory (1000 cycles for 64 rows x 64 columns of y, two CTAs to an SM): 8192 rows of
+//     rank 64, 4096 -> 4096, take 82 us, 201 MB at 2.4 TB/s; the same with mma.sync by the warps that copy took 113 us, and at
+//     rank 128 229 us, here 114.
+#include <atomic>
+
+#include "tcgen05.cuh"
+#include "../../include/ironmlx_b200_testing.h"
 
 namespace imx {
 
@@ -22,6 +28,8 @@ namespace {
 
 constexpr int kMaxRank = 256;
 constexpr int kThreads = 256;
+constexpr size_t kStatusBytes = 256;
+std::atomic<int> g_low_rank_spin_limit{kSpin};
 
 struct LowRankArgs {
     const __nv_bfloat16* y;
@@ -33,6 +41,8 @@ struct LowRankArgs {
     __nv_bfloat16* out;
     int n, in, n_out, count, rank;
     int wide;                 // y and out: rows of whole 16-byte pieces
+    int spin_limit;
+    int32_t* status;
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -66,9 +76,6 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&v)[4]) {
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr) : "memory");
 }
 // v = hi + lo to 16 bits (what is not finite stays in hi)
 __device__ __forceinline__ void split2(float v, __nv_bfloat16& hi, __nv_bfloat16& lo) {
@@ -315,7 +322,15 @@ low_rank_few_kernel(const LowRankArgs p, const int ctas, const int clusters) {
         float v = 0.f;
         if (r < m && k < rank) {
             const uint32_t at = smem_addr(&sums[r * rank + k]);
-            for (int peer = 0; peer < ctas; ++peer) v += ctas > 1 ? ld_peer(peer_addr(at, peer)) : sums[r * rank + k];
+            if (ctas > 1) {
+                float u[8];                   // all on their way before the first is added
+#pragma unroll
+                for (int peer = 0; peer < 8; ++peer) u[peer] = peer < ctas ? ld_peer(peer_addr(at, peer)) : 0.f;
+#pragma unroll
+                for (int peer = 0; peer < 8; ++peer) v += u[peer];
+            } else {
+                v = sums[r * rank + k];
+            }
             v *= sc;
         }
         split2(v, hi[r * pl.pitch + k], lo[r * pl.pitch + k]);
@@ -399,67 +414,136 @@ FewKernel few_kernel(int rank) {
 // ── many rows ───────────────────────────────────────────────────────────────
 constexpr int kTileRows = 64;
 constexpr int kCols = 64;                     // columns of a stage, of the input first, then of the output
-// Stages of columns in shared memory: what fits with two CTAs on an SM (one from a rank of 65 on).
-__host__ __device__ constexpr int tile_stages(int rank) { return rank > 128 ? 2 : (rank > 32 ? 4 : 6); }
 constexpr int kMaxBins = 2048;                // adapters + 1
 constexpr int kBlockRows = 8192;              // rows of a launch: each CTA looks through all their ids
-constexpr int kColPitch = (kCols / 8 + 1) * 16;   // bytes; an odd number of 16-byte pieces: eight rows meet no bank twice
+constexpr int kBlock = kTileRows * 128;       // bytes of 64 rows of 64 values in the MMA's K-major layout with 128-byte swizzle
+
+constexpr int kTileThreads = kThreads + 64;    // eight warps that copy and write out, one that issues the MMAs, one that loads a and b
+constexpr int kMaxStages = 5;
 
 struct TileShared {
     int32_t rows[kTileRows];
     int32_t warp_count[8];
     int32_t n_rows, id, first;
+    uint64_t rows_there[kMaxStages];          // the stage's rows of x (eight warps)
+    uint64_t loaded[kMaxStages];              // ... its part of a or b (TMA)
+    uint64_t used[kMaxStages];                // its MMAs are done
+    uint64_t sums_there[2], sums_free[2];     // second product: a stage's sums, and its place in tensor memory
+    uint64_t retired;
+    uint32_t tmem_base;
+    int abort;
+};
+struct TileMaps {
+    CUtensorMap a, b;
 };
 
-// Offsets in the dynamic shared memory.
+// NJ: blocks of 32 values of the rank (1, 2, 4 or 8).  The first product's sums have a place of their own up to a rank of 128
+// only: below 65 the stages and the low-rank rows of two CTAs fill an SM, and the sums go where the last stage of the first
+// product was; beyond 128 they take the stages' place.
 struct TilePlan {
-    int r16, pitch;                           // rank rounded up to 16; bytes of a row of it
-    int stage, sums_at, hi_at, lo_at, bytes;
-    __host__ __device__ explicit TilePlan(int rank) {
+    int r16, blocks;                          // rank rounded up to 16; blocks of 64 of it
+    int stages, stage, sums_at, hi_at, lo_at, bytes;
+    __host__ __device__ TilePlan(int rank, int nj) {
         r16 = (rank + 15) & ~15;
-        pitch = ((r16 / 8) | 1) * 16;
-        const int first = (kTileRows + r16) * kColPitch, second = kTileRows * kColPitch + kCols * pitch;
-        stage = first > second ? first : second;
-        sums_at = tile_stages(rank) * stage;
-        hi_at = sums_at + kTileRows * r16 * 4;
-        lo_at = hi_at + kTileRows * pitch;
-        bytes = lo_at + kTileRows * pitch;
+        blocks = (r16 + 63) / 64;
+        stages = nj <= 4 ? 5 : 3;
+        const int first = kBlock + r16 * 128, second = blocks * kBlock + kTileRows * 128;
+        stage = ((first > second ? first : second) + 1023) & ~1023;
+        hi_at = stages * stage;
+        lo_at = hi_at + blocks * kBlock;
+        sums_at = nj == 4 ? lo_at + blocks * kBlock : 0;
+        bytes = lo_at + blocks * kBlock + (nj == 4 ? kTileRows * r16 * 4 : 0);
     }
 };
 
-// NJ: tiles of 16 values of the rank that a warp multiplies (rank up to 32 NJ).
+// 16 lanes x 8 columns a count: thread t gets of each block of eight columns lane t / 4, columns 2 (t % 4), +1, and the same of
+// lane t / 4 + 8, as an mma.sync leaves its sums.
+__device__ __forceinline__ void tmem_ld_16x16(uint32_t taddr, float (&v)[8]) {
+    uint32_t u[8];
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7])
+                 : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(u[i]);
+}
+__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, float (&v)[16]) {
+    uint32_t u[16];
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]),
+                   "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+                 : "r"(taddr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(u[i]);
+}
+
+// Eight warps gather x, and y, by cp.async; a ninth issues the MMAs, a tenth brings a and b by TMA.  In the second product a warp
+// copies, adds and writes 16 rows x 32 columns that no other warp touches, so that the warps meet nowhere but at the
+// accumulators (with a __syncthreads and the MMAs' issue in every stage 8192 tokens of rank 16 took 97 us).
+// `clusters` clusters a unit: each multiplies x . a^T for itself and takes a part of the columns.
 template <int NJ>
-__global__ void __launch_bounds__(kThreads, NJ <= 2 ? 2 : 1)
-low_rank_tile_kernel(const LowRankArgs p, const int ctas) {
-    constexpr int kTileStages = tile_stages(32 * NJ);
-    extern __shared__ __align__(16) unsigned char smem[];
+__global__ void __launch_bounds__(kTileThreads, NJ <= 2 ? 2 : 1)
+low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, const __grid_constant__ TileMaps maps) {
+    extern __shared__ unsigned char smem_raw[];
     __shared__ TileShared s;
-    const TilePlan pl(p.rank);
+    unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    const TilePlan pl(p.rank, NJ);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int unit = blockIdx.x / ctas, c = ctas > 1 ? (int)cluster_rank() : 0;
+    const int cluster = blockIdx.x / ctas, unit = cluster / clusters, c = ctas > 1 ? (int)cluster_rank() : 0;
     // Units of this block of rows: adapter 0's rows in tiles of 64, adapter 1's, ..., at last the rows without one.  A warp
     // has an eighth of the ids, 32 at a time in batch order, all of them in registers: as loads of the loops below, one after
     // the other, they took 22 us.
     int32_t* bins = reinterpret_cast<int32_t*>(smem);
     const int n_bins = p.count + 1;
     constexpr int kIds = kBlockRows / kThreads;
-    const int groups = (p.n + kThreads - 1) / kThreads, from = warp * groups * 32;
+    const int groups = warp < 8 ? (p.n + kThreads - 1) / kThreads : 0, from = warp * groups * 32;
     int bin[kIds];
+    // (in lots of eight: what is done for none of the ids of a small batch costs it 2 us)
+    auto lots = [&](auto&& each) {
 #pragma unroll
-    for (int i = 0; i < kIds; ++i) {
+        for (int i = 0; i < kIds; ++i) {
+            if (i % 8 == 0 && i >= groups) break;
+            each(i);
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < kIds; ++i) bin[i] = -1;
+    lots([&](int i) {
         const int r = from + i * 32 + lane;
-        bin[i] = i < groups && r < p.n ? p.ids[r] : -1;
-        if (i < groups && r < p.n && (bin[i] < 0 || bin[i] >= p.count)) bin[i] = p.count;
+        if (i < groups && r < p.n) bin[i] = p.ids[r];
+    });
+    lots([&](int i) {
+        if (i < groups && from + i * 32 + lane < p.n && (bin[i] < 0 || bin[i] >= p.count)) bin[i] = p.count;
+    });
+    for (int i = tid; i < n_bins; i += kTileThreads) bins[i] = 0;
+    if (tid == 0) {
+        s.n_rows = 0;
+        s.abort = 0;
+        for (int i = 0; i < kMaxStages; ++i) {
+            tc::mbar_init(tc::smem_u32(&s.rows_there[i]), 8);
+            tc::mbar_init(tc::smem_u32(&s.loaded[i]), 1);
+            tc::mbar_init(tc::smem_u32(&s.used[i]), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(tc::smem_u32(&s.sums_there[i]), 1);
+            tc::mbar_init(tc::smem_u32(&s.sums_free[i]), 8);
+        }
+        tc::mbar_init(tc::smem_u32(&s.retired), 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    for (int i = tid; i < n_bins; i += kThreads) bins[i] = 0;
-    if (tid == 0) s.n_rows = 0;
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kIds; ++i) {
-        if (i >= groups) break;
-        const unsigned alike = __match_any_sync(0xffffffffu, bin[i]);
-        if (bin[i] >= 0 && lane == __ffs(alike) - 1) atomicAdd(&bins[bin[i]], __popc(alike));
-    }
+    // (votes first, all at once: one after the other with what follows from them they took 200 cycles each)
+    unsigned whole = 0;                       // groups of 32 inside a prompt
+    lots([&](int i) { whole |= (unsigned)__all_sync(0xffffffffu, bin[i] == __shfl_sync(0xffffffffu, bin[i], 0)) << i; });
+    lots([&](int i) {
+        if (whole >> i & 1u) {
+            if (lane == 0 && bin[i] >= 0) atomicAdd(&bins[bin[i]], 32);
+        } else {
+            const unsigned alike = __match_any_sync(0xffffffffu, bin[i]);
+            if (bin[i] >= 0 && lane == __ffs(alike) - 1) atomicAdd(&bins[bin[i]], __popc(alike));
+        }
+    });
     __syncthreads();
     if (warp == 0) {
         int before = 0;
@@ -482,31 +566,32 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas) {
     }
     __syncthreads();
     const int m = s.n_rows, id = s.id, skip = s.first;
-    if (m == 0) return;
+    if (m == 0) return;                       // fewer units than clusters: the whole cluster leaves
     {
         // the unit's rows: those of the bin from the skip-th on, in batch order
+        unsigned hit[kIds];
         int n = 0;
-#pragma unroll
-        for (int i = 0; i < kIds; ++i) n += __popc(__ballot_sync(0xffffffffu, bin[i] == id));
-        if (lane == 0) s.warp_count[warp] = n;
+        lots([&](int i) { hit[i] = __ballot_sync(0xffffffffu, bin[i] == id); });
+        lots([&](int i) { n += __popc(hit[i]); });
+        if (lane == 0 && warp < 8) s.warp_count[warp] = n;
         __syncthreads();
         n = -skip;
         for (int w = 0; w < warp; ++w) n += s.warp_count[w];
-#pragma unroll
-        for (int i = 0; i < kIds; ++i) {
-            const unsigned hit = __ballot_sync(0xffffffffu, bin[i] == id);
-            const int at = n + __popc(hit & ((1u << lane) - 1u));
-            if ((hit >> lane & 1u) && at >= 0 && at < m) s.rows[at] = from + i * 32 + lane;
-            n += __popc(hit);
-        }
+        lots([&](int i) {
+            const int at = n + __popc(hit[i] & ((1u << lane) - 1u));
+            if ((hit[i] >> lane & 1u) && at >= 0 && at < m) s.rows[at] = from + i * 32 + lane;
+            n += __popc(hit[i]);
+        });
     }
     __syncthreads();
     // chunks of the input and of the output dimension that this CTA takes
     const int ik = (p.in + kCols - 1) / kCols, on = (p.n_out + kCols - 1) / kCols;
-    const int k0 = ik * c / ctas, k1 = ik * (c + 1) / ctas, n0 = on * c / ctas, n1 = on * (c + 1) / ctas;
+    const int part_of = (cluster - unit * clusters) * ctas + c;
+    const int k0 = ik * c / ctas, k1 = ik * (c + 1) / ctas;
+    const int n0 = (int)((long)on * part_of / (ctas * clusters)), n1 = (int)((long)on * (part_of + 1) / (ctas * clusters));
     if (id == p.count) {
         if (p.out != p.y)
-            for (int r = warp; r < m; r += 8) {
+            for (int r = warp; r < m; r += kTileThreads / 32) {
                 const size_t at = (size_t)s.rows[r] * p.n_out;
                 const int end = min(n1 * kCols, p.n_out);
                 if (p.wide)
@@ -516,249 +601,315 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas) {
             }
         return;
     }
-    const int rank = p.rank, r16 = pl.r16;
-    const __nv_bfloat16* a = p.a + (size_t)id * rank * p.in;
-    const __nv_bfloat16* b = p.b + (size_t)id * p.n_out * rank;
-    const uint32_t base = smem_addr(smem);
-    // What a thread copies is the same in every stage but for the columns: of x and y a piece of two rows, of a and b NJ pieces.
-    const int cr = tid >> 3, cc = (tid & 7) * 8;
-    const __nv_bfloat16* xr[2];
-    const __nv_bfloat16* yr[2];
-    bool has[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        has[i] = cr + 32 * i < m;
-        const size_t row = s.rows[has[i] ? cr + 32 * i : 0];
-        xr[i] = p.x + row * p.in + cc;
-        yr[i] = p.y + row * p.n_out + cc;
+    constexpr uint32_t kTmem = NJ == 8 ? 256 : 128;        // the first product's sums, in their place two of a stage of the second
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&s.tmem_base)), "r"(kTmem) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    const int pieces = r16 / 8;
-    int b_left[NJ], b_to[NJ];                 // rows of b up to the end (0: zeros, below: nothing), and where the piece goes
-    const __nv_bfloat16* b_from[NJ];
-#pragma unroll
-    for (int i = 0; i < NJ; ++i) {
-        const int e = tid + i * kThreads, r = e / pieces, j = e - r * pieces;
-        b_left[i] = r < kCols ? (j * 8 < rank ? p.n_out - n0 * kCols - r : 0) : -(1 << 30);
-        b_from[i] = b + (size_t)(n0 * kCols + r) * rank + j * 8;
-        b_to[i] = kTileRows * kColPitch + r * pl.pitch + j * 16;
-    }
-    const uint32_t own = base + cr * kColPitch + cc * 2;
-    int in_left = p.in - k0 * kCols - cc, out_left = p.n_out - n0 * kCols - cc;      // columns of x and of y up to the end
-    const __nv_bfloat16* a_from = a + (size_t)cr * p.in + k0 * kCols + cc;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        xr[i] += k0 * kCols;
-        yr[i] += n0 * kCols;
-    }
-    // the next stage of the first product: 64 rows of x and the rank's rows of a, 64 columns each
-    auto load_in = [&](uint32_t st) {
-        const bool in = in_left > 0;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) copy16(own + st + i * 32 * kColPitch, in && has[i] ? xr[i] : p.x, in && has[i]);
-#pragma unroll
-        for (int i = 0; i < NJ; ++i)
-            if (cr + 32 * i < r16) {
-                const bool there = in && cr + 32 * i < rank;
-                copy16(own + st + (kTileRows + 32 * i) * kColPitch, there ? a_from + (size_t)(32 * i) * p.in : a, there);
-            }
-        in_left -= kCols;
-        a_from += kCols;
-        xr[0] += kCols;
-        xr[1] += kCols;
-    };
-    // ... of the second: 64 rows of y (where they are whole pieces) and 64 of b
-    auto load_out = [&](uint32_t st) {
-        if (p.wide) {
-            const bool in = out_left > 0;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) copy16(own + st + i * 32 * kColPitch, in && has[i] ? yr[i] : p.y, in && has[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < NJ; ++i) {
-            if (b_left[i] > -(1 << 29)) copy16(base + st + b_to[i], b_left[i] > 0 ? b_from[i] : b, b_left[i] > 0);
-            b_left[i] -= kCols;
-            b_from[i] += kCols * rank;
-        }
-        out_left -= kCols;
-        yr[0] += kCols;
-        yr[1] += kCols;
-    };
-    const int rt = warp & 3, half = warp >> 2;     // the warp's 16 rows, and its half of the rank's or the columns' tiles
-    // (ldmatrix: lanes 0..15 give the rows of the first eight columns, 16..31 those of the next)
-    const int lr = lane & 15, lc = (lane >> 4) * 16;
-    const int total = (k1 - k0) + (n1 - n0);       // both products' stages in one line
-    const uint32_t ring = (uint32_t)(kTileStages * pl.stage);
-    int loaded = 0;
-    uint32_t to_stage = 0, at_stage = 0;           // offsets of the stage to fill next and of the one to use next
-    auto load = [&]() {
-        if (loaded < k1 - k0) load_in(to_stage);
-        else if (loaded < total) load_out(to_stage);
-        copies_commit();
-        ++loaded;
-        to_stage += pl.stage;
-        if (to_stage == ring) to_stage = 0;
-    };
-    auto next_stage = [&]() {
-        at_stage += pl.stage;
-        if (at_stage == ring) at_stage = 0;
-    };
-    for (int i = 0; i < kTileStages - 1; ++i) load();
-    float acc[NJ][8] = {};
-    int it = 0;
-    for (; it < k1 - k0; ++it) {
-        copies_wait<kTileStages - 2>();
-        __syncthreads();
-        load();
-        const uint32_t xs = base + at_stage, as = xs + kTileRows * kColPitch;
-        next_stage();
-#pragma unroll
-        for (int kk = 0; kk < kCols / 16; ++kk) {
-            uint32_t va[4];
-            ldmatrix4(xs + (rt * 16 + lr) * kColPitch + kk * 32 + lc, va);
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-                const int t = half + 2 * j;
-                if (t * 16 >= r16) break;
-                uint32_t vb[4];
-                ldmatrix4(as + (t * 16 + lr) * kColPitch + kk * 32 + lc, vb);
-                float(&d0)[4] = *reinterpret_cast<float(*)[4]>(&acc[j][0]);
-                float(&d1)[4] = *reinterpret_cast<float(*)[4]>(&acc[j][4]);
-                mma(d0, va[0], va[1], va[2], va[3], vb[0], vb[2]);
-                mma(d1, va[0], va[1], va[2], va[3], vb[1], vb[3]);
-            }
-        }
-    }
-    // the low-rank rows: this CTA's part of the sums, then all of them as hi + lo in every CTA
-    const int g = lane >> 2, q = lane & 3;
-    float* sums = reinterpret_cast<float*>(smem + pl.sums_at);
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-        const int t = half + 2 * j;
-        if (t * 16 >= r16) break;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float* d = sums + (rt * 16 + g) * r16 + t * 16 + h * 8 + 2 * q;
-            *reinterpret_cast<float2*>(d) = make_float2(acc[j][4 * h], acc[j][4 * h + 1]);
-            *reinterpret_cast<float2*>(d + 8 * r16) = make_float2(acc[j][4 * h + 2], acc[j][4 * h + 3]);
-        }
-    }
-    if (ctas > 1) cluster_sync();
-    else __syncthreads();
-    const float sc = p.scale != nullptr ? p.scale[id] : 1.f;
-    for (int i = tid * ctas + c; i < kTileRows * pieces; i += kThreads * ctas) {
-        const int r = i / pieces, j = i - r * pieces;
-        float v[8] = {};
-        const uint32_t at = base + pl.sums_at + (uint32_t)(r * r16 + j * 8) * 4u;
-        for (int peer = 0; peer < ctas; ++peer) {
-            const uint32_t from = ctas > 1 ? peer_addr(at, peer) : at;
-            const float4 u = ld_peer4(from), w = ld_peer4(from + 16);
-            v[0] += u.x; v[1] += u.y; v[2] += u.z; v[3] += u.w;
-            v[4] += w.x; v[5] += w.y; v[6] += w.z; v[7] += w.w;
-        }
-        __nv_bfloat16 hi[8], lo[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) split2(v[e] * sc, hi[e], lo[e]);
-        const uint4 vh = make_uint4(pack2(hi[0], hi[1]), pack2(hi[2], hi[3]), pack2(hi[4], hi[5]), pack2(hi[6], hi[7]));
-        const uint4 vl = make_uint4(pack2(lo[0], lo[1]), pack2(lo[2], lo[3]), pack2(lo[4], lo[5]), pack2(lo[6], lo[7]));
-        const uint32_t to = base + (uint32_t)(r * pl.pitch + j * 16);
-        for (int peer = 0; peer < ctas; ++peer) {
-            const uint32_t dst = ctas > 1 ? peer_addr(to, peer) : to;
-            st_peer4(dst + pl.hi_at, vh);
-            st_peer4(dst + pl.lo_at, vl);
-        }
-    }
-    if (ctas > 1) cluster_sync();
-    else __syncthreads();
-    // up to a rank of 64 the low-rank rows stay in registers
-    constexpr int kKept = NJ <= 2 ? 2 * NJ : 0;
-    uint32_t kh[kKept > 0 ? kKept : 1][4], kl[kKept > 0 ? kKept : 1][4];
-    const uint32_t hi_own = base + pl.hi_at + (rt * 16 + lr) * pl.pitch + lc, lo_own = hi_own + pl.lo_at - pl.hi_at;
-#pragma unroll
-    for (int kk = 0; kk < kKept; ++kk)
-        if (kk * 16 < r16) {
-            ldmatrix4(hi_own + kk * 32, kh[kk]);
-            ldmatrix4(lo_own + kk * 32, kl[kk]);
-        }
-    __nv_bfloat16* to_own[2];
-    bool has_own[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int r = rt * 16 + (lane >> 2) + 8 * i;
-        has_own[i] = r < m;
-        to_own[i] = p.out + (size_t)s.rows[has_own[i] ? r : 0] * p.n_out + n0 * kCols + half * 32 + (lane & 3) * 8;
-    }
-    int n = n0 * kCols;                            // first column of the stage
-    for (; it < total; ++it) {
-        copies_wait<kTileStages - 2>();
-        __syncthreads();
-        load();
-        unsigned char* ys_p = smem + at_stage;
-        next_stage();
-        const uint32_t bs = smem_addr(ys_p) + kTileRows * kColPitch + (half * 32 + lr) * pl.pitch + lc;
-        float d[4][4] = {};                   // four tiles of eight columns of the warp's 32
-        auto step = [&](const uint32_t (&vh)[4], const uint32_t (&vl)[4], int kk) {
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                uint32_t vb[4];
-                ldmatrix4(bs + j * 16 * pl.pitch + kk * 32, vb);
-                mma(d[2 * j], vh[0], vh[1], vh[2], vh[3], vb[0], vb[2]);
-                mma(d[2 * j + 1], vh[0], vh[1], vh[2], vh[3], vb[1], vb[3]);
-                mma(d[2 * j], vl[0], vl[1], vl[2], vl[3], vb[0], vb[2]);
-                mma(d[2 * j + 1], vl[0], vl[1], vl[2], vl[3], vb[1], vb[3]);
-            }
-        };
-        if (kKept > 0) {
-#pragma unroll
-            for (int kk = 0; kk < kKept; ++kk)
-                if (kk * 16 < r16) step(kh[kk], kl[kk], kk);
-        } else {
-#pragma unroll 2
-            for (int kk = 0; kk < r16 / 16; ++kk) {
-                uint32_t vh[4], vl[4];
-                ldmatrix4(hi_own + kk * 32, vh);
-                ldmatrix4(lo_own + kk * 32, vl);
-                step(vh, vl, kk);
-            }
-        }
-        if (p.wide) {
-            // added in y's place, out in 16-byte pieces: 16 rows x 32 columns that no other warp touches
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    __nv_bfloat162* at = reinterpret_cast<__nv_bfloat162*>(ys_p + (rt * 16 + g + 8 * h) * kColPitch + (half * 32 + j * 8 + 2 * q) * 2);
-                    const float2 v = __bfloat1622float2(*at);
-                    *at = __floats2bfloat162_rn(v.x + d[j][2 * h], v.y + d[j][2 * h + 1]);
-                }
-            __syncwarp();
-            const int r0 = rt * 16 + (lane >> 2), col = half * 32 + (lane & 3) * 8;
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-                if (has_own[i] && n + col < p.n_out)
-                    *reinterpret_cast<uint4*>(to_own[i]) = *reinterpret_cast<const uint4*>(ys_p + (r0 + 8 * i) * kColPitch + col * 2);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int r = rt * 16 + g + 8 * (e >> 1), col = n + half * 32 + j * 8 + 2 * q + (e & 1);
-                    if (r < m && col < p.n_out) {
-                        const size_t at = (size_t)s.rows[r] * p.n_out + col;
-                        p.out[at] = __float2bfloat16_rn(__bfloat162float(p.y[at]) + d[j][e]);
+    tc::tc_fence_before();
+    __syncthreads();
+    tc::tc_fence_after();
+    const uint32_t tmem = s.tmem_base;
+    const int rank = p.rank, r16 = pl.r16, n_blocks = pl.blocks;
+    constexpr int S = NJ <= 4 ? 5 : 3;                     // (TilePlan::stages)
+    const uint32_t base = tc::smem_u32(smem);
+    // both products' stages in one line, stage i in the place i mod S: x or y, then a or b
+    const int n_in = k1 - k0, total = n_in + (n1 - n0);
+    const int early = NJ <= 4 ? total : n_in;              // (beyond a rank of 128 the second product's wait for the sums to leave)
+    volatile int* abort_flag = &s.abort;
+    int issued = 0;                                        // stages whose a or b is on its way
+
+    if (warp == 9) {
+        int slot = 0;
+        uint32_t ph = 1;                                   // of the MMAs that free the place, the first of which need not be waited for
+        bool ok = true;
+        auto fill = [&](int upto) {
+            for (; issued < upto && ok; ++issued) {
+                ok = tc::mbar_wait(tc::smem_u32(&s.used[slot]), ph, abort_flag, p.spin_limit);
+                if (!ok) break;
+                if (lane == 0) {
+                    const uint32_t to = base + (uint32_t)(slot * pl.stage + kBlock), bar = tc::smem_u32(&s.loaded[slot]);
+                    if (issued < n_in) {
+                        tc::mbar_expect_tx(bar, (uint32_t)(r16 * 128));
+                        tc::tma_load_2d(to, &maps.a, (k0 + issued) * kCols, id * rank, bar);
+                    } else {
+                        tc::mbar_expect_tx(bar, (uint32_t)(n_blocks * kBlock));
+                        for (int kb = 0; kb < n_blocks; ++kb)
+                            tc::tma_load_2d(to + kb * kBlock, &maps.b, kb * 64, id * p.n_out + (n0 + issued - n_in) * kCols, bar);
                     }
                 }
+                __syncwarp();
+                if (++slot == S) {
+                    slot = 0;
+                    ph ^= 1u;
+                }
+            }
+        };
+        // (no further than the places that the first product leaves free; the sums take one, or all, until the cluster has met twice)
+        fill(min(n_in + S - 1, early));
+        if (ctas > 1) cluster_sync();
+        else __syncthreads();
+        if (ctas > 1) cluster_sync();
+        else __syncthreads();
+        fill(total);
+    } else if (warp == 8) {
+        const uint32_t flag = tc::smem_u32(&s.abort);
+        int slot = 0;
+        uint32_t ph = 0;
+        auto next_stage = [&]() {
+            if (++slot == S) {
+                slot = 0;
+                ph ^= 1u;
+            }
+        };
+        for (int i = 0; i < n_in; ++i) {
+            tc::mbar_wait_on(tc::smem_u32(&s.rows_there[slot]), ph, flag, p.spin_limit);
+            tc::mbar_wait_on(tc::smem_u32(&s.loaded[slot]), ph, flag, p.spin_limit);
+            tc::tc_fence_after();
+            const uint32_t st = base + (uint32_t)(slot * pl.stage), idesc = tc::idesc_for(64, r16) | (1u << 7) | (1u << 10);      // bf16
+            if (tc::elect_one()) {
+#pragma unroll
+                for (int kk = 0; kk < kCols / 16; ++kk)
+                    tc::umma_ss(tmem, tc::smem_desc(st) + 2 * kk, tc::smem_desc(st + kBlock) + 2 * kk, idesc, i > 0 || kk > 0 ? 1u : 0u);
+                tc::umma_commit(tc::smem_u32(&s.used[slot]));
+            }
+            __syncwarp();
+            next_stage();
         }
-        n += kCols;
-        to_own[0] += kCols;
-        to_own[1] += kCols;
+        // the low-rank rows are made by the others
+        if (ctas > 1) cluster_sync();
+        else __syncthreads();
+        if (ctas > 1) cluster_sync();
+        else __syncthreads();
+        const uint64_t hi_desc = tc::smem_desc(base + (uint32_t)pl.hi_at), lo_desc = tc::smem_desc(base + (uint32_t)pl.lo_at);
+        const uint32_t idesc = tc::idesc_for(64, kCols) | (1u << 7) | (1u << 10);
+        const int kks = r16 / 16;
+        for (int e = 0; e < total - n_in; ++e) {
+            tc::mbar_wait_on(tc::smem_u32(&s.loaded[slot]), ph, flag, p.spin_limit);
+            if (e >= 2) tc::mbar_wait_on(tc::smem_u32(&s.sums_free[e & 1]), (uint32_t)((e - 2) >> 1) & 1u, flag, p.spin_limit);
+            tc::tc_fence_after();
+            const uint32_t d = tmem + (uint32_t)((e & 1) * 64);
+            const uint64_t b_desc = tc::smem_desc(base + (uint32_t)(slot * pl.stage + kBlock));
+            if (tc::elect_one()) {
+#pragma unroll
+                for (int part = 0; part < 2; ++part)
+#pragma unroll
+                    for (int kk = 0; kk < 2 * NJ; ++kk)
+                        if (kk < kks) {
+                            const uint64_t at = (uint64_t)((kk >> 2) * (kBlock >> 4) + 2 * (kk & 3));
+                            tc::umma_ss(d, (part ? lo_desc : hi_desc) + at, b_desc + at, idesc, part > 0 || kk > 0 ? 1u : 0u);
+                        }
+                tc::umma_commit(tc::smem_u32(&s.used[slot]));
+                tc::umma_commit(tc::smem_u32(&s.sums_there[e & 1]));
+            }
+            __syncwarp();
+            next_stage();
+        }
+    } else {
+        const int rt = warp & 3, half = warp >> 2, g = lane >> 2, q = lane & 3;    // the warp's 16 rows, and its half of the columns
+        auto wait = [&](uint64_t& bar, int phase) { tc::mbar_wait(tc::smem_u32(&bar), (uint32_t)phase & 1u, abort_flag, p.spin_limit); };
+        const float sc = p.scale != nullptr ? p.scale[id] : 1.f;
+        // What a thread copies is the same in every stage but for the columns: a piece of two rows of x, or of y.
+        const int cr = tid >> 3, cc = (tid & 7) * 8;
+        const __nv_bfloat16* xr[2];
+        const __nv_bfloat16* yr[2];
+        __nv_bfloat16* to_own[2];
+        uint32_t y_at[2];                     // of the piece in the stage
+        bool has[2], has_own[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            has[i] = cr + 32 * i < m;
+            xr[i] = p.x + (size_t)s.rows[has[i] ? cr + 32 * i : 0] * p.in + k0 * kCols + cc;
+            const int r = rt * 16 + g + 8 * i;
+            has_own[i] = r < m;
+            const size_t at = (size_t)s.rows[has_own[i] ? r : 0] * p.n_out + n0 * kCols + half * 32 + q * 8;
+            yr[i] = p.y + at;
+            to_own[i] = p.out + at;
+            y_at[i] = (uint32_t)(r * 128 + (((half * 4 + q) ^ (r & 7)) * 16));
+        }
+        const uint32_t x_at = (uint32_t)(cr * 128 + (((tid & 7) ^ (cr & 7)) * 16));
+        int in_left = p.in - k0 * kCols - cc, y_left = p.n_out - n0 * kCols - half * 32 - q * 8;      // columns of x and of y up to the end
+        int next = 0;                         // stage to copy next
+        uint32_t to = base;                   // its place
+        auto copy = [&](int upto) {
+            if (next < upto) {
+                if (next < n_in) {
+                    const bool in = in_left > 0;
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) copy16(to + x_at + i * 32 * 128, in && has[i] ? xr[i] : p.x, in && has[i]);
+                    in_left -= kCols;
+                    xr[0] += kCols;
+                    xr[1] += kCols;
+                } else {
+                    if (p.wide) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            if (y_left > 0 && has_own[i]) copy16(to + y_at[i], yr[i], true);
+                    }
+                    y_left -= kCols;
+                    yr[0] += kCols;
+                    yr[1] += kCols;
+                }
+                ++next;
+                to += pl.stage;
+                if (to == base + (uint32_t)(S * pl.stage)) to = base;
+            }
+            copies_commit();
+        };
+        auto arrived = [&]() {                // the oldest of S - 1 copies
+            if (NJ <= 4) copies_wait<3>();
+            else copies_wait<1>();
+        };
+        for (int i = 0; i < S - 1; ++i) copy(early);
+        for (int i = 0; i < n_in; ++i) {
+            arrived();
+            tc::fence_async_proxy();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s.rows_there[i % S]));
+            if (i > 0) wait(s.used[(i - 1) % S], (i - 1) / S);             // the place of the next copy is free
+            copy(early);
+        }
+        // the low-rank rows: this CTA's part of the sums, then all of them as hi + lo in every CTA
+        auto sums_of = [&](int cta) {         // their place in a CTA
+            return NJ <= 2 ? ((ik * (cta + 1) / ctas - ik * cta / ctas + S - 1) % S) * pl.stage : pl.sums_at;
+        };
+        float* sums = reinterpret_cast<float*>(smem + sums_of(c));
+        if (n_in > 0) wait(s.used[(n_in - 1) % S], (n_in - 1) / S);
+        tc::tc_fence_after();
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            const int t = half + 2 * j;
+            if (t * 16 >= r16) break;
+            float v[8] = {};
+            if (n_in > 0) tmem_ld_16x16(tmem + ((uint32_t)(rt * 32) << 16) + (uint32_t)(t * 16), v);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float* d = sums + (rt * 16 + g) * r16 + t * 16 + h * 8 + 2 * q;
+                *reinterpret_cast<float2*>(d) = make_float2(v[4 * h], v[4 * h + 1]);
+                *reinterpret_cast<float2*>(d + 8 * r16) = make_float2(v[4 * h + 2], v[4 * h + 3]);
+            }
+        }
+        tc::tc_fence_before();
+        if (ctas > 1) cluster_sync();
+        else __syncthreads();
+        const int pieces = r16 / 8;
+        for (int i = tid * ctas + c; i < m * pieces; i += kThreads * ctas) {      // (what is in the other rows reaches no output)
+            const int r = i / pieces, j = i - r * pieces;
+            float v[8] = {};
+            for (int first = 0; first < ctas; first += 4) {
+                float4 u[4], w[4];            // all on their way before the first is added
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (first + k < ctas) {
+                        const uint32_t at = base + (uint32_t)(sums_of(first + k) + (r * r16 + j * 8) * 4), src = ctas > 1 ? peer_addr(at, first + k) : at;
+                        u[k] = ld_peer4(src);
+                        w[k] = ld_peer4(src + 16);
+                    }
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (first + k < ctas) {
+                        v[0] += u[k].x; v[1] += u[k].y; v[2] += u[k].z; v[3] += u[k].w;
+                        v[4] += w[k].x; v[5] += w[k].y; v[6] += w[k].z; v[7] += w[k].w;
+                    }
+            }
+            __nv_bfloat16 hi[8], lo[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) split2(j * 8 < rank ? v[e] * sc : 0.f, hi[e], lo[e]);      // (past the rank: another adapter's)
+            const uint4 vh = make_uint4(pack2(hi[0], hi[1]), pack2(hi[2], hi[3]), pack2(hi[4], hi[5]), pack2(hi[6], hi[7]));
+            const uint4 vl = make_uint4(pack2(lo[0], lo[1]), pack2(lo[2], lo[3]), pack2(lo[4], lo[5]), pack2(lo[6], lo[7]));
+            const uint32_t dst0 = base + (uint32_t)((j >> 3) * kBlock + r * 128 + (((j & 7) ^ (r & 7)) * 16));
+            for (int peer = 0; peer < ctas; ++peer) {
+                const uint32_t dst = ctas > 1 ? peer_addr(dst0, peer) : dst0;
+                st_peer4(dst + pl.hi_at, vh);
+                st_peer4(dst + pl.lo_at, vl);
+            }
+        }
+        asm volatile("fence.proxy.async.shared::cluster;" ::: "memory");   // (what it wrote is read by MMAs, here and in the other CTAs)
+        if (ctas > 1) cluster_sync();
+        else __syncthreads();
+        if (NJ > 4)
+            for (int i = 0; i < S - 1; ++i) copy(total);
+        int n = n0 * kCols;                                // first column of the stage
+        unsigned char* y = smem + (n_in % S) * pl.stage;   // ... and its place
+        for (int e = 0; e < total - n_in; ++e) {
+            wait(s.sums_there[e & 1], e >> 1);
+            tc::tc_fence_after();
+            float d[16];
+            tmem_ld_16x32(tmem + ((uint32_t)(rt * 32) << 16) + (uint32_t)((e & 1) * 64 + half * 32), d);
+            tc::tc_fence_before();
+            arrived();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s.sums_free[e & 1]));
+            if (p.wide) {
+                // added in y's place, out in 16-byte pieces
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int r = rt * 16 + g + 8 * h;
+                        __nv_bfloat162* at = reinterpret_cast<__nv_bfloat162*>(y + r * 128 + (((half * 4 + j) ^ (r & 7)) * 16) + q * 4);
+                        const float2 v = __bfloat1622float2(*at);
+                        *at = __floats2bfloat162_rn(v.x + d[4 * j + 2 * h], v.y + d[4 * j + 2 * h + 1]);
+                    }
+                __syncwarp();
+                const bool in = n + half * 32 + q * 8 < p.n_out;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    if (has_own[h] && in) *reinterpret_cast<uint4*>(to_own[h]) = *reinterpret_cast<const uint4*>(y + y_at[h]);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+#pragma unroll
+                    for (int h = 0; h < 4; ++h) {
+                        const int r = rt * 16 + g + 8 * (h >> 1), col = n + half * 32 + j * 8 + 2 * q + (h & 1);
+                        if (r < m && col < p.n_out) {
+                            const size_t at = (size_t)s.rows[r] * p.n_out + col;
+                            p.out[at] = __float2bfloat16_rn(__bfloat162float(p.y[at]) + d[4 * j + h]);
+                        }
+                    }
+            }
+            n += kCols;
+            to_own[0] += kCols;
+            to_own[1] += kCols;
+            y += pl.stage;
+            if (y == smem + S * pl.stage) y = smem;
+            copy(total);                                   // into the place of the stage before this one, of y if not of x: see above
+        }
+        copies_wait<0>();
     }
-    copies_wait<0>();
+    __syncthreads();
+    if (s.abort != 0) {                                    // a wait ran out: NaN in this CTA's columns
+        if (warp == 8) {
+            if (tc::elect_one()) tc::umma_commit(tc::smem_u32(&s.retired));
+            __syncwarp();
+            tc::mbar_drain(tc::smem_u32(&s.retired), 0u);
+        } else if (warp == 9) {
+            for (int i = max(0, issued - S); i < issued; ++i) tc::mbar_drain(tc::smem_u32(&s.loaded[i % S]), (uint32_t)(i / S) & 1u);
+        }
+        if (tid == 0) atomicExch(p.status, 5);
+        for (int r = warp; r < m; r += kTileThreads / 32)
+            for (int col = n0 * kCols + lane; col < min(n1 * kCols, p.n_out); col += 32)
+                p.out[(size_t)s.rows[r] * p.n_out + col] = __float2bfloat16_rn(__uint_as_float(0x7fc00000u));
+        __syncthreads();
+    }
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmem) : "memory");
 }
 
-int launch_clusters(const void* kernel, unsigned grid, int ctas, size_t smem, cudaStream_t stream, void** args) {
+struct TileKernel {
+    const void* kernel;
+    int nj;
+};
+TileKernel tile_kernel(int rank) {
+    if (rank <= 32) return {(const void*)low_rank_tile_kernel<1>, 1};
+    if (rank <= 64) return {(const void*)low_rank_tile_kernel<2>, 2};
+    if (rank <= 128) return {(const void*)low_rank_tile_kernel<4>, 4};
+    return {(const void*)low_rank_tile_kernel<8>, 8};
+}
+
+int launch_clusters(const void* kernel, unsigned grid, int threads, int ctas, size_t smem, cudaStream_t stream, void** args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     cudaLaunchAttribute attr = {};
@@ -772,43 +923,66 @@ int launch_clusters(const void* kernel, unsigned grid, int ctas, size_t smem, cu
 }
 
 int launch_low_rank(LowRankArgs p, int sms, cudaStream_t stream) {
-    const int rows = p.n, step = rows <= kFewRows || p.count >= kMaxBins ? kFewRows : kBlockRows;
+    const int rows = p.n, step = rows <= kFewRows || p.count >= kMaxBins || (long)p.count * p.n_out > 0x7fffffffL ? kFewRows : kBlockRows;
     const LowRankArgs whole = p;
-    for (int r0 = 0; r0 < rows; r0 += step) {
+    TileMaps maps;
+    if (step != kFewRows) {
+        const int r16 = (p.rank + 15) & ~15;
+        IMX_TRY(encode_tensor_map_2d(p.a, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (size_t)p.count * p.rank, (size_t)p.in, (size_t)p.in * 2, kCols, r16, 128,
+                                     true, &maps.a));
+        IMX_TRY(encode_tensor_map_2d(p.b, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (size_t)p.count * p.n_out, (size_t)p.rank, (size_t)p.rank * 2, 64, kCols, 128,
+                                     true, &maps.b));
+    }
+    for (int r0 = 0; r0 < rows; r0 += step) {   
         p.n = rows - r0 < step ? rows - r0 : step;
         p.x = whole.x + (size_t)r0 * p.in;
         p.y = whole.y + (size_t)r0 * p.n_out;
         p.out = whole.out + (size_t)r0 * p.n_out;
         p.ids = whole.ids + r0;
         int ctas = 1;
-        void* args[] = {&p, &ctas, nullptr};
+        void* args[] = {&p, &ctas, nullptr, nullptr};
         if (step == kFewRows) {
             const FewKernel few = few_kernel(p.rank);
             while (ctas < 8 && p.n * ctas * 2 <= (few.rb <= 2 ? 3 : 2) * sms) ctas *= 2;
             int clusters = 1;
             while (clusters < 16 && p.n * ctas * clusters * 2 <= sms && p.n_out >= 128 * ctas * clusters) clusters *= 2;
             args[2] = &clusters;
-            IMX_TRY(launch_clusters(few.kernel, (unsigned)(p.n * ctas * clusters), ctas, (size_t)FewPlan(p.rank, few.rb).bytes, stream, args));
+            IMX_TRY(launch_clusters(few.kernel, (unsigned)(p.n * ctas * clusters), kThreads, ctas, (size_t)FewPlan(p.rank, few.rb).bytes, stream, args));
             continue;
         }
-        // no more units than these; CTAs for two on every SM
+        // no more units than these; CTAs for two on every SM: clusters of up to eight for a unit, then several of them
         const int units = p.n / kTileRows + (p.count + 1 < p.n ? p.count + 1 : p.n);
         while (ctas < 8 && units * ctas * 2 <= 2 * sms) ctas *= 2;
-        const void* kernel = p.rank <= 32 ? (const void*)low_rank_tile_kernel<1> : (p.rank <= 64 ? (const void*)low_rank_tile_kernel<2>
-                                          : (p.rank <= 128 ? (const void*)low_rank_tile_kernel<4> : (const void*)low_rank_tile_kernel<8>));
-        IMX_TRY(launch_clusters(kernel, (unsigned)(units * ctas), ctas, (size_t)TilePlan(p.rank).bytes, stream, args));
+        int clusters = 1;
+        while (clusters < 8 && units * ctas * clusters * 2 <= 2 * sms && p.n_out >= 2 * kCols * ctas * clusters) clusters *= 2;
+        const TileKernel tile = tile_kernel(p.rank);
+        args[2] = &clusters;
+        args[3] = &maps;
+        IMX_TRY(launch_clusters(tile.kernel, (unsigned)(units * ctas * clusters), kTileThreads, ctas, (size_t)TilePlan(p.rank, tile.nj).bytes + 1024, stream, args));
     }
     return IMX_OK;
 }
 
 }  // namespace
 
+// Test hook (include/ironmlx_b200_testing.h).
+void testing_low_rank_give_up(int on) { g_low_rank_spin_limit.store(on ? 0 : kSpin); }
+
 }  // namespace imx
 
 using namespace imx;
 
+extern "C" void imx_testing_low_rank_give_up(int on) { testing_low_rank_give_up(on); }
+
+extern "C" int imx_low_rank_scratch_bytes(int n_rows, int in, int n_out, int count, int rank, size_t* bytes) {
+    IMX_REQUIRE(bytes != nullptr && n_rows >= 0 && in > 0 && n_out > 0 && count > 0 && rank > 0 && rank <= kMaxRank,
+                "low_rank_scratch_bytes: bad arguments");
+    *bytes = kStatusBytes;
+    return IMX_OK;
+}
+
 extern "C" int imx_low_rank_add(const void* y, const void* x, int n_rows, int in, const imx_adapters* ad, const int32_t* ids, int n_out,
-                                void* out, void* stream) {
+                                void* out, void* scratch, size_t scratch_bytes, void* stream) {
     IMX_REQUIRE(n_rows >= 0 && n_out > 0 && in > 0 && in % 8 == 0,
                 "low_rank_add: sizes (%d rows, %d -> %d) must be positive, the input dimension a multiple of 8", n_rows, in, n_out);
     if (n_rows == 0) return IMX_OK;
@@ -819,26 +993,30 @@ extern "C" int imx_low_rank_add(const void* y, const void* x, int n_rows, int in
     IMX_REQUIRE((((uintptr_t)x | (uintptr_t)ad->a | (uintptr_t)ad->b) % 16) == 0, "low_rank_add: x, a and b must be 16-byte aligned");
     IMX_REQUIRE((((uintptr_t)ids | (uintptr_t)ad->scale) % 4) == 0, "low_rank_add: ids and scale must be aligned to their values");
     IMX_REQUIRE((((uintptr_t)y | (uintptr_t)out) % 2) == 0, "low_rank_add: y and out must be aligned to their bf16 values");
+    if (scratch == nullptr || (uintptr_t)scratch % 256 != 0 || scratch_bytes < kStatusBytes) {
+        set_error("low_rank_add: 256-byte aligned scratch of %zu bytes needed, %zu given", kStatusBytes, scratch_bytes);
+        return IMX_ERR_WORKSPACE;
+    }
     const size_t ob = (size_t)n_rows * n_out * 2;
     IMX_REQUIRE(out == y || !overlap(out, ob, y, ob), "low_rank_add: out overlaps y without being it");
     IMX_REQUIRE(!overlap(out, ob, x, (size_t)n_rows * in * 2) && !overlap(out, ob, ids, (size_t)n_rows * 4) &&
                 !overlap(out, ob, ad->a, (size_t)ad->count * ad->rank * in * 2) &&
                 !overlap(out, ob, ad->b, (size_t)ad->count * ad->rank * n_out * 2) &&
-                !overlap(out, ob, ad->scale, (size_t)ad->count * 4), "low_rank_add: out overlaps another array");
+                !overlap(out, ob, ad->scale, (size_t)ad->count * 4) && !overlap(out, ob, scratch, kStatusBytes), "low_rank_add: out overlaps another array");
     DeviceInfo di;
     IMX_TRY(current_device(&di));
     if (device_needs_setup(di.ordinal, kSetupLowRank)) {     // once per device
-        const void* kernels[4] = {(const void*)low_rank_tile_kernel<1>, (const void*)low_rank_tile_kernel<2>, (const void*)low_rank_tile_kernel<4>,
-                                  (const void*)low_rank_tile_kernel<8>};
-        for (int i = 0; i < 4; ++i) IMX_CHECK_CUDA(cudaFuncSetAttribute(kernels[i], cudaFuncAttributeMaxDynamicSharedMemorySize, TilePlan(32 << i).bytes));
         for (int rank : {8, 16, 32, 64, 128, 256}) {
             const FewKernel few = few_kernel(rank);
             IMX_CHECK_CUDA(cudaFuncSetAttribute(few.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FewPlan(rank, few.rb).bytes));
+            const TileKernel tile = tile_kernel(rank);
+            IMX_CHECK_CUDA(cudaFuncSetAttribute(tile.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TilePlan(rank, tile.nj).bytes + 1024));
         }
         device_mark_setup(di.ordinal, kSetupLowRank);
     }
     const int wide = n_out % 8 == 0 && (((uintptr_t)y | (uintptr_t)out) % 16) == 0;
     return launch_low_rank(LowRankArgs{(const __nv_bfloat16*)y, (const __nv_bfloat16*)x, (const __nv_bfloat16*)ad->a, (const __nv_bfloat16*)ad->b,
-                                       ad->scale, ids, (__nv_bfloat16*)out, n_rows, in, n_out, ad->count, ad->rank, wide},
+                                       ad->scale, ids, (__nv_bfloat16*)out, n_rows, in, n_out, ad->count, ad->rank, wide,
+                                       g_low_rank_spin_limit.load(), (int32_t*)scratch},
                            di.sms, (cudaStream_t)stream);
 }

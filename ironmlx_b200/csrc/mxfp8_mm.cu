@@ -162,29 +162,6 @@ __device__ __forceinline__ uint4 row_scales(const uint8_t* row, int group, int b
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
-// Wait of the warp that issues the MMAs.  Its outcome must not steer the code: the compiler would take all that follows for
-// divergent and move the operands of every MMA to uniform registers, 50 cycles each.  So an expired wait sets the abort flag,
-// the later ones return at once, and what is then multiplied is never used.
-__device__ __forceinline__ void mbar_wait_on(uint32_t bar, uint32_t parity, uint32_t abort_flag, int limit) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .u32 n, f;\n\t"
-        "mov.u32 n, %3;\n"
-        "try_again:\n\t"
-        "setp.eq.u32 p, n, 0;\n\t"
-        "@p bra expired;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%0], %1;\n\t"
-        "@p bra arrived;\n\t"
-        "sub.u32 n, n, 1;\n\t"
-        "ld.volatile.shared.u32 f, [%2];\n\t"
-        "setp.eq.u32 p, f, 0;\n\t"
-        "@p bra try_again;\n"
-        "expired:\n\t"
-        "st.volatile.shared.u32 [%2], 1;\n"
-        "arrived:\n\t}"
-        ::"r"(bar), "r"(parity), "r"(abort_flag), "r"(limit)
-        : "memory");
-}
-
 // Four values of an output row, whatever of them lies below n_out.
 __device__ __forceinline__ void store4(__nv_bfloat16* y, size_t row, int n, int n_out, float4 v, bool whole) {
     __nv_bfloat16* at = y + row * n_out + n;

@@ -62,6 +62,29 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
     *abort_flag = 1;
     return false;
 }
+// Wait of the warp that issues the MMAs.  Its outcome must not steer the code: the compiler would take all that follows for
+// divergent and move the operands of every MMA to uniform registers, 50 cycles each.  So an expired wait sets the abort flag,
+// the later ones return at once, and what is then multiplied is never used.
+__device__ __forceinline__ void mbar_wait_on(uint32_t bar, uint32_t parity, uint32_t abort_flag, int limit) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .u32 n, f;\n\t"
+        "mov.u32 n, %3;\n"
+        "try_again:\n\t"
+        "setp.eq.u32 p, n, 0;\n\t"
+        "@p bra expired;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%0], %1;\n\t"
+        "@p bra arrived;\n\t"
+        "sub.u32 n, n, 1;\n\t"
+        "ld.volatile.shared.u32 f, [%2];\n\t"
+        "setp.eq.u32 p, f, 0;\n\t"
+        "@p bra try_again;\n"
+        "expired:\n\t"
+        "st.volatile.shared.u32 [%2], 1;\n"
+        "arrived:\n\t}"
+        ::"r"(bar), "r"(parity), "r"(abort_flag), "r"(limit)
+        : "memory");
+}
+
 // The wait for what is still in flight once a kernel has given up: bounded too, and nothing follows from it.
 __device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
     for (int spin = 0; spin < kSpin && !mbar_try_wait(bar, parity); ++spin) {}

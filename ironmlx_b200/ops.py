@@ -281,7 +281,7 @@ _STATUS = {}
 
 
 def _status_block(index: int) -> torch.Tensor:
-    """The status block of a device's `mxfp8_matmul` calls: zero-filled once, kernels only ever set its first word."""
+    """The status block of a device's `mxfp8_matmul` and `low_rank_add` calls: zero-filled once, kernels only ever set its first word."""
     buf = _STATUS.get(index)
     if buf is None:
         buf = torch.zeros(256, dtype=torch.uint8, device=torch.device("cuda", index))
@@ -292,7 +292,7 @@ def _status_block(index: int) -> torch.Tensor:
 
 
 def check_status(device=None, stream=None) -> None:
-    """Raises if a bounded wait ran out in an `mxfp8_matmul` call on the device (default: the current one) since the last
+    """Raises if a bounded wait ran out in an `mxfp8_matmul` or `low_rank_add` call on the device (default: the current one) since the last
     check; synchronises the stream."""
     index = torch.device("cuda" if device is None else device).index
     buf = _STATUS.get(torch.cuda.current_device() if index is None else index)
@@ -359,6 +359,7 @@ def low_rank_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
     if out is None:
         out = torch.empty_like(y)
     ad = _lib.Adapters(a.data_ptr(), b.data_ptr(), None if scale is None else scale.data_ptr(), count, rank)
+    index = x.get_device()
     check(lib().imx_low_rank_add(y.data_ptr(), x.data_ptr(), rows, in_dim, C.byref(ad), ids.data_ptr(), n_out, out.data_ptr(),
-                                 _raw_stream(x.get_device())))
+                                 _status_block(index).data_ptr(), 256, _raw_stream(index)))
     return out

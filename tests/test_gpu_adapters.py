@@ -40,7 +40,7 @@ def run(p, ids, **kw):
 @pytest.mark.parametrize("t,k,n,count,rank", [
     (1, 2048, 8192, 1, 16), (1, 8, 1, 1, 8), (2, 64, 7, 3, 8), (5, 4096, 2048, 4, 64), (16, 2048, 512, 40, 32), (48, 4096, 2048, 40, 32),
     (31, 1000, 1001, 2, 24), (64, 512, 264, 64, 256), (100, 2048, 1024, 3, 128), (130, 96, 200, 5, 16), (300, 2048, 2048, 1, 16),
-    (777, 2056, 1032, 5, 40), (1100, 512, 513, 12, 64), (2050, 256, 384, 200, 8), (600, 4096, 136, 2, 256), (5000, 64, 96, 3, 16)])
+    (777, 2056, 1032, 5, 40), (1100, 512, 513, 12, 64), (140, 8, 16, 1, 8), (131, 200, 72, 3, 200), (8500, 128, 200, 9, 48), (150, 64, 128, 2500, 8), (2050, 256, 384, 200, 8), (600, 4096, 136, 2, 256), (5000, 64, 96, 3, 16), (400, 1024, 2048, 2, 128), (260, 3000, 1500, 1, 256)])
 @pytest.mark.parametrize("order", ["mixed", "runs"])
 def test_low_rank_add(cuda, t, k, n, count, rank, order):
     g = gen(t + k + n + rank)
@@ -102,11 +102,30 @@ def test_low_rank_add_at_any_place(cuda, t, n, at):
     src[at:at + t * n] = p["y"].flatten()
     buf = torch.full((t * n + 16,), 7.0, dtype=torch.bfloat16, device=cuda)
     ad = _lib.Adapters(p["a"].data_ptr(), p["b"].data_ptr(), p["scale"].data_ptr(), 4, 16)
+    scratch = torch.zeros(256, dtype=torch.uint8, device=cuda)
     for dst in (buf, src):
         _lib.check(_lib.lib().imx_low_rank_add(src.data_ptr() + 2 * at, p["x"].data_ptr(), t, 128, C.byref(ad), ids.data_ptr(), n,
-                                               dst.data_ptr() + 2 * at, torch.cuda.current_stream().cuda_stream))
+                                               dst.data_ptr() + 2 * at, scratch.data_ptr(), 256, torch.cuda.current_stream().cuda_stream))
         assert torch.equal(dst[at:at + t * n].view(t, n), want)
         assert (dst[:at] == dst[0]).all() and (dst[at + t * n:] == dst[0]).all()
+
+
+def test_expired_wait_gives_nan_and_a_status(cuda):
+    g = gen(19)
+    p = make(g, 400, 512, 520, 3, 32)
+    ids = torch.randint(-1, 3, (400,), generator=g, device="cuda", dtype=torch.int32)
+    want = run(p, ids)
+    _lib.lib().imx_testing_low_rank_give_up(1)
+    try:
+        out = run(p, ids)
+        torch.cuda.synchronize()
+    finally:
+        _lib.lib().imx_testing_low_rank_give_up(0)
+    assert out[ids >= 0].isnan().all() and torch.equal(out[ids < 0], p["y"][ids < 0])
+    with pytest.raises(_lib.IronMLXError):
+        ops.check_status(cuda)
+    assert torch.equal(run(p, ids), want)
+    ops.check_status(cuda)
 
 
 def test_adapters_on_streams(cuda):

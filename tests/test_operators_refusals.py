@@ -53,9 +53,9 @@ def test_mxfp8_matmul_refuses_scratch(kw):
     refused(product(**kw), b"scratch", _lib.ERR_WORKSPACE)
 
 
-def low_rank(y=A, x=B, n=4, n_in=64, a=D, b=D + 0x1000000, scale=None, count=3, rank=8, ids=E, n_out=64, out=F):
+def low_rank(y=A, x=B, n=4, n_in=64, a=D, b=D + 0x1000000, scale=None, count=3, rank=8, ids=E, n_out=64, out=F, scratch=G, nb=256):
     ad = _lib.Adapters(a, b, scale, count, rank)
-    return _lib.lib().imx_low_rank_add(y, x, n, n_in, C.byref(ad), ids, n_out, out, None)
+    return _lib.lib().imx_low_rank_add(y, x, n, n_in, C.byref(ad), ids, n_out, out, scratch, nb, None)
 
 
 @pytest.mark.parametrize("kw,needle", [
@@ -66,10 +66,15 @@ def low_rank(y=A, x=B, n=4, n_in=64, a=D, b=D + 0x1000000, scale=None, count=3, 
     (dict(x=B + 8), b"aligned"), (dict(a=D + 2), b"aligned"), (dict(b=D + 0x1000008), b"aligned"), (dict(y=A + 1), b"aligned"),
     (dict(out=F + 1), b"aligned"), (dict(ids=E + 2), b"aligned"), (dict(out=A + 2), b"without being it"), (dict(out=B), b"overlaps"),
     (dict(out=E), b"overlaps"), (dict(out=D + 16), b"overlaps"), (dict(out=D + 0x1000010), b"overlaps"),
-    (dict(scale=F + 4), b"overlaps"),
+    (dict(scale=F + 4), b"overlaps"), (dict(out=G), b"overlaps"),
 ])
 def test_low_rank_add_refuses(kw, needle):
     refused(low_rank(**kw), needle)
+
+
+@pytest.mark.parametrize("kw", [dict(scratch=None), dict(scratch=G + 64), dict(nb=0)])
+def test_low_rank_add_refuses_scratch(kw):
+    refused(low_rank(**kw), b"scratch", _lib.ERR_WORKSPACE)
 
 
 def test_no_rows_are_no_work():
@@ -85,6 +90,9 @@ def test_scratch_sizes():
     assert lib.imx_mxfp8_matmul_scratch_bytes(5, 100, 64, C.byref(nb)) == 0 and nb.value >= 256
     refused(lib.imx_mxfp8_matmul_scratch_bytes(5, 100, 60, C.byref(nb)), b"bad arguments")
     refused(lib.imx_mxfp8_matmul_scratch_bytes(5, 100, 64, None), b"bad arguments")
+    assert lib.imx_low_rank_scratch_bytes(5, 64, 64, 2, 8, C.byref(nb)) == 0 and nb.value >= 256
+    refused(lib.imx_low_rank_scratch_bytes(5, 64, 64, 0, 8, C.byref(nb)), b"bad arguments")
+    refused(lib.imx_low_rank_scratch_bytes(5, 64, 64, 1, 512, C.byref(nb)), b"bad arguments")
 
 
 def test_python_layer_refuses_host_tensors_and_other_formats():
