@@ -943,11 +943,12 @@ int launch_low_rank(LowRankArgs p, int sms, cudaStream_t stream) {
         void* args[] = {&p, &ctas, nullptr, nullptr};
         if (step == kFewRows) {
             const FewKernel few = few_kernel(p.rank);
-            while (ctas < 8 && p.n * ctas * 2 <= (few.rb <= 2 ? 3 : 2) * sms) ctas *= 2;
+            const int ids = p.count < p.n ? p.count + 1 : p.n, bound = p.n / kFewUnit + ids, units = bound < p.n ? bound : p.n;
+            while (ctas < 8 && units * ctas * 2 <= (few.rb <= 2 ? 3 : 2) * sms) ctas *= 2;
             int clusters = 1;
-            while (clusters < 16 && p.n * ctas * clusters * 2 <= sms && p.n_out >= 128 * ctas * clusters) clusters *= 2;
+            while (clusters < 16 && units * ctas * clusters * 2 <= sms && p.n_out >= 128 * ctas * clusters) clusters *= 2;
             args[2] = &clusters;
-            IMX_TRY(launch_clusters(few.kernel, (unsigned)(p.n * ctas * clusters), kThreads, ctas, (size_t)FewPlan(p.rank, few.rb).bytes, stream, args));
+            IMX_TRY(launch_clusters(few.kernel, (unsigned)(units * ctas * clusters), kThreads, ctas, (size_t)FewPlan(p.rank, few.rb).bytes, stream, args));
             continue;
         }
         // no more units than these; CTAs for two on every SM: clusters of up to eight for a unit, then several of them
