@@ -491,6 +491,16 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
     const TilePlan pl(p.rank, NJ);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int cluster = blockIdx.x / ctas, unit = cluster / clusters, c = ctas > 1 ? (int)cluster_rank() : 0;
+    // First of all the tensor memory: an SM starts its second CTA only when the first has given up the permit to allocate (with
+    // the allocation behind the ids half of the CTAs of 8192 rows started 6.7 us late, of 777 rows 3.2).
+    constexpr uint32_t kTmem = NJ == 8 ? 256 : 128;        // the first product's sums, in their place two of a stage of the second
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&s.tmem_base)), "r"(kTmem) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    auto give_back = [&]() {
+        if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(s.tmem_base), "r"(kTmem) : "memory");
+    };
     // Units of this block of rows: adapter 0's rows in tiles of 64, adapter 1's, ..., at last the rows without one.  A warp
     // has an eighth of the ids, 32 at a time in batch order, all of them in registers: as loads of the loops below, one after
     // the other, they took 22 us.
@@ -566,7 +576,10 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
     }
     __syncthreads();
     const int m = s.n_rows, id = s.id, skip = s.first;
-    if (m == 0) return;                       // fewer units than clusters: the whole cluster leaves
+    if (m == 0) {                             // fewer units than clusters: the whole cluster leaves
+        give_back();
+        return;
+    }
     {
         // the unit's rows: those of the bin from the skip-th on, in batch order
         unsigned hit[kIds];
@@ -583,13 +596,17 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
             n += __popc(hit[i]);
         });
     }
+    tc::tc_fence_before();
     __syncthreads();
+    tc::tc_fence_after();
+    const uint32_t tmem = s.tmem_base;
     // chunks of the input and of the output dimension that this CTA takes
     const int ik = (p.in + kCols - 1) / kCols, on = (p.n_out + kCols - 1) / kCols;
     const int part_of = (cluster - unit * clusters) * ctas + c;
     const int k0 = ik * c / ctas, k1 = ik * (c + 1) / ctas;
     const int n0 = (int)((long)on * part_of / (ctas * clusters)), n1 = (int)((long)on * (part_of + 1) / (ctas * clusters));
     if (id == p.count) {
+        give_back();
         if (p.out != p.y)
             for (int r = warp; r < m; r += kTileThreads / 32) {
                 const size_t at = (size_t)s.rows[r] * p.n_out;
@@ -601,15 +618,6 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
             }
         return;
     }
-    constexpr uint32_t kTmem = NJ == 8 ? 256 : 128;        // the first product's sums, in their place two of a stage of the second
-    if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&s.tmem_base)), "r"(kTmem) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    tc::tc_fence_before();
-    __syncthreads();
-    tc::tc_fence_after();
-    const uint32_t tmem = s.tmem_base;
     const int rank = p.rank, r16 = pl.r16, n_blocks = pl.blocks;
     constexpr int S = NJ <= 4 ? 5 : 3;                     // (TilePlan::stages)
     const uint32_t base = tc::smem_u32(smem);
@@ -793,36 +801,32 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
         if (ctas > 1) cluster_sync();
         else __syncthreads();
         const int pieces = r16 / 8;
-        for (int i = tid * ctas + c; i < m * pieces; i += kThreads * ctas) {      // (what is in the other rows reaches no output)
-            const int r = i / pieces, j = i - r * pieces;
+        // A CTA makes every ctas-th piece of eight values, ctas lanes one: each brings a CTA's part, they add them by a tree (the
+        // order is the same for all), and each writes the piece into one CTA.  By one lane it took 2.3 us, twice as long.
+        const int shift = 31 - __clz(ctas), peer = lane & (ctas - 1), parts_at = sums_of(peer);
+        for (int li = tid >> shift; (li - (lane >> shift)) * ctas + c < m * pieces; li += kThreads >> shift) {       // (what is in the other rows reaches no output)
+            const int i = li * ctas + c, r = i / pieces, j = i - r * pieces;
+            const bool mine = i < m * pieces;
             float v[8] = {};
-            for (int first = 0; first < ctas; first += 4) {
-                float4 u[4], w[4];            // all on their way before the first is added
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (first + k < ctas) {
-                        const uint32_t at = base + (uint32_t)(sums_of(first + k) + (r * r16 + j * 8) * 4), src = ctas > 1 ? peer_addr(at, first + k) : at;
-                        u[k] = ld_peer4(src);
-                        w[k] = ld_peer4(src + 16);
-                    }
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    if (first + k < ctas) {
-                        v[0] += u[k].x; v[1] += u[k].y; v[2] += u[k].z; v[3] += u[k].w;
-                        v[4] += w[k].x; v[5] += w[k].y; v[6] += w[k].z; v[7] += w[k].w;
-                    }
+            if (mine) {
+                const uint32_t at = base + (uint32_t)(parts_at + (r * r16 + j * 8) * 4), src = ctas > 1 ? peer_addr(at, peer) : at;
+                const float4 u = ld_peer4(src), w = ld_peer4(src + 16);
+                v[0] = u.x; v[1] = u.y; v[2] = u.z; v[3] = u.w;
+                v[4] = w.x; v[5] = w.y; v[6] = w.z; v[7] = w.w;
             }
+            for (int d = 1; d < ctas; d *= 2)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] += __shfl_xor_sync(0xffffffffu, v[e], d);
+            if (!mine) continue;
             __nv_bfloat16 hi[8], lo[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) split2(j * 8 < rank ? v[e] * sc : 0.f, hi[e], lo[e]);      // (past the rank: another adapter's)
             const uint4 vh = make_uint4(pack2(hi[0], hi[1]), pack2(hi[2], hi[3]), pack2(hi[4], hi[5]), pack2(hi[6], hi[7]));
             const uint4 vl = make_uint4(pack2(lo[0], lo[1]), pack2(lo[2], lo[3]), pack2(lo[4], lo[5]), pack2(lo[6], lo[7]));
             const uint32_t dst0 = base + (uint32_t)((j >> 3) * kBlock + r * 128 + (((j & 7) ^ (r & 7)) * 16));
-            for (int peer = 0; peer < ctas; ++peer) {
-                const uint32_t dst = ctas > 1 ? peer_addr(dst0, peer) : dst0;
-                st_peer4(dst + pl.hi_at, vh);
-                st_peer4(dst + pl.lo_at, vl);
-            }
+            const uint32_t dst = ctas > 1 ? peer_addr(dst0, peer) : dst0;
+            st_peer4(dst + pl.hi_at, vh);
+            st_peer4(dst + pl.lo_at, vl);
         }
         asm volatile("fence.proxy.async.shared::cluster;" ::: "memory");   // (what it wrote is read by MMAs, here and in the other CTAs)
         if (ctas > 1) cluster_sync();
@@ -892,7 +896,7 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
                 p.out[(size_t)s.rows[r] * p.n_out + col] = __float2bfloat16_rn(__uint_as_float(0x7fc00000u));
         __syncthreads();
     }
-    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmem) : "memory");
+    give_back();
 }
 
 struct TileKernel {
