@@ -45,11 +45,6 @@ struct LowRankArgs {
     int32_t* status;
 };
 
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-    return r;
-}
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
@@ -180,14 +175,14 @@ low_rank_few_kernel(const LowRankArgs p, const int ctas, const int clusters) {
     extern __shared__ __align__(16) unsigned char dyn[];
     constexpr int kPiece = kThreads * 16;     // bytes between a lane's pieces
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
-    const int c = ctas > 1 ? (int)cluster_rank() : 0;
+    const int c = (int)blockIdx.x & (ctas - 1);
     int id = -1;
-    const int cluster = blockIdx.x / ctas, unit = cluster / clusters;
-    const int m = find_unit(p, s, unit, id);
+    const int shift = 31 - __clz(ctas), cut = shift + 31 - __clz(clusters);       // (both are powers of two)
+    const int m = find_unit(p, s, (int)blockIdx.x >> cut, id);
     if (m == 0) return;                       // fewer units than clusters: the whole cluster leaves
     // output columns of this CTA, in tiles of eight
-    const int tiles = (p.n_out + 7) / 8, part_of = (cluster - unit * clusters) * ctas + c;
-    const int t0 = (int)((long)tiles * part_of / (ctas * clusters)), t1 = (int)((long)tiles * (part_of + 1) / (ctas * clusters));
+    const int tiles = (p.n_out + 7) / 8, part_of = (int)blockIdx.x & ((1 << cut) - 1);
+    const int t0 = (int)((long)tiles * part_of >> cut), t1 = (int)((long)tiles * (part_of + 1) >> cut);
     if (id < 0) {
         if (p.out != p.y)
             for (int r = 0; r < m; ++r) {
@@ -215,7 +210,7 @@ low_rank_few_kernel(const LowRankArgs p, const int ctas, const int clusters) {
     float acc[TP][4] = {};
     {
         constexpr int kPieces = TP + 2, kDepth = ring_pieces(RB) / kPieces;
-        const int blocks = (p.in + 31) / 32, b0 = blocks * c / ctas, b1 = blocks * (c + 1) / ctas;
+        const int blocks = (p.in + 31) / 32, b0 = (int)((long)blocks * c >> shift), b1 = (int)((long)blocks * (c + 1) >> shift);
         const int n = (b1 - b0 - wk + kWk - 1) / kWk;                     // blocks of this warp
         int k = (b0 + wk) * 32 + q * 8;                                   // of the next load
         const __nv_bfloat16* x0 = p.x + (size_t)row0 * p.in + k;
@@ -490,7 +485,8 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
     unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     const TilePlan pl(p.rank, NJ);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int cluster = blockIdx.x / ctas, unit = cluster / clusters, c = ctas > 1 ? (int)cluster_rank() : 0;
+    const int shift = 31 - __clz(ctas), cut = shift + 31 - __clz(clusters);       // (both are powers of two)
+    const int unit = (int)blockIdx.x >> cut, c = (int)blockIdx.x & (ctas - 1);
     // First of all the tensor memory: an SM starts its second CTA only when the first has given up the permit to allocate (with
     // the allocation behind the ids half of the CTAs of 8192 rows started 6.7 us late, of 777 rows 3.2).
     constexpr uint32_t kTmem = NJ == 8 ? 256 : 128;        // the first product's sums, in their place two of a stage of the second
@@ -543,16 +539,18 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     __syncthreads();
-    // (votes first, all at once: one after the other with what follows from them they took 200 cycles each)
-    unsigned whole = 0;                       // groups of 32 inside a prompt
-    lots([&](int i) { whole |= (unsigned)__all_sync(0xffffffffu, bin[i] == __shfl_sync(0xffffffffu, bin[i], 0)) << i; });
+    // A group of 32 inside a prompt is one addition, lane i's for group i, all groups of an adapter's one; the ids of the others
+    // are added one by one.  (One after the other the groups took 120 cycles each.)
+    int all = -1;                             // the adapter of the whole of group `lane`
     lots([&](int i) {
-        if (whole >> i & 1u) {
-            if (lane == 0 && bin[i] >= 0) atomicAdd(&bins[bin[i]], 32);
-        } else {
-            const unsigned alike = __match_any_sync(0xffffffffu, bin[i]);
-            if (bin[i] >= 0 && lane == __ffs(alike) - 1) atomicAdd(&bins[bin[i]], __popc(alike));
-        }
+        const int first = __shfl_sync(0xffffffffu, bin[i], 0);
+        const bool whole = __all_sync(0xffffffffu, bin[i] == first);
+        if (whole && lane == i) all = first;
+    });
+    const unsigned alike = __match_any_sync(0xffffffffu, all), whole = __ballot_sync(0xffffffffu, all >= 0);
+    if (all >= 0 && lane == __ffs(alike) - 1) atomicAdd(&bins[all], 32 * __popc(alike));
+    lots([&](int i) {
+        if (!(whole >> i & 1u) && bin[i] >= 0) atomicAdd(&bins[bin[i]], 1);
     });
     __syncthreads();
     if (warp == 0) {
@@ -581,20 +579,30 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
         return;
     }
     {
-        // the unit's rows: those of the bin from the skip-th on, in batch order
-        unsigned hit[kIds];
-        int n = 0;
-        lots([&](int i) { hit[i] = __ballot_sync(0xffffffffu, bin[i] == id); });
-        lots([&](int i) { n += __popc(hit[i]); });
-        if (lane == 0 && warp < 8) s.warp_count[warp] = n;
-        __syncthreads();
-        n = -skip;
-        for (int w = 0; w < warp; ++w) n += s.warp_count[w];
+        // the unit's rows: those of the bin from the skip-th on, in batch order; lane i has group i
+        unsigned hit = 0;
         lots([&](int i) {
-            const int at = n + __popc(hit[i] & ((1u << lane) - 1u));
-            if ((hit[i] >> lane & 1u) && at >= 0 && at < m) s.rows[at] = from + i * 32 + lane;
-            n += __popc(hit[i]);
+            const unsigned h = __ballot_sync(0xffffffffu, bin[i] == id);
+            if (lane == i) hit = h;
         });
+        int up_to = __popc(hit);
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+            const int v = __shfl_up_sync(0xffffffffu, up_to, o);
+            if (lane >= o) up_to += v;
+        }
+        if (lane == 31 && warp < 8) s.warp_count[warp] = up_to;
+        __syncthreads();
+        int start = up_to - __popc(hit) - skip;
+        for (int w = 0; w < min(warp, 8); ++w) start += s.warp_count[w];
+        unsigned todo = __ballot_sync(0xffffffffu, hit != 0 && start < m && start + __popc(hit) > 0);
+        while (todo != 0) {
+            const int i = __ffs(todo) - 1;
+            todo &= todo - 1;
+            const unsigned h = __shfl_sync(0xffffffffu, hit, i);
+            const int at = __shfl_sync(0xffffffffu, start, i) + __popc(h & ((1u << lane) - 1u));
+            if ((h >> lane & 1u) && at >= 0 && at < m) s.rows[at] = from + i * 32 + lane;
+        }
     }
     tc::tc_fence_before();
     __syncthreads();
@@ -602,9 +610,9 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
     const uint32_t tmem = s.tmem_base;
     // chunks of the input and of the output dimension that this CTA takes
     const int ik = (p.in + kCols - 1) / kCols, on = (p.n_out + kCols - 1) / kCols;
-    const int part_of = (cluster - unit * clusters) * ctas + c;
-    const int k0 = ik * c / ctas, k1 = ik * (c + 1) / ctas;
-    const int n0 = (int)((long)on * part_of / (ctas * clusters)), n1 = (int)((long)on * (part_of + 1) / (ctas * clusters));
+    const int part_of = (int)blockIdx.x & ((1 << cut) - 1);
+    const int k0 = (int)((long)ik * c >> shift), k1 = (int)((long)ik * (c + 1) >> shift);
+    const int n0 = (int)((long)on * part_of >> cut), n1 = (int)((long)on * (part_of + 1) >> cut);
     if (id == p.count) {
         give_back();
         if (p.out != p.y)
@@ -779,7 +787,7 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
         }
         // the low-rank rows: this CTA's part of the sums, then all of them as hi + lo in every CTA
         auto sums_of = [&](int cta) {         // their place in a CTA
-            return NJ <= 2 ? ((ik * (cta + 1) / ctas - ik * cta / ctas + S - 1) % S) * pl.stage : pl.sums_at;
+            return NJ <= 2 ? (((int)((long)ik * (cta + 1) >> shift) - (int)((long)ik * cta >> shift) + S - 1) % S) * pl.stage : pl.sums_at;
         };
         float* sums = reinterpret_cast<float*>(smem + sums_of(c));
         if (n_in > 0) wait(s.used[(n_in - 1) % S], (n_in - 1) / S);
@@ -803,7 +811,7 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
         const int pieces = r16 / 8;
         // A CTA makes every ctas-th piece of eight values, ctas lanes one: each brings a CTA's part, they add them by a tree (the
         // order is the same for all), and each writes the piece into one CTA.  By one lane it took 2.3 us, twice as long.
-        const int shift = 31 - __clz(ctas), peer = lane & (ctas - 1), parts_at = sums_of(peer);
+        const int peer = lane & (ctas - 1), parts_at = sums_of(peer);
         for (int li = tid >> shift; (li - (lane >> shift)) * ctas + c < m * pieces; li += kThreads >> shift) {       // (what is in the other rows reaches no output)
             const int i = li * ctas + c, r = i / pieces, j = i - r * pieces;
             const bool mine = i < m * pieces;
