@@ -101,6 +101,22 @@ def test_rows_are_those_of_quantize_where_the_factor_is_one(cuda):
     assert np.array_equal(rows.packed.cpu().numpy().view(np.uint32), p) and np.array_equal(rows.scales.cpu().numpy(), s)
 
 
+@pytest.mark.parametrize("rows,hidden", [(2048, 8192), (4096, 512)])
+def test_codes_next_to_the_middle_of_two(cuda, rows, hidden):
+    """Where the sum of squares is exact the codes are those of the formula in 64 bits, all of them: fp32's roundings alone put
+    some of 17 million on the other side of the middle between two codes."""
+    g = gen(rows)
+    x = torch.where(torch.rand(rows, hidden, generator=g, device="cuda") < torch.rand(rows, 1, generator=g, device="cuda"), 2.0, -1.0).bfloat16()
+    w = (1 + torch.randn(hidden, generator=g, device="cuda").abs()).bfloat16()
+    _, _, got = ops.add_rms_norm(x, None, w, 0.0, "mxfp8")
+    v = x.double()
+    u = v / torch.sqrt((v * v).mean(-1, keepdim=True)) * w.double()
+    scaled = u / torch.exp2(got.scales.double() - 127).repeat_interleave(32, -1)
+    step = torch.exp2(torch.floor(torch.log2(scaled.abs())) - 3)         # (no value is below the smallest normal number)
+    want = (torch.round(scaled / step) * step).clamp(-448, 448)
+    assert (scaled.abs() > 2.0 ** -6).all() and torch.equal(got.packed.view(torch.float8_e4m3fn).double(), want)
+
+
 def test_norm_in_place_and_leading_dimensions(cuda):
     g = gen(4)
     x, r, w = bf16(g, 2, 37, 1056), bf16(g, 2, 37, 1056), bf16(g, 1056)
