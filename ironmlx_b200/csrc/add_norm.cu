@@ -173,17 +173,15 @@ add_rms_norm_kernel(const __nv_bfloat16* x, const __nv_bfloat16* residual, int n
 
 int launch_add_rms_norm(const void* x, const void* residual, int n, int H, const void* w, float eps, const NormOut& out, cudaStream_t stream) {
     const int pieces = H / 8;
-    // As few threads a row as hold it in eight pieces each while there are rows enough to fill the GPU; one piece a
-    // thread, the shortest way, for a few rows.
+    // As few threads a row as hold it in four pieces each (eight of the longest rows) while there are rows enough to fill the
+    // GPU; two or one piece a thread, the shorter way, for a few rows.
     DeviceInfo di;
     IMX_TRY(current_device(&di));
-    int T = 32;
-    while (T < 512 && T * 4 < pieces) T *= 2;
-    const int most = pieces <= 2 * 1024 ? 1024 : 512;
-    while (T < most && T < pieces && (long)n * T < 1024L * di.sms) T *= 2;
-    const int block = T > 256 ? T : 256;
-    const int grid = ceil_div(n, block / T);
-    const int nv = ceil_div(pieces, T);
+    auto threads = [&](int nv) { return ceil_div(ceil_div(pieces, nv), 32) * 32; };
+    int nv = threads(4) <= max_threads(4) ? 4 : 8;
+    while (nv > 1 && threads(nv / 2) <= max_threads(nv / 2) && (threads(nv / 2) == threads(nv) || (long)n * threads(nv / 2) <= 1024L * di.sms)) nv /= 2;
+    const int T = threads(nv), rows = T < 256 ? 256 / T : 1, block = T * rows;
+    const int grid = ceil_div(n, rows);
     auto kernel = nv <= 1 ? add_rms_norm_kernel<1> : (nv <= 2 ? add_rms_norm_kernel<2> : (nv <= 4 ? add_rms_norm_kernel<4> : add_rms_norm_kernel<8>));
     kernel<<<grid, block, 0, stream>>>((const __nv_bfloat16*)x, (const __nv_bfloat16*)residual, n, H, (const __nv_bfloat16*)w, eps,
                                        out, T, 1. / H); IMX_LAUNCHED();
