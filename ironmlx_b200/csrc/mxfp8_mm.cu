@@ -636,12 +636,13 @@ int launch(const Call& c, int lg_splits) {
 // of tiles, fitted to the kernels alone on a B200 (2048 -> 8192 unless said; measured, in brackets the model):
 //   1 row     S16 8.9 (8.6), S16 cut in 2 7.7 (7.8), N64 9.4 (9.6);   2048 -> 512  S16 cut in 1, 2, 4, 8  8.2, 6.3, 5.4, 5.3
 //   64 rows   S64 11.4 (11.3), S64 cut in 2 10.9 (9.9), N64 9.7 (9.6);   4096 -> 2048  S64 cut in 4 9.6 (9.9), N64 14.0 (14.4)
-//   256 rows  N64 15.4 (14.4), N128 11.1 (10.9), P256 13.0 (11.7);   777 rows 4096 -> 2048  N128 16.4 (17.0), P256 17.9 (17.8)
+//   256 rows  N64 15.0 (14.4), N128 10.9 (10.9), P128 10.6 (10.5), P256 12.5 (11.7)
+//   777 rows 4096 -> 2048  N128 16.5 (17.0), P128 14.5 (14.8), P256 17.9 (17.8)
 //   1024 rows N128 27.6 (23.0), P256 19.8 (18.0);   2048 -> 152064, 64 rows  S64 60.4, N64 91, N128 61, P256 70 (memory: 52)
 // Clusters of eight that fill the GPU find no place together: 4096 -> 2048, 1 row, cut in 8 (128 CTAs) 11.8, in 4 7.3.
 int run(const Call& c) {
     const int steps = ceil_div(c.in, kMxK);
-    enum { S16, S32, S64, N64, N128, P256 } best = P256;
+    enum { S16, S32, S64, N64, N128, P128, P256 } best = P256;
     int best_lg = 0;
     float least = 1e30f;
     auto offer = [&](decltype(best) kernel, int lg, float fixed, long tiles, int at_once, float step) {
@@ -661,6 +662,7 @@ int run(const Call& c) {
     const long rows128 = ceil_div(c.m, 128);
     offer(N64, 0, 4.8f, rows128 * ceil_div(c.n_out, 64), c.sms, 0.30f);
     offer(N128, 0, 4.8f, rows128 * ceil_div(c.n_out, 128), c.sms, 0.38f);
+    offer(P128, 0, 6.2f, (long)ceil_div(c.m, 256) * ceil_div(c.n_out, 128), c.sms / 2, 0.27f);
     offer(P256, 0, 5.5f, (long)ceil_div(c.m, 256) * ceil_div(c.n_out, 256), c.sms / 2, 0.39f);
     switch (best) {
         case S16: return launch<16, true>(c, best_lg);
@@ -668,6 +670,7 @@ int run(const Call& c) {
         case S64: return launch<64, true>(c, best_lg);
         case N64: return launch<64, false>(c, 0);
         case N128: return launch<128, false>(c, 0);
+        case P128: return launch<128, false, true>(c, 0);
         default: return launch<256, false, true>(c, 0);
     }
 }
@@ -715,6 +718,7 @@ int imx_mxfp8_matmul(const void* x_q, const void* x_scales, int m, const imx_qte
         IMX_TRY((set_up<64, true>()));
         IMX_TRY((set_up<64, false>()));
         IMX_TRY((set_up<128, false>()));
+        IMX_TRY((set_up<128, false, true>()));
         IMX_TRY((set_up<256, false, true>()));
         device_mark_setup(di.ordinal, kSetupMxfp8);
     }
