@@ -27,7 +27,8 @@ struct NormOut {
     uint8_t* scales;
 };
 
-// Biased exponent of the scale of 32 values: e + 127, e the smallest integer in [-127, 127] with amax / 448 <= 2^e.
+// Biased exponent of the scale of 32 values: e + 127, e the smallest integer in [-127, 127] with amax / 448 <= 2^e
+// (an infinity among them: 255, which is NaN).
 __device__ __forceinline__ uint32_t scale_code(float amax) {
     const uint32_t b = __float_as_uint(__fdiv_rn(amax, 448.f));
     const uint32_t exp = b >> 23, man = b & 0x7fffffu;
@@ -64,7 +65,7 @@ add_rms_norm_kernel(const __nv_bfloat16* x, const __nv_bfloat16* residual, int n
                     const NormOut out, int T, double per_value) {
     __shared__ double s_part[32];
     const int row_in = threadIdx.x / T, t = threadIdx.x - row_in * T;
-    const int row = blockIdx.x * (blockDim.x / T) + row_in;
+    const long row = (long)blockIdx.x * (blockDim.x / T) + row_in;
     const int pieces = row < n ? H / 8 : 0;
     const size_t base = (size_t)row * H;
     float v[NV][8];

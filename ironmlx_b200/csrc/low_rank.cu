@@ -29,6 +29,7 @@ namespace {
 constexpr int kMaxRank = 256;
 constexpr int kThreads = 256;
 constexpr size_t kStatusBytes = 256;
+constexpr int kMostColumns = 1 << 30;         // of x and y: columns past the end of a row are counted in 31 bits
 std::atomic<int> g_low_rank_spin_limit{kSpin};
 
 struct LowRankArgs {
@@ -494,6 +495,7 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&s.tmem_base)), "r"(kTmem) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    // (No CTA that holds all 512 columns and waits for another SM's is ever beside this one: their shared memories do not fit.)
     auto give_back = [&]() {
         if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(s.tmem_base), "r"(kTmem) : "memory");
     };
@@ -998,6 +1000,7 @@ extern "C" int imx_low_rank_add(const void* y, const void* x, int n_rows, int in
                                 void* out, void* scratch, size_t scratch_bytes, void* stream) {
     IMX_REQUIRE(n_rows >= 0 && n_out > 0 && in > 0 && in % 8 == 0,
                 "low_rank_add: sizes (%d rows, %d -> %d) must be positive, the input dimension a multiple of 8", n_rows, in, n_out);
+    IMX_REQUIRE(in <= kMostColumns && n_out <= kMostColumns, "low_rank_add: dimensions of at most %d", kMostColumns);
     if (n_rows == 0) return IMX_OK;
     IMX_REQUIRE(y && x && ad && ids && out, "low_rank_add: y, x, adapters, ids and out are required");
     IMX_REQUIRE(ad->a && ad->b && ad->count > 0, "low_rank_add: at least one adapter is required");

@@ -236,6 +236,13 @@ def _require_same_device(name, first, *tensors):
             raise IronMLXError(_lib.ERR_INVALID, f"{name}: tensors on {first.device} and {t.device}")
 
 
+def _row_count(name: str, x: torch.Tensor, length: int) -> int:
+    n = x.numel() // length
+    if n > 0x7fffffff:
+        raise IronMLXError(_lib.ERR_INVALID, f"{name}: {n} rows, at most 2^31 - 1")
+    return n
+
+
 def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: Optional[torch.Tensor], eps: float,
                  out: str = "bf16", stream=None):
     """`h = x + residual` and `rms_norm(h)` in one pass, sums in fp32, each output rounded once.
@@ -261,6 +268,7 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: Opti
     if _elsewhere(x, stream):
         with _on(x, stream):
             return add_rms_norm(x, residual, weight, eps, out)
+    n = _row_count("add_rms_norm", x, hidden)
     device = x.device
     h = x if residual is None else torch.empty_like(x)
     y = rows = None
@@ -270,7 +278,7 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: Opti
         lead = tuple(shape)[:-1]
         rows = Mxfp8Rows(torch.empty(*lead, hidden // 4, dtype=torch.int32, device=device),
                          torch.empty(*lead, hidden // 32, dtype=torch.uint8, device=device))
-    check(lib().imx_add_rms_norm(x.data_ptr(), None if residual is None else residual.data_ptr(), x.numel() // hidden, hidden,
+    check(lib().imx_add_rms_norm(x.data_ptr(), None if residual is None else residual.data_ptr(), n, hidden,
                                  None if weight is None else weight.data_ptr(), eps, None if residual is None else h.data_ptr(),
                                  None if y is None else y.data_ptr(), None if rows is None else rows[0].data_ptr(),
                                  None if rows is None else rows[1].data_ptr(), _raw_stream(x.get_device())))
@@ -320,10 +328,11 @@ def mxfp8_matmul(rows, w: torch.Tensor, scales: torch.Tensor, stream=None) -> to
     if _elsewhere(x, stream):
         with _on(x, stream):
             return mxfp8_matmul(rows, w, scales)
+    n = _row_count("mxfp8_matmul", x, words)
     index = x.get_device()
     y = torch.empty(*lead, n_out, dtype=torch.bfloat16, device=x.device)
     qt = QTensor(w.data_ptr(), scales.data_ptr(), None, 1.0)
-    check(lib().imx_mxfp8_matmul(x.data_ptr(), xs.data_ptr(), x.numel() // words, C.byref(qt), n_out, words * 4, y.data_ptr(),
+    check(lib().imx_mxfp8_matmul(x.data_ptr(), xs.data_ptr(), n, C.byref(qt), n_out, words * 4, y.data_ptr(),
                                  _status_block(index).data_ptr(), 256, _raw_stream(index)))
     return y
 
@@ -346,7 +355,7 @@ def low_rank_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
     if len(xshape) == 0 or len(yshape) == 0 or xshape[-1] != in_dim or yshape[-1] != n_out or xshape[:-1] != yshape[:-1]:
         raise IronMLXError(_lib.ERR_INVALID,
                            f"low_rank_add: x {tuple(xshape)} and y {tuple(yshape)} do not match adapters {in_dim} -> {n_out}")
-    rows = x.numel() // in_dim
+    rows = _row_count("low_rank_add", x, in_dim)
     if ids.dtype != torch.int32 or ids.numel() != rows:
         raise IronMLXError(_lib.ERR_INVALID, f"low_rank_add: ids must be int32, one for each of the {rows} rows")
     if scale is not None and (scale.dtype != torch.float32 or scale.numel() != count):

@@ -39,6 +39,7 @@ def product(xq=A, xs=B, m=4, w=D, ws=E, biases=None, n_out=64, n_in=64, y=F, scr
 
 @pytest.mark.parametrize("kw,needle", [
     (dict(m=-1), b"sizes"), (dict(n_out=0), b"sizes"), (dict(n_in=0), b"sizes"), (dict(n_in=48), b"multiple of 32"),
+    (dict(m=0x7fffff80), b"at most"), (dict(n_out=0x7fffffff), b"at most"),
     (dict(xq=None), b"required"), (dict(xs=None), b"required"), (dict(w=None), b"required"), (dict(ws=None), b"required"),
     (dict(y=None), b"required"), (dict(biases=A), b"biases"), (dict(xq=A + 4), b"aligned"), (dict(w=D + 8), b"aligned"),
     (dict(y=F + 1), b"aligned"), (dict(y=A + 128), b"overlaps"), (dict(y=B), b"overlaps"), (dict(y=D - 2), b"overlaps"),
@@ -60,6 +61,7 @@ def low_rank(y=A, x=B, n=4, n_in=64, a=D, b=D + 0x1000000, scale=None, count=3, 
 
 @pytest.mark.parametrize("kw,needle", [
     (dict(n=-1), b"sizes"), (dict(n_in=0), b"sizes"), (dict(n_in=60), b"multiple of 8"), (dict(n_out=0), b"sizes"),
+    (dict(n_in=(1 << 30) + 8), b"at most"), (dict(n_out=(1 << 30) + 1), b"at most"),
     (dict(y=None), b"required"), (dict(x=None), b"required"), (dict(ids=None), b"required"), (dict(out=None), b"required"),
     (dict(a=None), b"adapter"), (dict(b=None), b"adapter"), (dict(count=0), b"adapter"),
     (dict(rank=0), b"rank"), (dict(rank=12), b"rank"), (dict(rank=264), b"rank"),
@@ -93,6 +95,13 @@ def test_scratch_sizes():
     assert lib.imx_low_rank_scratch_bytes(5, 64, 64, 2, 8, C.byref(nb)) == 0 and nb.value >= 256
     refused(lib.imx_low_rank_scratch_bytes(5, 64, 64, 0, 8, C.byref(nb)), b"bad arguments")
     refused(lib.imx_low_rank_scratch_bytes(5, 64, 64, 1, 512, C.byref(nb)), b"bad arguments")
+
+
+def test_more_rows_than_an_int_counts():
+    x = torch.empty(1, 8, device="meta")
+    assert ops._row_count("op", x.expand(0x7fffffff, 8), 8) == 0x7fffffff
+    with pytest.raises(_lib.IronMLXError, match="rows"):
+        ops._row_count("op", x.expand(1 << 31, 8), 8)
 
 
 def test_python_layer_refuses_host_tensors_and_other_formats():
