@@ -9,14 +9,15 @@
 // Which rows make up a unit every CTA finds out by itself from the ids: the units of an adapter are its rows in batch order,
 // so that the result does not depend on who runs when.  Rows without an adapter are units of their own that are copied.
 //
-// Two kernels:
+// Two kernels (times on a B200, of the kernels alone):
 //   few rows (at most 128): a and b are read once and go straight into the fragments of mma.sync, whose k order is permuted so
-//     that a lane's 16 bytes are four k pairs.  Bound by latency: one row of rank 16, 2048 -> 2048, takes 5.5 us; 48 rows of 12
-//     adapters of rank 64, 4096 -> 4096 (12.6 MB: 1.9 us at the copy bandwidth), 11.8 us.
-//   many rows: tiles of 64 rows by tcgen05.mma, x and y gathered by cp.async, a and b brought by TMA.  Bound by how fast the
-//     warps move a stage through shared memory (1000 cycles for 64 rows x 64 columns of y, two CTAs to an SM): 8192 rows of
-//     rank 64, 4096 -> 4096, take 82 us, 201 MB at 2.4 TB/s; the same with mma.sync by the warps that copy took 113 us, and at
-//     rank 128 229 us, here 114.
+//     that a lane's 16 bytes are four k pairs.  Bound by latency, of memory (each lane brings what it alone reads, through a
+//     ring of cp.async) and of the cluster's two meetings: one row of rank 16, 2048 -> 8192, takes 5.2 us; 48 rows of 40
+//     adapters of rank 32, 4096 -> 2048 (16 MB: 2.5 us at the copy bandwidth), 11.2 us.
+//   many rows: tiles of 64 rows by tcgen05.mma, x and y gathered by cp.async, a and b brought by TMA.  8192 rows of rank 64,
+//     2048 -> 8192, take 76 us, 318 MB at 4.2 TB/s: y comes and leaves at 6.2 TB/s, close to the copy bandwidth, but the ids
+//     (5 us), x . a^T (7 us) and the cluster's exchange (5 us) come before it, for all CTAs at the same time.  With mma.sync by
+//     the warps that copy it was 113 us; rank 128 takes 109 us (229).  777 rows of rank 16 take 17 us, each phase a latency or two.
 #include <atomic>
 
 #include "tcgen05.cuh"
@@ -936,6 +937,9 @@ int launch_clusters(const void* kernel, unsigned grid, int threads, int ctas, si
     return IMX_OK;
 }
 
+// 128 rows, 2048 -> 4096, by the two kernels, in us: 16 adapters of rank 16, 64, 128  9.4, 14.5, 26.8 and (tiles) 18.3, 19.3, 30.0;
+// 120 adapters  17.4, 28.0, 68.0 and 38.5, 42.7, 67.2; 2 adapters  8.7, 11.7, 20.3 and 11.0, 13.1, 17.0.  So up to 128 rows are
+// few; so are, 128 at a time, more of them where the tile kernel cannot count the adapters or name b's rows in 31 bits.
 int launch_low_rank(LowRankArgs p, int sms, cudaStream_t stream) {
     const int rows = p.n, step = rows <= kFewRows || p.count >= kMaxBins || (long)p.count * p.n_out > 0x7fffffffL ? kFewRows : kBlockRows;
     const LowRankArgs whole = p;
@@ -956,6 +960,10 @@ int launch_low_rank(LowRankArgs p, int sms, cudaStream_t stream) {
         int ctas = 1;
         void* args[] = {&p, &ctas, nullptr, nullptr};
         if (step == kFewRows) {
+            // Units: no more than every 16th row leads because 16 have gone before, and one of every id.  A cluster up to
+            // CTAs for three on every SM (two, where the rings leave room for no more): 48 rows of 40 adapters with two 12.4
+            // us, with one 14.0, with three 11.7.  More clusters of a unit repeat x . a^T and pay while SMs are idle: one row,
+            // 2048 -> 8192, 5.5 us, in one cluster 8.1.
             const FewKernel few = few_kernel(p.rank);
             const int ids = p.count < p.n ? p.count + 1 : p.n, bound = p.n / kFewUnit + ids, units = bound < p.n ? bound : p.n;
             while (ctas < 8 && units * ctas * 2 <= (few.rb <= 2 ? 3 : 2) * sms) ctas *= 2;
@@ -965,7 +973,9 @@ int launch_low_rank(LowRankArgs p, int sms, cudaStream_t stream) {
             IMX_TRY(launch_clusters(few.kernel, (unsigned)(units * ctas * clusters), kThreads, ctas, (size_t)FewPlan(p.rank, few.rb).bytes, stream, args));
             continue;
         }
-        // no more units than these; CTAs for two on every SM: clusters of up to eight for a unit, then several of them
+        // No more units than these; CTAs for two on every SM (for one 8192 rows of rank 64 take 103 us, for four 98, not 82):
+        // clusters of up to eight for a unit (777 rows of rank 16: clusters of 8, 4, 2, 1 take 20.4, 21.2, 23.8, 24.4 us),
+        // then several of them (200 rows, 2048 -> 8192, with one 18.4 us, with more 16.2).
         const int units = p.n / kTileRows + (p.count + 1 < p.n ? p.count + 1 : p.n);
         while (ctas < 8 && units * ctas * 2 <= 2 * sms) ctas *= 2;
         int clusters = 1;

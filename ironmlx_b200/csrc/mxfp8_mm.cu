@@ -6,9 +6,12 @@
 // Both operands have the same form, so that one kernel serves both orientations: P (128 rows, the lanes of the accumulator) and
 // Q (NT rows, its columns), both K-major with 128-byte swizzle, 128 codes a stage.
 //   few rows of x   P = weight, Q = the rows (SWAP): the weight's bytes bound it, its tiles are spread over the SMs
-//   many rows       P = the rows, Q = weight: the tensor cores bound it
-// Few tiles for the GPU: the K range of a tile is cut over the CTAs of a cluster; each leaves its fp32 sums in shared memory
-// and adds one part of the tile over all of them, in rank order.
+//   many rows       P = the rows, Q = weight: the tensor cores bound it.  With 128 columns or more by pairs of CTAs
+//                   (cta_group::2), each of which brings half of Q: an SM takes in 85 to 95 GB/s of tiles, whatever their
+//                   shape, and that bounds all products that are not large.
+// Few tiles for the GPU: the K range of a tile is cut over the CTAs of a cluster; each leaves its fp32 sums in shared memory,
+// sends every other CTA its columns in one bulk copy (7.7 us for a row, 2048 -> 8192; read by the receiver 8.7, sent word by
+// word 9.5) and adds its own over all of them, in rank order.
 //
 // Scales lie in memory as the format has them, [rows, in / 32] bytes.  The MMA reads them from tensor memory, four K steps in
 // a word, row r in lane r mod 32 of column r / 32: four warps fetch them as 16-byte pieces a row (four stages at a time, one
@@ -16,10 +19,15 @@
 // follow it.  A stage's slot in tensor memory is written again no sooner than its shared memory, whose release waits for the
 // MMAs that read both.  Rows and blocks past the end get the scale 1 and, from TMA, codes of zero.
 //
-// Ten warps: 0..3 epilogue, 4..7 scales, 8 MMA and tensor memory, 9 loads.  Two accumulators alternate, so that the next
+// Eleven warps: 0..3 epilogue, 4..7 scales, 8 MMA and tensor memory, 9 loads, 10 (of a pair) tells CTA 0, whose warp 8 issues
+// the MMAs of both, what has arrived in its own.  Two accumulators alternate, so that the next
 // tile's MMAs run beside the epilogue; 2 x 256 columns leave no room for the scales: at NT = 256 the two share 48 columns,
 // which the epilogue takes out first.  Every wait is bounded; on expiry what is in flight is waited for, tensor memory is
 // freed, the status word is set and the tiles concerned are NaN.
+//
+// On a B200, the kernel alone: 8192 rows, 2048 -> 8192, 105 us, 2.6 PFLOP/s, 79% of twice cuBLAS' bf16 rate (the tensor cores
+// busy 73% of the time, the card at its power limit); 777 rows, 4096 -> 2048, 14.6 us; 64 rows, 2048 -> 152064, 61 us, 5.6 TB/s;
+// one row, 2048 -> 8192, 7.8 us, of which 4.6 are a launch's, the ring's filling and the cluster's.
 #include <atomic>
 
 #include "tcgen05.cuh"
