@@ -14,6 +14,9 @@
 //                               forward_with_stream)
 //   ops::quantized_matmul, ops::dequantize   mlx/src/ops.rs:653-727
 //
+// Without a counterpart there: RMSNorm::forward_residual and QuantizedLinear::forward_rows / ops::mxfp8_matmul (rows in
+// 8 bits between a norm and a projection), LowRankAdapters (the adapters of many requests beside a projection).
+//
 // Differences a port has to know: outputs are written into caller-provided
 // arrays (no allocator here), the routed experts are held as the two fused
 // checkpoint tensors (mlx/src/model/qwen35.rs:581-590) instead of a Vec of

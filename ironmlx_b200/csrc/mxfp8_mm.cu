@@ -25,8 +25,8 @@
 // which the epilogue takes out first.  Every wait is bounded; on expiry what is in flight is waited for, tensor memory is
 // freed, the status word is set and the tiles concerned are NaN.
 //
-// On a B200, the kernel alone: 8192 rows, 2048 -> 8192, 105 us, 2.6 PFLOP/s, 79% of twice cuBLAS' bf16 rate (the tensor cores
-// busy 73% of the time, the card at its power limit); 777 rows, 4096 -> 2048, 14.6 us; 64 rows, 2048 -> 152064, 61 us, 5.6 TB/s;
+// On a B200, the kernel alone: 8192 rows, 2048 -> 8192, 105 us, 2.6 PFLOP/s, 79% of twice cuBLAS' bf16 rate (the tensor
+// cores busy 73% of the time; in a loop of seconds the power limit makes it 122 us); 777 rows, 4096 -> 2048, 14.6 us; 64 rows, 2048 -> 152064, 61 us, 5.6 TB/s;
 // one row, 2048 -> 8192, 7.8 us, of which 4.6 are a launch's, the ring's filling and the cluster's.
 #include <atomic>
 
