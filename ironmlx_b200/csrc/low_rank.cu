@@ -99,6 +99,14 @@ __device__ __forceinline__ uint4 ld_shared16(uint32_t addr) {
     return v;
 }
 
+// Four 8 x 8 matrices of 16-bit values; lane l gives the address of row l % 8 of matrix l / 8.
+__device__ __forceinline__ void ld_matrices(uint32_t addr, uint32_t (&v)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void st_matrices(uint32_t addr, const uint32_t (&v)[4]) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+}
+
 // ── few rows ────────────────────────────────────────────────────────────────
 constexpr int kFewRows = 128;                 // rows of a launch
 constexpr int kFewUnit = 16;
@@ -845,7 +853,8 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
         if (NJ > 4)
             for (int i = 0; i < S - 1; ++i) copy(total);
         int n = n0 * kCols;                                // first column of the stage
-        unsigned char* y = smem + (n_in % S) * pl.stage;   // ... and its place
+        uint32_t y = base + (uint32_t)((n_in % S) * pl.stage);                   // ... and its place
+        const uint32_t frag_at = (uint32_t)((rt * 16 + (lane & 7)) * 128 + (((half * 4 + (lane >> 3)) ^ (lane & 7)) * 16));
         for (int e = 0; e < total - n_in; ++e) {
             wait(s.sums_there[e & 1], e >> 1);
             tc::tc_fence_after();
@@ -856,21 +865,26 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s.sums_free[e & 1]));
             if (p.wide) {
-                // added in y's place, out in 16-byte pieces
+                // added in y's place, which is read and written as 8 x 8 matrices (the sums' layout), out in 16-byte pieces
+                uint32_t v[2][4];
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int h = 0; h < 2; ++h) ld_matrices(y + frag_at + h * 1024, v[h]);
+                __syncwarp();
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int r = rt * 16 + g + 8 * h;
-                        __nv_bfloat162* at = reinterpret_cast<__nv_bfloat162*>(y + r * 128 + (((half * 4 + j) ^ (r & 7)) * 16) + q * 4);
-                        const float2 v = __bfloat1622float2(*at);
-                        *at = __floats2bfloat162_rn(v.x + d[4 * j + 2 * h], v.y + d[4 * j + 2 * h + 1]);
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v[h][j]));
+                        const __nv_bfloat162 o = __floats2bfloat162_rn(f.x + d[4 * j + 2 * h], f.y + d[4 * j + 2 * h + 1]);
+                        v[h][j] = *reinterpret_cast<const uint32_t*>(&o);
                     }
+                    st_matrices(y + frag_at + h * 1024, v[h]);
+                }
                 __syncwarp();
                 const bool in = n + half * 32 + q * 8 < p.n_out;
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    if (has_own[h] && in) *reinterpret_cast<uint4*>(to_own[h]) = *reinterpret_cast<const uint4*>(y + y_at[h]);
+                const uint4 o0 = ld_shared16(y + y_at[0]), o1 = ld_shared16(y + y_at[1]);
+                if (has_own[0] && in) *reinterpret_cast<uint4*>(to_own[0]) = o0;
+                if (has_own[1] && in) *reinterpret_cast<uint4*>(to_own[1]) = o1;
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
@@ -887,7 +901,7 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
             to_own[0] += kCols;
             to_own[1] += kCols;
             y += pl.stage;
-            if (y == smem + S * pl.stage) y = smem;
+            if (y == base + (uint32_t)(S * pl.stage)) y = base;
             copy(total);                                   // into the place of the stage before this one, of y if not of x: see above
         }
         copies_wait<0>();
