@@ -425,6 +425,7 @@ constexpr int kBlock = kTileRows * 128;       // bytes of 64 rows of 64 values i
 
 constexpr int kTileThreads = kThreads + 64;    // eight warps that copy and write out, one that issues the MMAs, one that loads a and b
 constexpr int kMaxStages = 5;
+constexpr size_t kPrefetch = (size_t)64 << 20;     // bytes of x that L2 takes in and keeps until they are read
 
 struct TileShared {
     int32_t rows[kTileRows];
@@ -472,15 +473,17 @@ __device__ __forceinline__ void tmem_ld_16x16(uint32_t taddr, float (&v)[8]) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(u[i]);
 }
-__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, float (&v)[16]) {
-    uint32_t u[16];
+// (On its way until tmem_wait.)
+__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t (&u)[16]) {
     asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
                  : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]),
                    "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
                  : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(u[i]);
+}
+__device__ __forceinline__ void tmem_wait(uint32_t (&u)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(u[0]), "+r"(u[1]), "+r"(u[2]), "+r"(u[3]), "+r"(u[4]), "+r"(u[5]), "+r"(u[6]), "+r"(u[7]), "+r"(u[8]), "+r"(u[9]),
+                   "+r"(u[10]), "+r"(u[11]), "+r"(u[12]), "+r"(u[13]), "+r"(u[14]), "+r"(u[15])::"memory");
 }
 
 // Eight warps gather x, and y, by cp.async; a ninth issues the MMAs, a tenth brings a and b by TMA.  In the second product a warp
@@ -533,6 +536,14 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
     lots([&](int i) {
         if (i < groups && from + i * 32 + lane < p.n && (bin[i] < 0 || bin[i] >= p.count)) bin[i] = p.count;
     });
+    // While the others count, memory would be idle: x on its way into L2, a part of the rows by each CTA.
+    if (warp == 9 && (size_t)p.n * p.in * 2 <= kPrefetch)
+        for (long r = (long)p.n * blockIdx.x / gridDim.x + lane; r < (long)p.n * (blockIdx.x + 1) / gridDim.x; r += 32) {
+            const int j = p.ids[r];
+            if (j >= 0 && j < p.count)
+                asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(p.x + (size_t)r * p.in), "r"(p.in * 2) : "memory");
+        }
+    __syncwarp();
     for (int i = tid; i < n_bins; i += kTileThreads) bins[i] = 0;
     if (tid == 0) {
         s.n_rows = 0;
@@ -858,18 +869,23 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
         for (int e = 0; e < total - n_in; ++e) {
             wait(s.sums_there[e & 1], e >> 1);
             tc::tc_fence_after();
-            float d[16];
-            tmem_ld_16x32(tmem + ((uint32_t)(rt * 32) << 16) + (uint32_t)((e & 1) * 64 + half * 32), d);
-            tc::tc_fence_before();
+            uint32_t u[16], v[2][4];
+            tmem_ld_16x32(tmem + ((uint32_t)(rt * 32) << 16) + (uint32_t)((e & 1) * 64 + half * 32), u);
             arrived();
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s.sums_free[e & 1]));
             if (p.wide) {
-                // added in y's place, which is read and written as 8 x 8 matrices (the sums' layout), out in 16-byte pieces
-                uint32_t v[2][4];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) ld_matrices(y + frag_at + h * 1024, v[h]);
-                __syncwarp();
+            }
+            tmem_wait(u);
+            tc::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s.sums_free[e & 1]));
+            float d[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) d[i] = __uint_as_float(u[i]);
+            if (p.wide) {
+                // added in y's place, which is read and written as 8 x 8 matrices (the sums' layout), out in 16-byte pieces
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
 #pragma unroll
