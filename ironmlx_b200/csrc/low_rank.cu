@@ -15,9 +15,9 @@
 //     ring of cp.async) and of the cluster's two meetings: one row of rank 16, 2048 -> 8192, takes 5.2 us; 48 rows of 40
 //     adapters of rank 32, 4096 -> 2048 (16 MB: 2.5 us at the copy bandwidth), 11.2 us.
 //   many rows: tiles of 64 rows by tcgen05.mma, x and y gathered by cp.async, a and b brought by TMA.  8192 rows of rank 64,
-//     2048 -> 8192, take 76 us, 318 MB at 4.2 TB/s: y comes and leaves at 6.2 TB/s, close to the copy bandwidth, but the ids
+//     2048 -> 8192, take 71 us, 318 MB at 4.5 TB/s: y comes and leaves at 6.2 TB/s, close to the copy bandwidth, but the ids
 //     (5 us), x . a^T (7 us) and the cluster's exchange (5 us) come before it, for all CTAs at the same time.  With mma.sync by
-//     the warps that copy it was 113 us; rank 128 takes 109 us (229).  777 rows of rank 16 take 17 us, each phase a latency or two.
+//     the warps that copy it was 113 us; rank 128 takes 110 us (229).  777 rows of rank 16 take 17 us, each phase a latency or two.
 #include <atomic>
 
 #include "tcgen05.cuh"
@@ -118,7 +118,7 @@ __host__ __device__ constexpr int ring_pieces(int rb) { return rb == 8 ? 18 : (r
 struct FewPlan {
     int pitch, sums_at, part_at, lo_at, bytes;       // pitch: values of a row of hi or lo
     __host__ __device__ FewPlan(int rank, int rb) {
-        pitch = rb * 32 + 8;
+        pitch = rb * 32 + 32;                        // (lanes that read together are in different banks)
         sums_at = kThreads * ring_pieces(rb) * 16;
         part_at = sums_at + kFewUnit * rank * 4;
         lo_at = part_at + kFewUnit * pitch * 2;
@@ -201,6 +201,7 @@ low_rank_few_kernel(const LowRankArgs p, const int ctas, const int clusters) {
             }
         return;
     }
+    const float sc = p.scale != nullptr ? p.scale[id] : 1.f;
     // a lane multiplies the rows g and g + 8 of the unit
     const int row0 = s.rows[min(g, m - 1)], row1 = s.rows[min(g + 8, m - 1)];
     const bool has0 = g < m, has1 = g + 8 < m, more = m > 8;
@@ -321,7 +322,6 @@ low_rank_few_kernel(const LowRankArgs p, const int ctas, const int clusters) {
     }
     if (ctas > 1) cluster_sync();
     else __syncthreads();
-    const float sc = p.scale != nullptr ? p.scale[id] : 1.f;
     for (int i = tid; i < kFewUnit * RB * 32; i += kThreads) {
         const int r = i / (RB * 32), k = i % (RB * 32);
         float v = 0.f;
@@ -348,7 +348,8 @@ low_rank_few_kernel(const LowRankArgs p, const int ctas, const int clusters) {
     const uint4* h1 = reinterpret_cast<const uint4*>(hi + (g + 8) * pl.pitch + q * 8);
     const uint4* l0 = reinterpret_cast<const uint4*>(lo + g * pl.pitch + q * 8);
     const uint4* l1 = reinterpret_cast<const uint4*>(lo + (g + 8) * pl.pitch + q * 8);
-    constexpr int kKept = RB <= 2 ? RB : 1;   // up to a rank of 64 the low-rank rows stay in registers
+    // up to a rank of 128 the low-rank rows stay in registers (read for every tile they cost a rank of 128 half of its time)
+    constexpr int kKept = RB <= 4 ? RB : 1;
     uint4 vh0[kKept], vh1[kKept], vl0[kKept], vl1[kKept];
 #pragma unroll
     for (int kb = 0; kb < kKept; ++kb) {
@@ -376,12 +377,14 @@ low_rank_few_kernel(const LowRankArgs p, const int ctas, const int clusters) {
 #pragma unroll
         for (int kb = 0; kb < RB; ++kb) {
             const uint4 w = ld_shared16(from + (1 + kb) * kPiece);
-            const int i0 = RB <= 2 ? kb : 0;
-            if (RB > 2) {
+            const int i0 = kKept == RB ? kb : 0;
+            if (kKept != RB) {
                 vh0[0] = h0[kb * 4];
-                vh1[0] = h1[kb * 4];
                 vl0[0] = l0[kb * 4];
-                vl1[0] = l1[kb * 4];
+                if (more) {
+                    vh1[0] = h1[kb * 4];
+                    vl1[0] = l1[kb * 4];
+                }
             }
             mma(d, vh0[i0].x, vh1[i0].x, vh0[i0].y, vh1[i0].y, w.x, w.y);
             mma(e, vl0[i0].x, vl1[i0].x, vl0[i0].y, vl1[i0].y, w.x, w.y);
@@ -967,8 +970,8 @@ int launch_clusters(const void* kernel, unsigned grid, int threads, int ctas, si
     return IMX_OK;
 }
 
-// 128 rows, 2048 -> 4096, by the two kernels, in us: 16 adapters of rank 16, 64, 128  9.4, 14.5, 26.8 and (tiles) 18.3, 19.3, 30.0;
-// 120 adapters  17.4, 28.0, 68.0 and 38.5, 42.7, 67.2; 2 adapters  8.7, 11.7, 20.3 and 11.0, 13.1, 17.0.  So up to 128 rows are
+// 128 rows, 2048 -> 4096, by the two kernels, in us: 16 adapters of rank 16, 64, 128  9.0, 13.9, 19.9 and (tiles) 18.3, 19.3, 30.0;
+// 120 adapters  16.8, 27.1, 46.0 and 38.5, 42.7, 67.2; 2 adapters  8.2, 11.2, 16.0 and 11.0, 13.1, 17.0.  So up to 128 rows are
 // few; so are, 128 at a time, more of them where the tile kernel cannot count the adapters or name b's rows in 31 bits.
 int launch_low_rank(LowRankArgs p, int sms, cudaStream_t stream) {
     const int rows = p.n, step = rows <= kFewRows || p.count >= kMaxBins || (long)p.count * p.n_out > 0x7fffffffL ? kFewRows : kBlockRows;
