@@ -211,16 +211,20 @@ class Mxfp8Rows(NamedTuple):
 def _on(x: torch.Tensor, stream):
     """The device of x, and the given stream, made current: what is allocated within belongs to that stream, and the
     launches go to that device."""
-    return torch.cuda.device(x.device) if stream is None else torch.cuda.stream(stream)
+    if stream is None:
+        return torch.cuda.device(x.device)
+    if stream.device_index != x.get_device():
+        raise IronMLXError(_lib.ERR_INVALID, f"a stream of device {stream.device_index} cannot take work on {x.device}")
+    return torch.cuda.stream(stream)
 
 
 def _elsewhere(x: torch.Tensor, stream) -> bool:
     """Whether a call on x has to switch stream or device first (`_on`)."""
-    return stream is not None or x.get_device() != torch.cuda.current_device()
+    return stream is not None or x.get_device() != _current_device()
 
 
-# The current stream's handle: a call of a few microseconds would spend three on the Stream object.
-_raw_stream = torch._C._cuda_getCurrentRawStream
+# The current device, and its current stream's handle: a call of a few microseconds would spend three on the Stream object.
+_current_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
 
 
 def _require_same_device(name, first, *tensors):
@@ -228,11 +232,9 @@ def _require_same_device(name, first, *tensors):
         raise IronMLXError(_lib.ERR_INVALID, f"{name}: tensors must be contiguous CUDA tensors")
     device = first.get_device()
     for t in tensors:
-        if t is None:
-            continue
-        if not t.is_cuda or not t.is_contiguous():
-            raise IronMLXError(_lib.ERR_INVALID, f"{name}: tensors must be contiguous CUDA tensors")
-        if t.get_device() != device:
+        if t is not None and (t.get_device() != device or not t.is_contiguous()):
+            if not t.is_cuda or not t.is_contiguous():
+                raise IronMLXError(_lib.ERR_INVALID, f"{name}: tensors must be contiguous CUDA tensors")
             raise IronMLXError(_lib.ERR_INVALID, f"{name}: tensors on {first.device} and {t.device}")
 
 
@@ -253,8 +255,8 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: Opti
     if out not in ("bf16", "mxfp8", "both"):
         raise IronMLXError(_lib.ERR_INVALID, f"add_rms_norm: out must be bf16, mxfp8 or both, not {out!r}")
     shape = x.shape
-    if (x.dtype != torch.bfloat16 or (residual is not None and residual.dtype != torch.bfloat16)
-            or (weight is not None and weight.dtype != torch.bfloat16)):
+    bf16 = torch.bfloat16
+    if x.dtype != bf16 or (residual is not None and residual.dtype != bf16) or (weight is not None and weight.dtype != bf16):
         raise IronMLXError(_lib.ERR_INVALID, "add_rms_norm: x, residual and weight must be bfloat16")
     if len(shape) == 0 or shape[-1] == 0:
         raise IronMLXError(_lib.ERR_INVALID, "add_rms_norm: x has no last dimension")
@@ -269,19 +271,22 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: Opti
         with _on(x, stream):
             return add_rms_norm(x, residual, weight, eps, out)
     n = _row_count("add_rms_norm", x, hidden)
-    device = x.device
-    h = x if residual is None else torch.empty_like(x)
-    y = rows = None
+    h, y, rows = x, None, None
+    residual_at = h_at = y_at = q_at = scales_at = None
+    if residual is not None:
+        h = torch.empty_like(x)
+        residual_at, h_at = residual.data_ptr(), h.data_ptr()
     if out != "mxfp8":
         y = torch.empty_like(x)
+        y_at = y.data_ptr()
     if out != "bf16":
-        lead = tuple(shape)[:-1]
-        rows = Mxfp8Rows(torch.empty(*lead, hidden // 4, dtype=torch.int32, device=device),
-                         torch.empty(*lead, hidden // 32, dtype=torch.uint8, device=device))
-    check(lib().imx_add_rms_norm(x.data_ptr(), None if residual is None else residual.data_ptr(), n, hidden,
-                                 None if weight is None else weight.data_ptr(), eps, None if residual is None else h.data_ptr(),
-                                 None if y is None else y.data_ptr(), None if rows is None else rows[0].data_ptr(),
-                                 None if rows is None else rows[1].data_ptr(), _raw_stream(x.get_device())))
+        lead, device = shape[:-1], x.device
+        q = torch.empty(*lead, hidden // 4, dtype=torch.int32, device=device)
+        scales = torch.empty(*lead, hidden // 32, dtype=torch.uint8, device=device)
+        rows = Mxfp8Rows(q, scales)
+        q_at, scales_at = q.data_ptr(), scales.data_ptr()
+    check(lib().imx_add_rms_norm(x.data_ptr(), residual_at, n, hidden, None if weight is None else weight.data_ptr(), eps, h_at, y_at,
+                                 q_at, scales_at, _raw_stream(x.get_device())))
     return h, y, rows
 
 

@@ -104,6 +104,20 @@ def test_more_rows_than_an_int_counts():
         ops._row_count("op", x.expand(1 << 31, 8), 8)
 
 
+def test_streams_of_another_device():
+    class Stream:
+        device_index = 1
+
+    class Tensor:
+        device = "cuda:0"
+
+        def get_device(self):
+            return 0
+
+    with pytest.raises(_lib.IronMLXError, match="stream"):
+        ops._on(Tensor(), Stream())
+
+
 def test_python_layer_refuses_host_tensors_and_other_formats():
     x = torch.zeros(2, 64, dtype=torch.bfloat16)
     ids = torch.zeros(2, dtype=torch.int32)
