@@ -500,7 +500,7 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
     __shared__ TileShared s;
     unsigned char* smem = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     const TilePlan pl(p.rank, NJ);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int shift = 31 - __clz(ctas), cut = shift + 31 - __clz(clusters);       // (both are powers of two)
     const int unit = (int)blockIdx.x >> cut, c = (int)blockIdx.x & (ctas - 1);
     // First of all the tensor memory: an SM starts its second CTA only when the first has given up the permit to allocate (with
@@ -632,7 +632,7 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
     tc::tc_fence_before();
     __syncthreads();
     tc::tc_fence_after();
-    const uint32_t tmem = s.tmem_base;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, s.tmem_base, 0);
     // chunks of the input and of the output dimension that this CTA takes
     const int ik = (p.in + kCols - 1) / kCols, on = (p.n_out + kCols - 1) / kCols;
     const int part_of = (int)blockIdx.x & ((1 << cut) - 1);
@@ -694,7 +694,7 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
         else __syncthreads();
         fill(total);
     } else if (warp == 8) {
-        const uint32_t flag = tc::smem_u32(&s.abort);
+        const uint32_t flag = tc::smem_u32(&s.abort), me = tc::elect_one() ? 1u : 0u;
         int slot = 0;
         uint32_t ph = 0;
         auto next_stage = [&]() {
@@ -708,12 +708,10 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
             tc::mbar_wait_on(tc::smem_u32(&s.loaded[slot]), ph, flag, p.spin_limit);
             tc::tc_fence_after();
             const uint32_t st = base + (uint32_t)(slot * pl.stage), idesc = tc::idesc_for(64, r16) | (1u << 7) | (1u << 10);      // bf16
-            if (tc::elect_one()) {
 #pragma unroll
-                for (int kk = 0; kk < kCols / 16; ++kk)
-                    tc::umma_ss(tmem, tc::smem_desc(st) + 2 * kk, tc::smem_desc(st + kBlock) + 2 * kk, idesc, i > 0 || kk > 0 ? 1u : 0u);
-                tc::umma_commit(tc::smem_u32(&s.used[slot]));
-            }
+            for (int kk = 0; kk < kCols / 16; ++kk)
+                tc::umma_ss_if(me, tmem, tc::smem_desc(st) + 2 * kk, tc::smem_desc(st + kBlock) + 2 * kk, idesc, i > 0 || kk > 0 ? 1u : 0u);
+            tc::umma_commit_if<false>(me, tc::smem_u32(&s.used[slot]));
             __syncwarp();
             next_stage();
         }
@@ -731,18 +729,16 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
             tc::tc_fence_after();
             const uint32_t d = tmem + (uint32_t)((e & 1) * 64);
             const uint64_t b_desc = tc::smem_desc(base + (uint32_t)(slot * pl.stage + kBlock));
-            if (tc::elect_one()) {
 #pragma unroll
-                for (int part = 0; part < 2; ++part)
+            for (int part = 0; part < 2; ++part)
 #pragma unroll
-                    for (int kk = 0; kk < 2 * NJ; ++kk)
-                        if (kk < kks) {
-                            const uint64_t at = (uint64_t)((kk >> 2) * (kBlock >> 4) + 2 * (kk & 3));
-                            tc::umma_ss(d, (part ? lo_desc : hi_desc) + at, b_desc + at, idesc, part > 0 || kk > 0 ? 1u : 0u);
-                        }
-                tc::umma_commit(tc::smem_u32(&s.used[slot]));
-                tc::umma_commit(tc::smem_u32(&s.sums_there[e & 1]));
-            }
+                for (int kk = 0; kk < 2 * NJ; ++kk)
+                    if (kk < kks) {
+                        const uint64_t at = (uint64_t)((kk >> 2) * (kBlock >> 4) + 2 * (kk & 3));
+                        tc::umma_ss_if(me, d, (part ? lo_desc : hi_desc) + at, b_desc + at, idesc, part > 0 || kk > 0 ? 1u : 0u);
+                    }
+            tc::umma_commit_if<false>(me, tc::smem_u32(&s.used[slot]));
+            tc::umma_commit_if<false>(me, tc::smem_u32(&s.sums_there[e & 1]));
             __syncwarp();
             next_stage();
         }

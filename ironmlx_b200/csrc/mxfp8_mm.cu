@@ -88,6 +88,7 @@ struct MxArgs {
     __nv_bfloat16* y;
     int n_out;
     int tiles, tiles_q;
+    int height;                         // rows of P in a tile (SWAP: 128 or fewer)
     int stage_bytes;                    // that the loads of a stage bring
     int y_map;                          // y leaves by TMA (rows that start on 16 bytes)
     int piece_p, piece_q;               // bytes of scales that one load may fetch: 16, 4 or 1
@@ -103,28 +104,32 @@ __device__ __forceinline__ uint32_t mx_idesc(int m, int n, int kk) {
     return (1u << 23) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 7) << 27) | ((uint32_t)kk << 4) | ((uint32_t)kk << 29);
 }
 template <bool PAIR>
-__device__ __forceinline__ void umma_mx(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t accumulate) {
+__device__ __forceinline__ void umma_mx(uint32_t me, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb, uint32_t accumulate) {
     if (PAIR)
         asm volatile(
-            "{\n\t.reg .pred p;\n\t"
+            "{\n\t.reg .pred p, q;\n\t"
             "setp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+            "setp.ne.b32 q, %7, 0;\n\t"
+            "@q tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate), "r"(me)
             : "memory");
     else
         asm volatile(
-            "{\n\t.reg .pred p;\n\t"
+            "{\n\t.reg .pred p, q;\n\t"
             "setp.ne.b32 p, %6, 0;\n\t"
-            "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
-            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate)
+            "setp.ne.b32 q, %7, 0;\n\t"
+            "@q tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accumulate), "r"(me)
             : "memory");
 }
 // 32 x 16 bytes of shared memory -> four columns of all four 32-lane parts (of both CTAs of a pair, each from its own)
 template <bool PAIR>
-__device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint32_t smem) {
+__device__ __forceinline__ void tmem_copy_scales(uint32_t me, uint32_t taddr, uint32_t smem) {
     const uint64_t desc = (uint64_t)((smem >> 4) & 0x3fffu) | (8ull << 16) | (8ull << 32) | (1ull << 46);     // no swizzle, 8 rows of 16 bytes together
-    if (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
-    else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+    if (PAIR)
+        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(taddr), "l"(desc), "r"(me) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t@q tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n\t}" ::"r"(taddr), "l"(desc), "r"(me) : "memory");
 }
 __device__ __forceinline__ void st_shared(uint32_t addr, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
 __device__ __forceinline__ void st_shared4(uint32_t addr, uint4 v) {
@@ -198,7 +203,7 @@ mxfp8_mm_kernel(const MxArgs a, const int lg_splits, const __grid_constant__ MxM
     unsigned char* base = reinterpret_cast<unsigned char*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     // 1024-byte aligned: the stages, then the epilogue's, then the scales
     const uint32_t sbase = smem_u32(base), out_base = sbase + P::kStages * P::kTile, sf_base = out_base + P::kOut;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     volatile int* abort_flag = &bars.abort;
     const int spin = a.spin_limit;
 
@@ -240,7 +245,7 @@ mxfp8_mm_kernel(const MxArgs a, const int lg_splits, const __grid_constant__ MxM
     if (PAIR || (SWAP && lg_splits > 0)) cluster_arrive();
     if (PAIR && warp != 9) cluster_wait();
     tc_fence_after();
-    const uint32_t tmem = warp == 9 ? 0u : bars.tmem_base;
+    const uint32_t tmem = warp == 9 ? 0u : __shfl_sync(0xffffffffu, bars.tmem_base, 0);
 
     // a cluster a tile when the K range is cut, else every CTA (pair) takes every stride-th tile whole
     const int splits = 1 << lg_splits, rank = PAIR || (SWAP && lg_splits > 0) ? (int)cluster_ctarank() : 0;
@@ -251,7 +256,7 @@ mxfp8_mm_kernel(const MxArgs a, const int lg_splits, const __grid_constant__ MxM
     const int p_own = PAIR ? rank * 128 : 0;                 // ... of which this CTA's start here
     auto place = [&](int t, int& p0, int& q0) {              // of a tile (in P, this CTA's half)
         const int p = a.tiles_q == 1 ? t : (int)((unsigned)t / (unsigned)a.tiles_q);
-        p0 = p * kPRows + p_own;
+        p0 = p * (SWAP ? a.height : kPRows) + p_own;
         q0 = (t - p * a.tiles_q) * NT;
     };
     // K range cut: columns of the tile that CTA r of the cluster adds (none past the last row of Q)
@@ -316,6 +321,7 @@ mxfp8_mm_kernel(const MxArgs a, const int lg_splits, const __grid_constant__ MxM
         const uint32_t flag = smem_u32(&bars.abort);
         int s = 0, g = 0, done = 0;
         uint32_t ph = 0, g_ph = 0;
+        const uint32_t me = elect_one() ? 1u : 0u;
         for (int t = first; t < a.tiles; t += stride, ++done) {
             const int before = done - P::kLag;               // the tile whose drain makes room for this one
             if (before >= 0) mbar_wait_on(smem_u32(&bars.drained[before & 1]), (uint32_t)(before >> 1) & 1u, flag, spin);
@@ -332,25 +338,16 @@ mxfp8_mm_kernel(const MxArgs a, const int lg_splits, const __grid_constant__ MxM
                 tc_fence_after();
                 const uint32_t st = sbase + (uint32_t)s * P::kTile, sf = sf_base + (uint32_t)(g * P::kGroup + (k & 3) * P::kSf);
                 const uint32_t sp = tmem + (uint32_t)(P::kSf0 + s * P::kSfCols), sq = sp + 4;
-                if (elect_one()) {
-                    tmem_copy_scales<PAIR>(sp, sf);
+                tmem_copy_scales<PAIR>(me, sp, sf);
 #pragma unroll
-                    for (int h = 0; h < P::kQParts; ++h) tmem_copy_scales<PAIR>(sq + 4 * h, sf + 512 * (1 + h));
+                for (int h = 0; h < P::kQParts; ++h) tmem_copy_scales<PAIR>(me, sq + 4 * h, sf + 512 * (1 + h));
 #pragma unroll
-                    for (int kk = 0; kk < 4; ++kk)
-                        umma_mx<PAIR>(acc, smem_desc(st) + 2 * kk, smem_desc(st + 128 * kMxK) + 2 * kk, mx_idesc(kPRows, NT, kk), sp, sq,
-                                      (k > k0 || kk > 0) ? 1u : 0u);
-                    if (PAIR) umma_commit_pair(smem_u32(&bars.empty[s]));
-                    else umma_commit(smem_u32(&bars.empty[s]));
-                    if (last) {
-                        if (PAIR) umma_commit_pair(smem_u32(&bars.used[g]));
-                        else umma_commit(smem_u32(&bars.used[g]));
-                    }
-                    if (k == k1 - 1) {
-                        if (PAIR) umma_commit_pair(smem_u32(&bars.acc_full[done & 1]));
-                        else umma_commit(smem_u32(&bars.acc_full[done & 1]));
-                    }
-                }
+                for (int kk = 0; kk < 4; ++kk)
+                    umma_mx<PAIR>(me, acc, smem_desc(st) + 2 * kk, smem_desc(st + 128 * kMxK) + 2 * kk, mx_idesc(kPRows, NT, kk), sp, sq,
+                                  (k > k0 || kk > 0) ? 1u : 0u);
+                umma_commit_if<PAIR>(me, smem_u32(&bars.empty[s]));
+                if (last) umma_commit_if<PAIR>(me, smem_u32(&bars.used[g]));
+                if (k == k1 - 1) umma_commit_if<PAIR>(me, smem_u32(&bars.acc_full[done & 1]));
                 __syncwarp();
                 if (++s == P::kStages) {
                     s = 0;
@@ -467,7 +464,7 @@ mxfp8_mm_kernel(const MxArgs a, const int lg_splits, const __grid_constant__ MxM
                         for (int i = 0; i < (NT < 32 ? NT : 32); ++i)
                             if (q0 + c + i < a.q_rows) part[i * 128] = __uint_as_float(v[h][i]);
                     } else if (SWAP) {
-                        if (p0 + l < a.n_out) {
+                        if (p0 + l < a.n_out && l < a.height) {
                             __nv_bfloat16* at = a.y + (size_t)(q0 + c) * a.n_out + p0 + l;
 #pragma unroll
                             for (int i = 0; i < (NT < 32 ? NT : 32); ++i)
@@ -574,7 +571,7 @@ mxfp8_mm_kernel(const MxArgs a, const int lg_splits, const __grid_constant__ MxM
             place(t, p0, q0);
             for (int i = tid; i < 128 * NT; i += kMxThreads) {
                 const int p = p0 + i / NT, q = q0 + i % NT;
-                if (p < a.p_rows && q < a.q_rows) a.y[SWAP ? (size_t)q * a.n_out + p : (size_t)p * a.n_out + q] = __float2bfloat16_rn(__uint_as_float(0x7fc00000u));
+                if (p < a.p_rows && q < a.q_rows && (!SWAP || i / NT < a.height)) a.y[SWAP ? (size_t)q * a.n_out + p : (size_t)p * a.n_out + q] = __float2bfloat16_rn(__uint_as_float(0x7fc00000u));
             }
         }
     }
@@ -596,7 +593,7 @@ struct Call {
 };
 
 template <int NT, bool SWAP, bool PAIR = false>
-int launch(const Call& c, int lg_splits) {
+int launch(const Call& c, int lg_splits, int height = PAIR ? 256 : 128) {
     const int splits = 1 << lg_splits;
     MxArgs a = {};
     a.ps = SWAP ? c.ws : c.xs;
@@ -607,7 +604,8 @@ int launch(const Call& c, int lg_splits) {
     a.y = c.y;
     a.n_out = c.n_out;
     a.tiles_q = ceil_div(a.q_rows, NT);
-    const long tiles = (long)ceil_div(a.p_rows, PAIR ? 256 : 128) * a.tiles_q;
+    a.height = height;
+    const long tiles = (long)ceil_div(a.p_rows, height) * a.tiles_q;
     IMX_REQUIRE(tiles <= 0x7fffffffL / kMxMaxSplits, "mxfp8_matmul: too many outputs");
     a.tiles = (int)tiles;
     auto piece = [&](const uint8_t* s) { return (uintptr_t)s % 16 == 0 && c.in % 512 == 0 ? 16 : ((uintptr_t)s % 4 == 0 && c.in % 128 == 0 ? 4 : 1); };
@@ -616,7 +614,7 @@ int launch(const Call& c, int lg_splits) {
     a.spin_limit = g_mx_spin_limit.load();
     a.status = c.status;
     // rows of x that do not exist are not brought: what the lanes hold in their place reaches no output
-    const int p_box = !SWAP && c.m < 128 ? (c.m + 7) & ~7 : 128;
+    const int p_box = SWAP ? height : (c.m < 128 ? (c.m + 7) & ~7 : 128);
     a.stage_bytes = (p_box + Plan<NT, SWAP, PAIR>::kQRows) * kMxK;
     MxMaps maps;
     IMX_TRY(encode_tensor_map_2d(SWAP ? c.w : c.x, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, (size_t)a.p_rows, (size_t)c.in, (size_t)c.in, kMxK, p_box, 128, true, &maps.p));
@@ -643,12 +641,13 @@ int launch(const Call& c, int lg_splits) {
 
 // Which kernel: the least of a model of their times in us, a part that does not shrink and a time for each K step of each wave
 // of tiles, fitted to the kernels alone on a B200 (2048 -> 8192 unless said; measured, in brackets the model):
-//   1 row     S16 8.9 (8.6), S16 cut in 2 7.7 (7.8), N64 9.4 (9.6);   2048 -> 512  S16 cut in 1, 2, 4, 8  8.2, 6.3, 5.4, 5.3
-//   64 rows   S64 11.4 (11.3), S64 cut in 2 10.9 (9.9), N64 9.7 (9.6);   4096 -> 2048  S64 cut in 4 9.6 (9.9), N64 14.0 (14.4)
-//   256 rows  N64 15.0 (14.4), N128 10.9 (10.9), P128 10.6 (10.5), P256 12.5 (11.7)
-//   777 rows 4096 -> 2048  N128 16.5 (17.0), P128 14.5 (14.8), P256 17.9 (17.8)
-//   1024 rows N128 27.6 (23.0), P256 19.8 (18.0);   2048 -> 152064, 64 rows  S64 60.4, N64 91, N128 61, P256 70 (memory: 52)
-// Clusters of eight that fill the GPU find no place together: 4096 -> 2048, 1 row, cut in 8 (128 CTAs) 11.8, in 4 7.3.
+//   1 row     S16 7.3 (7.3), S16 cut in 2 7.1 (6.7);   2048 -> 512  S16 cut in 1, 2, 4, 8  6.6, 5.8, 5.1, 5.1
+//   64 rows   S64 9.5 (9.4), S64 cut in 2 10.2, N64 8.0 (7.9);   4096 -> 2048  S64 cut in 4 8.5 (8.8), N64 10.2 (11.2)
+//   256 rows  N64 11.6 (11.2), N128 9.1 (9.2), P128 9.5 (9.5), P256 11.9 (12.1)
+//   777 rows 4096 -> 2048  N64 17.8 (17.8), N128 12.9 (12.9), P128 12.9 (12.8), P256 17.1 (17.8)
+//   1024 rows N128 20.8 (20.4), P128 19.4 (19.5), P256 18.2 (17.8);   8192 rows  N128 131, P128 116, P256 100
+//   64 rows 2048 -> 152064  S64 58, N64 65, N128 59, P128 73, P256 71 (memory: 52)
+// Clusters of eight that fill the GPU find no place together: 4096 -> 2048, 1 row, cut in 8 (128 CTAs) 11.3, in 4 6.7.
 int run(const Call& c) {
     const int steps = ceil_div(c.in, kMxK);
     enum { S16, S32, S64, N64, N128, P128, P256 } best = P256;
@@ -666,17 +665,23 @@ int run(const Call& c) {
     const int nt = c.m <= 16 ? 16 : (c.m <= 32 ? 32 : 64);
     const long tiles = (long)ceil_div(c.n_out, 128) * ceil_div(c.m, nt);
     for (int lg = 0; lg < 4 && (lg == 0 || (tiles << lg <= (lg == 3 ? 64 : c.sms) && steps >= 2 << lg)); ++lg)
-        offer(nt == 16 ? S16 : (nt == 32 ? S32 : S64), lg, 4.6f + 0.03f * nt + (lg > 0 ? 1.f : 0.f), tiles, lg > 0 ? (int)tiles : c.sms,
-              nt == 64 ? 0.30f : 0.22f);
+        offer(nt == 16 ? S16 : (nt == 32 ? S32 : S64), lg, 3.4f + 0.044f * nt + (lg > 0 ? 1.f : 0.f), tiles, lg > 0 ? (int)tiles : c.sms, 0.2f);
     const long rows128 = ceil_div(c.m, 128);
-    offer(N64, 0, 4.8f, rows128 * ceil_div(c.n_out, 64), c.sms, 0.30f);
-    offer(N128, 0, 4.8f, rows128 * ceil_div(c.n_out, 128), c.sms, 0.38f);
-    offer(P128, 0, 6.2f, (long)ceil_div(c.m, 256) * ceil_div(c.n_out, 128), c.sms / 2, 0.27f);
-    offer(P256, 0, 5.5f, (long)ceil_div(c.m, 256) * ceil_div(c.n_out, 256), c.sms / 2, 0.39f);
+    offer(N64, 0, 4.6f, rows128 * ceil_div(c.n_out, 64), c.sms, 0.206f);
+    offer(N128, 0, 5.4f, rows128 * ceil_div(c.n_out, 128), c.sms, 0.235f);
+    offer(P128, 0, 6.1f, (long)ceil_div(c.m, 256) * ceil_div(c.n_out, 128), c.sms / 2, 0.21f);
+    offer(P256, 0, 6.3f, (long)ceil_div(c.m, 256) * ceil_div(c.n_out, 256), c.sms / 2, 0.36f);
+    // More than one wave of weight tiles: all of them as low as the number of waves allows, so that the last is full too.  64
+    // rows, 2048 -> 152064 (9 waves for 8.03 of 128 outputs) 55.3 us, with 128 56.7; 8 rows, 2048 -> 40000, 17.8 and 19.9.
+    int height = 128;
+    if (best <= S64 && best_lg == 0 && tiles > c.sms) {
+        const long per_q = (tiles + c.sms - 1) / c.sms * c.sms / ceil_div(c.m, nt);
+        height = (int)((c.n_out + per_q - 1) / per_q + 3) & ~3;
+    }
     switch (best) {
-        case S16: return launch<16, true>(c, best_lg);
-        case S32: return launch<32, true>(c, best_lg);
-        case S64: return launch<64, true>(c, best_lg);
+        case S16: return launch<16, true>(c, best_lg, height);
+        case S32: return launch<32, true>(c, best_lg, height);
+        case S64: return launch<64, true>(c, best_lg, height);
         case N64: return launch<64, false>(c, 0);
         case N128: return launch<128, false>(c, 0);
         case P128: return launch<128, false, true>(c, 0);

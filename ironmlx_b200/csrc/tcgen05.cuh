@@ -149,6 +149,32 @@ __device__ __forceinline__ void umma_ss(uint32_t tmem_d, uint64_t da, uint64_t d
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
+// The same for the lane whose `me` is 1 (one of the warp, elected before), by a predicate: without a branch around them the
+// operands stay in uniform registers.  Four block-scaled MMAs, two copies of scales and a commit take 160 cycles to issue so,
+// under `if (elect_one())` 360 (M = 128, N = 16).  The warp's number and what it has from shared memory have to be uniform for
+// the compiler too (__shfl_sync), which saves another 60.
+__device__ __forceinline__ void umma_ss_if(uint32_t me, uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %6, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+        ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate), "r"(0u), "r"(me)
+        : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void umma_commit_if(uint32_t me, uint32_t bar) {
+    if (PAIR)
+        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %2, 0;\n\t"
+                     "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}"
+                     ::"r"(bar), "h"((uint16_t)3), "r"(me)
+                     : "memory");
+    else
+        asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+                     "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+                     ::"r"(bar), "r"(me)
+                     : "memory");
+}
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 "

@@ -178,7 +178,7 @@ def check_product(y, rows, w):
     (1, 32, 1), (1, 2048, 8192), (1, 544, 129), (2, 64, 7), (5, 96, 40), (8, 4096, 512), (16, 512, 1000), (17, 160, 128), (33, 2048, 384),
     (64, 2048, 2048), (65, 128, 256), (100, 8192, 64), (128, 1056, 136), (129, 2048, 1024), (200, 512, 4096), (300, 4128, 520),
     (777, 4096, 2048), (1000, 64, 2000), (1025, 2048, 2056), (2300, 512, 777), (513, 96, 8200), (4100, 1024, 1280),
-    (400, 2080, 2501), (390, 2112, 2504)])
+    (400, 2080, 2501), (390, 2112, 2504), (5, 512, 20000), (40, 1056, 19001), (20, 256, 40010)])
 def test_mxfp8_matmul(cuda, m, n_in, n_out):
     g = gen(m + n_in + n_out)
     rows, w = mx(g, m, n_in), mx(g, n_out, n_in, 0.02)
@@ -189,7 +189,7 @@ def test_mxfp8_matmul(cuda, m, n_in, n_out):
     ops.check_status(cuda)
 
 
-@pytest.mark.parametrize("m,n_in,n_out", [(3, 512, 200), (48, 2048, 256), (130, 1152, 300), (700, 256, 1030), (390, 2112, 2504)])
+@pytest.mark.parametrize("m,n_in,n_out", [(3, 512, 200), (48, 2048, 256), (130, 1152, 300), (700, 256, 1030), (390, 2112, 2504), (8, 544, 20004)])
 def test_mxfp8_matmul_of_whole_numbers_is_exact(cuda, m, n_in, n_out):
     """Codes -1, 0, 1 with scales 2^-2 .. 2^2 (a different one for every block): sums are multiples of 2^-4 under 2^16, exact
     in fp32 in any order, so that every output is the one rounding of its sum.  A scale that reaches the wrong row, column or
@@ -279,7 +279,7 @@ def test_layers(cuda):
         nn.QuantizedLinear.new(*q4, 64, 4).forward_rows(rows)
 
 
-@pytest.mark.parametrize("m,n_in,n_out", [(8, 2048, 256), (600, 512, 1024), (128, 64, 40000), (400, 2080, 2504)])
+@pytest.mark.parametrize("m,n_in,n_out", [(8, 2048, 256), (600, 512, 1024), (128, 64, 40000), (400, 2080, 2504), (8, 256, 20000)])
 def test_expired_wait_gives_nan_and_a_status(cuda, m, n_in, n_out):
     """With every wait giving up at once nothing is copied or multiplied: outputs are NaN, the status is reported once, the
     next call is right again."""
