@@ -6,12 +6,11 @@
 // Both operands have the same form, so that one kernel serves both orientations: P (128 rows, the lanes of the accumulator) and
 // Q (NT rows, its columns), both K-major with 128-byte swizzle, 128 codes a stage.
 //   few rows of x   P = weight, Q = the rows (SWAP): the weight's bytes bound it, its tiles are spread over the SMs
-//   many rows       P = the rows, Q = weight: the tensor cores bound it.  With 128 columns or more by pairs of CTAs
-//                   (cta_group::2), each of which brings half of Q: an SM takes in 85 to 95 GB/s of tiles, whatever their
-//                   shape, and that bounds all products that are not large.
+//   many rows       P = the rows, Q = weight: the tensor cores bound it.  Tiles of 256 rows by pairs of CTAs
+//                   (cta_group::2), each of which brings half of Q.
 // Few tiles for the GPU: the K range of a tile is cut over the CTAs of a cluster; each leaves its fp32 sums in shared memory,
-// sends every other CTA its columns in one bulk copy (7.7 us for a row, 2048 -> 8192; read by the receiver 8.7, sent word by
-// word 9.5) and adds its own over all of them, in rank order.
+// sends every other CTA its columns in one bulk copy (a row, 2048 -> 8192, cut in two: 7.7 us, read by the receiver
+// 8.7, sent word by word 9.5, when the rest took 0.7 longer than now) and adds its own over all of them, in rank order.
 //
 // Scales lie in memory as the format has them, [rows, in / 32] bytes.  The MMA reads them from tensor memory, four K steps in
 // a word, row r in lane r mod 32 of column r / 32: four warps fetch them as 16-byte pieces a row (four stages at a time, one
@@ -20,14 +19,14 @@
 // MMAs that read both.  Rows and blocks past the end get the scale 1 and, from TMA, codes of zero.
 //
 // Eleven warps: 0..3 epilogue, 4..7 scales, 8 MMA and tensor memory, 9 loads, 10 (of a pair) tells CTA 0, whose warp 8 issues
-// the MMAs of both, what has arrived in its own.  Two accumulators alternate, so that the next
-// tile's MMAs run beside the epilogue; 2 x 256 columns leave no room for the scales: at NT = 256 the two share 48 columns,
+// the MMAs of both, what has arrived in its own.  Two accumulators alternate, so that the next tile's MMAs run beside the epilogue; 2 x 256 columns leave no room for the scales: at NT = 256 the two share 48 columns,
 // which the epilogue takes out first.  Every wait is bounded; on expiry what is in flight is waited for, tensor memory is
 // freed, the status word is set and the tiles concerned are NaN.
 //
-// On a B200, the kernel alone: 8192 rows, 2048 -> 8192, 105 us, 2.6 PFLOP/s, 79% of twice cuBLAS' bf16 rate (the tensor
-// cores busy 73% of the time; in a loop of seconds the power limit makes it 122 us); 777 rows, 4096 -> 2048, 14.6 us; 64 rows, 2048 -> 152064, 61 us, 5.6 TB/s;
-// one row, 2048 -> 8192, 7.8 us, of which 4.6 are a launch's, the ring's filling and the cluster's.
+// On a B200, the kernel alone: 8192 rows, 2048 -> 8192, 102 us, 2.7 PFLOP/s, 81% of twice cuBLAS' bf16 rate (in a loop of
+// seconds the power limit makes it 122 to 125 us); 777 rows, 4096 -> 2048, 12.2 us; 64 rows, 2048 -> 152064, 55 us, 6.2 TB/s; one row,
+// 2048 -> 8192, 7 us, of which 4 are a launch's and the ring's filling.  What a K step of 128 costs beside its MMAs bounds all that
+// is not large: 340 cycles for the warp that issues them, before it issued by predicates and looked ahead 600.
 #include <atomic>
 
 #include "tcgen05.cuh"
@@ -322,6 +321,7 @@ mxfp8_mm_kernel(const MxArgs a, const int lg_splits, const __grid_constant__ MxM
         int s = 0, g = 0, done = 0;
         uint32_t ph = 0, g_ph = 0;
         const uint32_t me = elect_one() ? 1u : 0u;
+        uint32_t ready = 0;
         for (int t = first; t < a.tiles; t += stride, ++done) {
             const int before = done - P::kLag;               // the tile whose drain makes room for this one
             if (before >= 0) mbar_wait_on(smem_u32(&bars.drained[before & 1]), (uint32_t)(before >> 1) & 1u, flag, spin);
@@ -330,12 +330,15 @@ mxfp8_mm_kernel(const MxArgs a, const int lg_splits, const __grid_constant__ MxM
             for (int k = k0; k < k1; ++k) {
                 const bool last = (k & 3) == 3 || k == k1 - 1;           // of the group
                 if (PAIR) {
-                    mbar_wait_on(smem_u32(&bars.both[s]), ph, flag, spin);
+                    mbar_wait_on(smem_u32(&bars.both[s]), ph, flag, spin, ready);
                 } else {
-                    mbar_wait_on(smem_u32(&bars.full[s]), ph, flag, spin);
+                    mbar_wait_on(smem_u32(&bars.full[s]), ph, flag, spin, ready);
                     if (k == k0 || (k & 3) == 0) mbar_wait_on(smem_u32(&bars.scales[g]), g_ph, flag, spin);
                 }
                 tc_fence_after();
+                // (the next stage, looked at while this one's MMAs are issued: a wait that need not be costs 80 cycles)
+                const bool wrap = s + 1 == P::kStages;
+                ready = mbar_peek(smem_u32(PAIR ? &bars.both[wrap ? 0 : s + 1] : &bars.full[wrap ? 0 : s + 1]), ph ^ (uint32_t)wrap);
                 const uint32_t st = sbase + (uint32_t)s * P::kTile, sf = sf_base + (uint32_t)(g * P::kGroup + (k & 3) * P::kSf);
                 const uint32_t sp = tmem + (uint32_t)(P::kSf0 + s * P::kSfCols), sq = sp + 4;
                 tmem_copy_scales<PAIR>(me, sp, sf);
@@ -641,12 +644,12 @@ int launch(const Call& c, int lg_splits, int height = PAIR ? 256 : 128) {
 
 // Which kernel: the least of a model of their times in us, a part that does not shrink and a time for each K step of each wave
 // of tiles, fitted to the kernels alone on a B200 (2048 -> 8192 unless said; measured, in brackets the model):
-//   1 row     S16 7.3 (7.3), S16 cut in 2 7.1 (6.7);   2048 -> 512  S16 cut in 1, 2, 4, 8  6.6, 5.8, 5.1, 5.1
-//   64 rows   S64 9.5 (9.4), S64 cut in 2 10.2, N64 8.0 (7.9);   4096 -> 2048  S64 cut in 4 8.5 (8.8), N64 10.2 (11.2)
-//   256 rows  N64 11.6 (11.2), N128 9.1 (9.2), P128 9.5 (9.5), P256 11.9 (12.1)
-//   777 rows 4096 -> 2048  N64 17.8 (17.8), N128 12.9 (12.9), P128 12.9 (12.8), P256 17.1 (17.8)
-//   1024 rows N128 20.8 (20.4), P128 19.4 (19.5), P256 18.2 (17.8);   8192 rows  N128 131, P128 116, P256 100
-//   64 rows 2048 -> 152064  S64 58, N64 65, N128 59, P128 73, P256 71 (memory: 52)
+//   1 row     S16 6.9 (7.0), S16 cut in 2 7.1 (7.5);   2048 -> 512  S16 cut in 1, 2, 4, 8  6.1, 5.6, 5.0, 5.1
+//   64 rows   S64 9.5 (9.4), S64 cut in 2 10.2 (9.8), N64 7.7 (7.7);   4096 -> 2048  S64 cut in 4 8.5 (8.8), N64 9.6 (10.6)
+//   256 rows  N64 11.1 (10.6), N128 9.1 (9.0), P128 9.7 (9.5), P256 11.9 (12.1)
+//   777 rows 4096 -> 2048  N64 16.7 (16.5), N128 12.6 (12.6), P128 12.8 (12.8), P256 17.4 (17.8)
+//   1024 rows N128 20.8 (19.8), P128 19.4 (19.5), P256 18.2 (17.8);   8192 rows  N128 130, P128 115, P256 99
+//   64 rows 2048 -> 152064  S64 55, N64 63, N128 58, P128 70, P256 68 (memory: 52)
 // Clusters of eight that fill the GPU find no place together: 4096 -> 2048, 1 row, cut in 8 (128 CTAs) 11.3, in 4 6.7.
 int run(const Call& c) {
     const int steps = ceil_div(c.in, kMxK);
@@ -665,10 +668,11 @@ int run(const Call& c) {
     const int nt = c.m <= 16 ? 16 : (c.m <= 32 ? 32 : 64);
     const long tiles = (long)ceil_div(c.n_out, 128) * ceil_div(c.m, nt);
     for (int lg = 0; lg < 4 && (lg == 0 || (tiles << lg <= (lg == 3 ? 64 : c.sms) && steps >= 2 << lg)); ++lg)
-        offer(nt == 16 ? S16 : (nt == 32 ? S32 : S64), lg, 3.4f + 0.044f * nt + (lg > 0 ? 1.f : 0.f), tiles, lg > 0 ? (int)tiles : c.sms, 0.2f);
+        offer(nt == 16 ? S16 : (nt == 32 ? S32 : S64), lg, 3.4f + 0.044f * nt + (lg > 0 ? 1.f : 0.f) + (lg > 0 && tiles << lg > c.sms / 2 ? 1.f : 0.f), tiles,
+              lg > 0 ? (int)tiles : c.sms, nt == 64 ? 0.2f : 0.18f);
     const long rows128 = ceil_div(c.m, 128);
-    offer(N64, 0, 4.6f, rows128 * ceil_div(c.n_out, 64), c.sms, 0.206f);
-    offer(N128, 0, 5.4f, rows128 * ceil_div(c.n_out, 128), c.sms, 0.235f);
+    offer(N64, 0, 4.7f, rows128 * ceil_div(c.n_out, 64), c.sms, 0.185f);
+    offer(N128, 0, 5.4f, rows128 * ceil_div(c.n_out, 128), c.sms, 0.225f);
     offer(P128, 0, 6.1f, (long)ceil_div(c.m, 256) * ceil_div(c.n_out, 128), c.sms / 2, 0.21f);
     offer(P256, 0, 6.3f, (long)ceil_div(c.m, 256) * ceil_div(c.n_out, 256), c.sms / 2, 0.36f);
     // More than one wave of weight tiles: all of them as low as the number of waves allows, so that the last is full too.  64

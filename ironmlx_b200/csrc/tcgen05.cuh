@@ -65,10 +65,18 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatil
 // Wait of the warp that issues the MMAs.  Its outcome must not steer the code: the compiler would take all that follows for
 // divergent and move the operands of every MMA to uniform registers, 50 cycles each.  So an expired wait sets the abort flag,
 // the later ones return at once, and what is then multiplied is never used.
-__device__ __forceinline__ void mbar_wait_on(uint32_t bar, uint32_t parity, uint32_t abort_flag, int limit) {
+// `ready`: what mbar_peek said of the same barrier and phase a while before.
+__device__ __forceinline__ uint32_t mbar_peek(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+    return ok;
+}
+__device__ __forceinline__ void mbar_wait_on(uint32_t bar, uint32_t parity, uint32_t abort_flag, int limit, uint32_t ready = 0) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t.reg .u32 n, f;\n\t"
-        "mov.u32 n, %3;\n"
+        "mov.u32 n, %3;\n\t"
+        "setp.ne.u32 p, %4, 0;\n\t"
+        "@p bra arrived;\n"
         "try_again:\n\t"
         "setp.eq.u32 p, n, 0;\n\t"
         "@p bra expired;\n\t"
@@ -81,7 +89,7 @@ __device__ __forceinline__ void mbar_wait_on(uint32_t bar, uint32_t parity, uint
         "expired:\n\t"
         "st.volatile.shared.u32 [%2], 1;\n"
         "arrived:\n\t}"
-        ::"r"(bar), "r"(parity), "r"(abort_flag), "r"(limit)
+        ::"r"(bar), "r"(parity), "r"(abort_flag), "r"(limit), "r"(ready)
         : "memory");
 }
 
