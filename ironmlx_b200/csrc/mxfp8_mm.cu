@@ -19,7 +19,7 @@
 // MMAs that read both.  Rows and blocks past the end get the scale 1 and, from TMA, codes of zero.
 //
 // Eleven warps: 0..3 epilogue, 4..7 scales, 8 MMA and tensor memory, 9 loads, 10 (of a pair) tells CTA 0, whose warp 8 issues
-// the MMAs of both, what has arrived in its own.  Two accumulators alternate, so that the next tile's MMAs run beside the epilogue; 2 x 256 columns leave no room for the scales: at NT = 256 the two share 48 columns,
+// the MMAs of both, what has arrived in its own.  Two accumulators alternate, so that the next tile's MMAs run beside the epilogue; 2 x 256 columns leave no room for the scales: at NT = 256 the two share 60 columns,
 // which the epilogue takes out first.  Every wait is bounded; on expiry what is in flight is waited for, tensor memory is
 // freed, the status word is set and the tiles concerned are NaN.
 //
@@ -57,13 +57,14 @@ struct Plan {
     // epilogue: 32 rows x 64 outputs for each of its warps; SWAP: the tile's fp32 sums, a part from each CTA of the cluster
     static constexpr int kOut = SWAP ? 128 * NT * 4 : 4 * 4096;
     static constexpr int kFit = (int)((227 * 1024 - 4096 - kMxGroups * kGroup - kOut) / kTile);
-    static constexpr int kStages = kFit < kMxMaxStages ? kFit : kMxMaxStages;
+    static constexpr int kMost = NT == 256 ? 5 : kMxMaxStages;           // (so that the accumulators share 64 columns at most)
+    static constexpr int kStages = kFit < kMost ? kFit : kMost;
     static constexpr int kSfCols = 4 * (1 + kQParts);
     static constexpr int kSf0 = NT == 256 ? 512 - kStages * kSfCols : 256;   // columns of the scales, a place for every stage, ...
     static constexpr int kAcc1 = NT == 256 ? kSf0 - 256 : NT;            // ... of the second accumulator
     static constexpr int kLag = NT == 256 ? 1 : 2;                       // a tile's MMAs wait for the drain of the kLag-th before
     static constexpr size_t kSmem = (size_t)kStages * kTile + kMxGroups * kGroup + kOut + 2048;
-    static_assert(kSf0 + kStages * kSfCols <= 512 && (NT < 256 || kAcc1 >= 128), "tensor memory");
+    static_assert(kSf0 + kStages * kSfCols <= 512 && (NT < 256 || kAcc1 >= 192), "tensor memory");
 };
 
 struct MxBars {
@@ -445,11 +446,11 @@ mxfp8_mm_kernel(const MxArgs a, const int lg_splits, const __grid_constant__ MxM
             const uint32_t acc = tmem + quarter + (buf ? (uint32_t)P::kAcc1 : 0u);
             for (int pr = 0; pr < kPairs; ++pr) {
                 // the columns that the two accumulators share come first
-                const int c0 = NT == 256 && buf == 0 ? (2 * pr + 4) & 7 : 2 * pr;
+                const int c0 = NT == 256 && buf == 0 ? (2 * pr + 6) & 7 : 2 * pr;
                 uint32_t v[2][32];
                 tmem_ld32(acc + (uint32_t)(c0 * 32), v[0]);
                 if (kChunks > 1) tmem_ld32(acc + (uint32_t)(c0 * 32 + 32), v[1]);
-                if (pr == (NT == 256 ? 1 : kPairs - 1)) {
+                if (pr == (NT == 256 ? 0 : kPairs - 1)) {
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) {
