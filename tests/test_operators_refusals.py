@@ -1,6 +1,9 @@
 """What `imx_add_rms_norm`, `imx_mxfp8_matmul` and `imx_low_rank_add` refuse, and that they refuse it on the host: the
 addresses given here are not memory, no GPU is needed."""
 import ctypes as C
+import os
+import shutil
+import subprocess
 
 import pytest
 import torch
@@ -102,6 +105,29 @@ def test_more_rows_than_an_int_counts():
     assert ops._row_count("op", x.expand(0x7fffffff, 8), 8) == 0x7fffffff
     with pytest.raises(_lib.IronMLXError, match="rows"):
         ops._row_count("op", x.expand(1 << 31, 8), 8)
+
+
+def build_cpp(out_dir):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    exe, cuda, lib_dir = os.path.join(out_dir, "operators_main"), os.environ.get("CUDA_HOME", "/usr/local/cuda"), os.path.dirname(_lib.LIB_PATH)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-I", os.path.join(root, "include"), "-I", os.path.join(cuda, "include"),
+                    os.path.join(root, "tests", "cpp", "operators_main.cpp"), "-o", exe, "-L", lib_dir, "-l:libironmlx_b200.so",
+                    "-L", os.path.join(cuda, "lib64"), "-lcudart", f"-Wl,-rpath,{lib_dir}", f"-Wl,-rpath,{os.path.join(cuda, 'lib64')}"],
+                   check=True, capture_output=True, text=True)
+    return exe
+
+
+def test_cpp_mirror_refuses_shapes(tmp_path):
+    if shutil.which("g++") is None or not os.path.exists(_lib.LIB_PATH):
+        pytest.skip("g++ or the library is missing")
+    done = subprocess.run([build_cpp(str(tmp_path)), "refuse"], capture_output=True, text=True)
+    assert done.returncode == 0, done.stdout + done.stderr
+
+
+@pytest.mark.gpu
+def test_cpp_mirror_runs_the_operators(cuda, tmp_path):
+    done = subprocess.run([build_cpp(str(tmp_path)), "run"], capture_output=True, text=True)
+    assert done.returncode == 0, done.stdout + done.stderr
 
 
 def test_streams_of_another_device():
