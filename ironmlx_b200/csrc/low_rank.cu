@@ -493,7 +493,8 @@ __device__ __forceinline__ void tmem_wait(uint32_t (&u)[16]) {
 // copies, adds and writes 16 rows x 32 columns that no other warp touches, so that the warps meet nowhere but at the
 // accumulators (with a __syncthreads and the MMAs' issue in every stage 8192 tokens of rank 16 took 97 us).
 // `clusters` clusters a unit: each multiplies x . a^T for itself and takes a part of the columns.
-template <int NJ>
+// WIDE: rows of y and of out are whole 16-byte pieces.
+template <int NJ, bool WIDE>
 __global__ void __launch_bounds__(kTileThreads, NJ <= 2 ? 2 : 1)
 low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, const __grid_constant__ TileMaps maps) {
     extern __shared__ unsigned char smem_raw[];
@@ -644,7 +645,7 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
             for (int r = warp; r < m; r += kTileThreads / 32) {
                 const size_t at = (size_t)s.rows[r] * p.n_out;
                 const int end = min(n1 * kCols, p.n_out);
-                if (p.wide)
+                if (WIDE)
                     for (int n = n0 * kCols + lane * 8; n < end; n += 256) *reinterpret_cast<uint4*>(p.out + at + n) = *reinterpret_cast<const uint4*>(p.y + at + n);
                 else
                     for (int n = n0 * kCols + lane; n < end; n += 32) p.out[at + n] = p.y[at + n];
@@ -778,7 +779,7 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
                     xr[0] += kCols;
                     xr[1] += kCols;
                 } else {
-                    if (p.wide) {
+                    if (WIDE) {
 #pragma unroll
                         for (int i = 0; i < 2; ++i)
                             if (y_left > 0 && has_own[i]) copy16(to + y_at[i], yr[i], true);
@@ -865,6 +866,21 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
         int n = n0 * kCols;                                // first column of the stage
         uint32_t y = base + (uint32_t)((n_in % S) * pl.stage);                   // ... and its place
         const uint32_t frag_at = (uint32_t)((rt * 16 + (lane & 7)) * 128 + (((half * 4 + (lane >> 3)) ^ (lane & 7)) * 16));
+        // Rows that start on 4 bytes, not on 16: a lane's own values two at a time, a stage ahead (5034 outputs, 2579 rows of rank
+        // 128: 66 us, one by one when they are needed 171).  Rows of an odd number are left at that.
+        const bool pairs = !WIDE && p.n_out % 2 == 0 && (((uintptr_t)p.y | (uintptr_t)p.out) % 4) == 0;
+        const size_t row_at[2] = {(size_t)s.rows[has_own[0] ? rt * 16 + g : 0] * p.n_out, (size_t)s.rows[has_own[1] ? rt * 16 + g + 8 : 0] * p.n_out};
+        uint32_t ahead[2][4];
+        auto fetch = [&](int from) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int col = from + half * 32 + j * 8 + 2 * q;
+                    ahead[h][j] = has_own[h] && col < p.n_out ? *reinterpret_cast<const uint32_t*>(p.y + row_at[h] + col) : 0u;
+                }
+        };
+        if (pairs && total > n_in) fetch(n);
         for (int e = 0; e < total - n_in; ++e) {
             wait(s.sums_there[e & 1], e >> 1);
             tc::tc_fence_after();
@@ -872,7 +888,7 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
             tmem_ld_16x32(tmem + ((uint32_t)(rt * 32) << 16) + (uint32_t)((e & 1) * 64 + half * 32), u);
             arrived();
             __syncwarp();
-            if (p.wide) {
+            if (WIDE) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) ld_matrices(y + frag_at + h * 1024, v[h]);
             }
@@ -883,7 +899,7 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
             float d[16];
 #pragma unroll
             for (int i = 0; i < 16; ++i) d[i] = __uint_as_float(u[i]);
-            if (p.wide) {
+            if (WIDE) {
                 // added in y's place, which is read and written as 8 x 8 matrices (the sums' layout), out in 16-byte pieces
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -900,14 +916,31 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
                 const uint4 o0 = ld_shared16(y + y_at[0]), o1 = ld_shared16(y + y_at[1]);
                 if (has_own[0] && in) *reinterpret_cast<uint4*>(to_own[0]) = o0;
                 if (has_own[1] && in) *reinterpret_cast<uint4*>(to_own[1]) = o1;
+            } else if (pairs) {
+                uint32_t now[2][4];
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) now[h][j] = ahead[h][j];
+                if (e + 1 < total - n_in) fetch(n + kCols);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int col = n + half * 32 + j * 8 + 2 * q;
+                        if (!has_own[h] || col >= p.n_out) continue;
+                        const float2 f = __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&now[h][j]));
+                        const __nv_bfloat162 o = __floats2bfloat162_rn(f.x + d[4 * j + 2 * h], f.y + d[4 * j + 2 * h + 1]);
+                        *reinterpret_cast<__nv_bfloat162*>(p.out + row_at[h] + col) = o;
+                    }
             } else {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
 #pragma unroll
                     for (int h = 0; h < 4; ++h) {
-                        const int r = rt * 16 + g + 8 * (h >> 1), col = n + half * 32 + j * 8 + 2 * q + (h & 1);
-                        if (r < m && col < p.n_out) {
-                            const size_t at = (size_t)s.rows[r] * p.n_out + col;
+                        const int col = n + half * 32 + j * 8 + 2 * q + (h & 1);
+                        if (has_own[h >> 1] && col < p.n_out) {
+                            const size_t at = row_at[h >> 1] + col;
                             p.out[at] = __float2bfloat16_rn(__bfloat162float(p.y[at]) + d[4 * j + h]);
                         }
                     }
@@ -943,12 +976,14 @@ struct TileKernel {
     const void* kernel;
     int nj;
 };
-TileKernel tile_kernel(int rank) {
-    if (rank <= 32) return {(const void*)low_rank_tile_kernel<1>, 1};
-    if (rank <= 64) return {(const void*)low_rank_tile_kernel<2>, 2};
-    if (rank <= 128) return {(const void*)low_rank_tile_kernel<4>, 4};
-    return {(const void*)low_rank_tile_kernel<8>, 8};
+template <bool WIDE>
+TileKernel tile_kernel_of(int rank) {
+    if (rank <= 32) return {(const void*)low_rank_tile_kernel<1, WIDE>, 1};
+    if (rank <= 64) return {(const void*)low_rank_tile_kernel<2, WIDE>, 2};
+    if (rank <= 128) return {(const void*)low_rank_tile_kernel<4, WIDE>, 4};
+    return {(const void*)low_rank_tile_kernel<8, WIDE>, 8};
 }
+TileKernel tile_kernel(int rank, bool wide) { return wide ? tile_kernel_of<true>(rank) : tile_kernel_of<false>(rank); }
 
 int launch_clusters(const void* kernel, unsigned grid, int threads, int ctas, size_t smem, cudaStream_t stream, void** args) {
     cudaLaunchConfig_t cfg = {};
@@ -1009,7 +1044,7 @@ int launch_low_rank(LowRankArgs p, int sms, cudaStream_t stream) {
         while (ctas < 8 && units * ctas * 2 <= 2 * sms) ctas *= 2;
         int clusters = 1;
         while (clusters < 8 && units * ctas * clusters * 2 <= 2 * sms && p.n_out >= 2 * kCols * ctas * clusters) clusters *= 2;
-        const TileKernel tile = tile_kernel(p.rank);
+        const TileKernel tile = tile_kernel(p.rank, p.wide != 0);
         args[2] = &clusters;
         args[3] = &maps;
         IMX_TRY(launch_clusters(tile.kernel, (unsigned)(units * ctas * clusters), kTileThreads, ctas, (size_t)TilePlan(p.rank, tile.nj).bytes + 1024, stream, args));
@@ -1064,8 +1099,10 @@ extern "C" int imx_low_rank_add(const void* y, const void* x, int n_rows, int in
         for (int rank : {8, 16, 32, 64, 128, 256}) {
             const FewKernel few = few_kernel(rank);
             IMX_CHECK_CUDA(cudaFuncSetAttribute(few.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FewPlan(rank, few.rb).bytes));
-            const TileKernel tile = tile_kernel(rank);
-            IMX_CHECK_CUDA(cudaFuncSetAttribute(tile.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TilePlan(rank, tile.nj).bytes + 1024));
+            for (bool wide : {false, true}) {
+                const TileKernel tile = tile_kernel(rank, wide);
+                IMX_CHECK_CUDA(cudaFuncSetAttribute(tile.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TilePlan(rank, tile.nj).bytes + 1024));
+            }
         }
         device_mark_setup(di.ordinal, kSetupLowRank);
     }

@@ -40,7 +40,8 @@ def run(p, ids, **kw):
 @pytest.mark.parametrize("t,k,n,count,rank", [
     (1, 2048, 8192, 1, 16), (1, 8, 1, 1, 8), (2, 64, 7, 3, 8), (5, 4096, 2048, 4, 64), (16, 2048, 512, 40, 32), (48, 4096, 2048, 40, 32),
     (31, 1000, 1001, 2, 24), (64, 512, 264, 64, 256), (100, 2048, 1024, 3, 128), (130, 96, 200, 5, 16), (300, 2048, 2048, 1, 16),
-    (777, 2056, 1032, 5, 40), (1100, 512, 513, 12, 64), (140, 8, 16, 1, 8), (131, 200, 72, 3, 200), (8500, 128, 200, 9, 48), (150, 64, 128, 2500, 8), (2050, 256, 384, 200, 8), (600, 4096, 136, 2, 256), (5000, 64, 96, 3, 16), (400, 1024, 2048, 2, 128), (260, 3000, 1500, 1, 256)])
+    (777, 2056, 1032, 5, 40), (1100, 512, 513, 12, 64), (140, 8, 16, 1, 8), (131, 200, 72, 3, 200), (8500, 128, 200, 9, 48), (150, 64, 128, 2500, 8), (2050, 256, 384, 200, 8), (600, 4096, 136, 2, 256), (5000, 64, 96, 3, 16), (400, 1024, 2048, 2, 128), (260, 3000, 1500, 1, 256),
+    (300, 512, 1030, 4, 24), (145, 64, 70, 2, 72)])
 @pytest.mark.parametrize("order", ["mixed", "runs"])
 def test_low_rank_add(cuda, t, k, n, count, rank, order):
     g = gen(t + k + n + rank)
