@@ -14,7 +14,7 @@
 //
 // Scales lie in memory as the format has them, [rows, in / 32] bytes.  The MMA reads them from tensor memory, four K steps in
 // a word, row r in lane r mod 32 of column r / 32: four warps fetch them as 16-byte pieces a row (four stages at a time, one
-// fetch ahead), write them into that order beside the stage, and tcgen05.cp takes them over, ordered before the MMAs that
+// fetch ahead; as words where rows do not start on 16 bytes), write them into that order beside the stage, and tcgen05.cp takes them over, ordered before the MMAs that
 // follow it.  A stage's slot in tensor memory is written again no sooner than its shared memory, whose release waits for the
 // MMAs that read both.  Rows and blocks past the end get the scale 1 and, from TMA, codes of zero.
 //
@@ -28,6 +28,7 @@
 // 2048 -> 8192, 7 us, of which 4 are a launch's and the ring's filling.  What a K step of 128 costs beside its MMAs bounds all that
 // is not large: 340 cycles for the warp that issues them, before it issued by predicates and looked ahead 600.
 #include <atomic>
+#include <type_traits>
 
 #include "tcgen05.cuh"
 #include "../../include/ironmlx_b200_testing.h"
@@ -91,7 +92,7 @@ struct MxArgs {
     int height;                         // rows of P in a tile (SWAP: 128 or fewer)
     int stage_bytes;                    // that the loads of a stage bring
     int y_map;                          // y leaves by TMA (rows that start on 16 bytes)
-    int piece_p, piece_q;               // bytes of scales that one load may fetch: 16, 4 or 1
+    int piece_p, piece_q;               // bytes on which the scales' rows start: 16 (and no row ends in a group), 4 or 1
     int spin_limit;
     int32_t* status;
 };
@@ -160,18 +161,58 @@ __device__ __forceinline__ int ld_cluster_int(uint32_t addr, uint32_t rank) {
     return v;
 }
 
-// Scales of a row for the four K steps of a group (16 blocks), 1 (127) past the end.
-__device__ __forceinline__ uint4 row_scales(const uint8_t* row, int group, int blocks, int piece) {
-    const int b0 = group * 16;
-    if (piece == 16) return __ldg(reinterpret_cast<const uint4*>(row + b0));
+// Scales of a row for the four K steps of a group (16 blocks), in the words that they lie in: what is loaded is not touched until
+// finish_scales, a group later.  (8192 rows, 2080 -> 8192, whose rows of scales start anywhere: 140 us, byte by byte 252.)
+struct RowScales {
+    uint32_t w[5];
+};
+// ALL16: every row's groups are 16-byte pieces (the other ways beside this one cost it 5%).
+template <bool ALL16>
+__device__ __forceinline__ RowScales load_scales(const uint8_t* row, int group, int blocks, int piece, const uint8_t* first, const uint8_t* last) {
+    RowScales s;
+    const uint8_t* p = row + group * 16;
+    if (ALL16 || piece == 16) {
+        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+        s.w[0] = v.x;
+        s.w[1] = v.y;
+        s.w[2] = v.z;
+        s.w[3] = v.w;
+        s.w[4] = 0;
+        return s;
+    }
+    if (piece == 4) {                         // (whole words then, up to the end of the row)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s.w[i] = group * 16 + 4 * i < blocks ? __ldg(reinterpret_cast<const uint32_t*>(p) + i) : 0x7f7f7f7fu;
+        s.w[4] = 0;
+        return s;
+    }
+    const uint8_t* word = reinterpret_cast<const uint8_t*>((uintptr_t)p & ~(uintptr_t)3);
+    const uint8_t* end = p + min(16, blocks - group * 16);
+#pragma unroll
+    for (int i = 0; i < 5; ++i, word += 4) {
+        s.w[i] = 0;
+        if (word >= end) continue;
+        if (word >= first && word + 4 <= last) {
+            s.w[i] = __ldg(reinterpret_cast<const uint32_t*>(word));
+        } else {                              // the array's first or last word, not all of which is its own
+            for (int j = 0; j < 4; ++j)
+                if (word + j >= first && word + j < last) s.w[i] |= (uint32_t)__ldg(word + j) << (8 * j);
+        }
+    }
+    return s;
+}
+// ... 1 (127) past the end of the row.
+template <bool ALL16>
+__device__ __forceinline__ uint4 finish_scales(const RowScales& s, const uint8_t* row, int group, int blocks, int piece) {
+    if (ALL16 || piece != 1) return make_uint4(s.w[0], s.w[1], s.w[2], s.w[3]);
+    const int n = blocks - group * 16, shift = (int)((uintptr_t)row & 3) * 8;
     uint32_t v[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const int b = b0 + 4 * i;
-        v[i] = 0x7f7f7f7fu;
-        if (b + 4 <= blocks && piece == 4) v[i] = __ldg(reinterpret_cast<const uint32_t*>(row + b));
-        else
-            for (int j = 0; j < 4 && b + j < blocks; ++j) v[i] = (v[i] & ~(255u << (8 * j))) | ((uint32_t)__ldg(row + b + j) << (8 * j));
+        v[i] = __funnelshift_r(s.w[i], s.w[i + 1], shift);
+        const int keep = n - 4 * i;
+        const uint32_t own = keep >= 4 ? 0xffffffffu : (keep <= 0 ? 0u : (1u << (8 * keep)) - 1u);
+        v[i] = (v[i] & own) | (0x7f7f7f7fu & ~own);
     }
     return make_uint4(v[0], v[1], v[2], v[3]);
 }
@@ -380,56 +421,64 @@ mxfp8_mm_kernel(const MxArgs a, const int lg_splits, const __grid_constant__ MxM
                 row[1 + h] = r < NT && q0 + r < a.q_rows ? a.qs + (size_t)(q0 + r) * blocks : nullptr;
             }
         };
-        auto fetch = [&](int i, uint4 (&v)[1 + P::kQParts]) {
-#pragma unroll
-            for (int j = 0; j < 1 + P::kQParts; ++j)
-                v[j] = row[j] != nullptr ? row_scales(row[j], g0 + i, blocks, j == 0 ? a.piece_p : a.piece_q) : make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
-        };
-        auto prefetch = [&](int from) {
-            for (int b = from; b < min(k1 * 4, blocks); b += 32)
+        auto bring = [&](auto all16) {
+            constexpr bool ALL16 = decltype(all16)::value;
+            const uint8_t *p_end = a.ps + (size_t)a.p_rows * blocks, *q_end = a.qs + (size_t)a.q_rows * blocks;
+            RowScales next[1 + P::kQParts];
+            auto fetch = [&](int i) {
 #pragma unroll
                 for (int j = 0; j < 1 + P::kQParts; ++j)
-                    if (row[j] != nullptr) asm volatile("prefetch.global.L2 [%0];" ::"l"(row[j] + b));
-        };
-        uint4 v[1 + P::kQParts], next[1 + P::kQParts];
-        rows_of(first);
-        fetch(0, next);
-        prefetch(g0 * 16 + 32);
-        int g = 0;
-        uint32_t g_ph = 0;
-        bool ok = true;
-        for (int t = first; t < a.tiles && ok; t += stride) {
-            for (int i = 0; i < groups; ++i) {
+                    if (row[j] != nullptr) next[j] = load_scales<ALL16>(row[j], g0 + i, blocks, j == 0 ? a.piece_p : a.piece_q, j == 0 ? a.ps : a.qs, j == 0 ? p_end : q_end);
+            };
+            auto prefetch = [&](int from) {
+                for (int b = from; b < min(k1 * 4, blocks); b += 32)
 #pragma unroll
-                for (int j = 0; j < 1 + P::kQParts; ++j) v[j] = next[j];
-                if (i + 1 < groups) {
-                    fetch(i + 1, next);
-                } else if (t + stride < a.tiles) {
-                    rows_of(t + stride);
-                    fetch(0, next);
-                    prefetch(g0 * 16 + 32);
-                }
-                if (!mbar_wait(smem_u32(&bars.used[g]), g_ph ^ 1u, abort_flag, spin)) {
-                    ok = false;
-                    break;
-                }
+                    for (int j = 0; j < 1 + P::kQParts; ++j)
+                        if (row[j] != nullptr) asm volatile("prefetch.global.L2 [%0];" ::"l"(row[j] + b));
+            };
+            uint4 v[1 + P::kQParts];
+            rows_of(first);
+            fetch(0);
+            prefetch(g0 * 16 + 32);
+            int g = 0;
+            uint32_t g_ph = 0;
+            bool ok = true;
+            for (int t = first; t < a.tiles && ok; t += stride) {
+                for (int i = 0; i < groups; ++i) {
 #pragma unroll
-                for (int j = 0; j < 1 + P::kQParts; ++j) {
-                    const uint32_t to = at + (uint32_t)(g * P::kGroup + j * 512);
-                    st_shared(to, v[j].x);
-                    st_shared(to + P::kSf, v[j].y);
-                    st_shared(to + 2 * P::kSf, v[j].z);
-                    st_shared(to + 3 * P::kSf, v[j].w);
-                }
-                fence_async_proxy();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(smem_u32(&bars.scales[g]));
-                if (++g == kMxGroups) {
-                    g = 0;
-                    g_ph ^= 1u;
+                    for (int j = 0; j < 1 + P::kQParts; ++j)
+                        v[j] = row[j] != nullptr ? finish_scales<ALL16>(next[j], row[j], g0 + i, blocks, j == 0 ? a.piece_p : a.piece_q) : make_uint4(0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu);
+                    if (i + 1 < groups) {
+                        fetch(i + 1);
+                    } else if (t + stride < a.tiles) {
+                        rows_of(t + stride);
+                        fetch(0);
+                        prefetch(g0 * 16 + 32);
+                    }
+                    if (!mbar_wait(smem_u32(&bars.used[g]), g_ph ^ 1u, abort_flag, spin)) {
+                        ok = false;
+                        break;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 1 + P::kQParts; ++j) {
+                        const uint32_t to = at + (uint32_t)(g * P::kGroup + j * 512);
+                        st_shared(to, v[j].x);
+                        st_shared(to + P::kSf, v[j].y);
+                        st_shared(to + 2 * P::kSf, v[j].z);
+                        st_shared(to + 3 * P::kSf, v[j].w);
+                    }
+                    fence_async_proxy();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(smem_u32(&bars.scales[g]));
+                    if (++g == kMxGroups) {
+                        g = 0;
+                        g_ph ^= 1u;
+                    }
                 }
             }
-        }
+        };
+        if (a.piece_p == 16 && a.piece_q == 16) bring(std::true_type{});
+        else bring(std::false_type{});
     } else {
         const int l = warp * 32 + lane;                      // lane of the accumulator
         const uint32_t quarter = (uint32_t)(warp * 32) << 16;
