@@ -3,7 +3,7 @@
 // and a row whose id is outside [0, count) gets out[t] = y[t].
 //
 // One launch does both products.  A cluster of CTAs takes a unit, up to 16 (64) rows of one adapter: each CTA multiplies its
-// part of the input dimension, the cluster adds the parts through its shared memories, in rank order, and each CTA multiplies
+// part of the input dimension, the cluster adds the parts through its shared memories, in one order, and each CTA multiplies
 // its part of the output columns.  Sums are in fp32; for the second product the scaled low-rank row becomes two bf16 numbers,
 // hi + lo (16 bits: with one, its rounding would weigh as much as the output's), two MMAs for one.
 // Which rows make up a unit every CTA finds out by itself from the ids: the units of an adapter are its rows in batch order,
@@ -17,7 +17,7 @@
 //   many rows: tiles of 64 rows by tcgen05.mma, x and y gathered by cp.async, a and b brought by TMA.  8192 rows of rank 64,
 //     2048 -> 8192, take 71 us, 318 MB at 4.5 TB/s: y comes and leaves at 6.2 TB/s, close to the copy bandwidth, but the ids
 //     (5 us), x . a^T (7 us) and the cluster's exchange (5 us) come before it, for all CTAs at the same time.  With mma.sync by
-//     the warps that copy it was 113 us; rank 128 takes 110 us (229).  777 rows of rank 16 take 17 us, each phase a latency or two.
+//     the warps that copy it was 113 us; rank 128 takes 93 us (229).  777 rows of rank 16 take 16 us, each phase a latency or two.
 #include <atomic>
 
 #include "tcgen05.cuh"

@@ -14,14 +14,16 @@
 //
 // Scales lie in memory as the format has them, [rows, in / 32] bytes.  The MMA reads them from tensor memory, four K steps in
 // a word, row r in lane r mod 32 of column r / 32: four warps fetch them as 16-byte pieces a row (four stages at a time, one
-// fetch ahead; as words where rows do not start on 16 bytes), write them into that order beside the stage, and tcgen05.cp takes them over, ordered before the MMAs that
-// follow it.  A stage's slot in tensor memory is written again no sooner than its shared memory, whose release waits for the
-// MMAs that read both.  Rows and blocks past the end get the scale 1 and, from TMA, codes of zero.
+// fetch ahead; as words where rows do not start on 16 bytes), write them into that order beside the stage, and tcgen05.cp takes
+// them over, ordered before the MMAs that follow it.  A stage's slot in tensor memory is written again no sooner than its shared
+// memory, whose release waits for the MMAs that read both.  Rows and blocks past the end get the scale 1 and, from TMA, codes of
+// zero.
 //
 // Eleven warps: 0..3 epilogue, 4..7 scales, 8 MMA and tensor memory, 9 loads, 10 (of a pair) tells CTA 0, whose warp 8 issues
-// the MMAs of both, what has arrived in its own.  Two accumulators alternate, so that the next tile's MMAs run beside the epilogue; 2 x 256 columns leave no room for the scales: at NT = 256 the two share 60 columns,
-// which the epilogue takes out first.  Every wait is bounded; on expiry what is in flight is waited for, tensor memory is
-// freed, the status word is set and the tiles concerned are NaN.
+// the MMAs of both, what has arrived in its own.  Two accumulators alternate, so that the next tile's MMAs run beside the
+// epilogue; 2 x 256 columns leave no room for the scales: at NT = 256 the two share 60 columns, which the epilogue takes out
+// first.  Every wait is bounded; on expiry what is in flight is waited for, tensor memory is freed, the status word is set and
+// the tiles concerned are NaN.
 //
 // On a B200, the kernel alone: 8192 rows, 2048 -> 8192, 102 us, 2.7 PFLOP/s, 81% of twice cuBLAS' bf16 rate (in a loop of
 // seconds the power limit makes it 122 to 125 us); 777 rows, 4096 -> 2048, 12.2 us; 64 rows, 2048 -> 152064, 55 us, 6.2 TB/s; one row,
