@@ -142,6 +142,23 @@ def test_adapters_on_streams(cuda):
     assert ops.low_rank_add(p["y"][:0], p["x"][:0], p["a"], p["b"], ip[:0]).shape == (0, 512)
 
 
+def test_adapters_beside_products(cuda):
+    """Tiles of adapters (two CTAs an SM, 128 columns of tensor memory each) and pairs of the product (all 512) on two streams at
+    the same time: the values of the calls alone."""
+    g = gen(77)
+    p = make(g, 700, 1024, 2048, 5, 16)
+    ids = torch.randint(-1, 5, (700,), generator=g, device="cuda", dtype=torch.int32)
+    rows = ops.quantize(torch.randn(700, 2048, generator=g, device="cuda"), mode="mxfp8")[:2]
+    w = ops.quantize(torch.randn(1024, 2048, generator=g, device="cuda"), mode="mxfp8")[:2]
+    alone = run(p, ids), ops.mxfp8_matmul(rows, *w)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [(run(p, ids, stream=streams[i & 1]), ops.mxfp8_matmul(rows, *w, stream=streams[1 - (i & 1)])) for i in range(40)]
+    torch.cuda.synchronize()
+    ops.check_status()
+    assert all(torch.equal(x, alone[0]) and torch.equal(y, alone[1]) for x, y in got)
+
+
 @pytest.mark.parametrize("kind", ["dense", "affine", "mxfp8"])
 def test_projection_with_adapters(cuda, kind):
     g = gen(21)
