@@ -4,8 +4,8 @@
 //
 // One launch does both products.  A cluster of CTAs takes a unit, up to 16 (64) rows of one adapter: each CTA multiplies its
 // part of the input dimension, the cluster adds the parts through its shared memories, in one order, and each CTA multiplies
-// its part of the output columns.  Sums are in fp32; for the second product the scaled low-rank row becomes two bf16 numbers,
-// hi + lo (16 bits: with one, its rounding would weigh as much as the output's), two MMAs for one.
+// its part of the output columns.  Sums are in fp32; for the second product the scaled low-rank row becomes three bf16 numbers
+// that add up to it exactly (8 bits each of its 24), three MMAs for one.
 // Which rows make up a unit every CTA finds out by itself from the ids: the units of an adapter are its rows in batch order,
 // so that the result does not depend on who runs when.  Rows without an adapter are units of their own that are copied.
 //
@@ -74,13 +74,17 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// v = hi + lo to 16 bits (what is not finite stays in hi)
-__device__ __forceinline__ void split2(float v, __nv_bfloat16& hi, __nv_bfloat16& lo) {
-    hi = __float2bfloat16_rn(v);
-    const float h = __bfloat162float(hi);
-    lo = __float2bfloat16_rn(isfinite(h) ? v - h : 0.f);
+// v = hi + mid + lo (parts 0, 1, 2), each the next 8 of its 24 bits: bf16 numbers in the upper halves of 32 bits.  (Cut off, not
+// rounded: hi is finite where v is; what is not finite stays in hi.)
+__device__ __forceinline__ uint32_t upper(float v) { return __float_as_uint(v) & 0xffff0000u; }
+__device__ __forceinline__ void split3(float v, uint32_t (&part)[3]) {
+    const bool finite = fabsf(v) < INFINITY;
+    part[0] = finite ? upper(v) : __float_as_uint(v) | (v == v ? 0u : 0x400000u);
+    const float left = finite ? v - __uint_as_float(part[0]) : 0.f;
+    part[1] = upper(left);
+    part[2] = __float_as_uint(left - __uint_as_float(part[1]));
 }
-__device__ __forceinline__ uint32_t pack2(__nv_bfloat16 a, __nv_bfloat16 b) { return (uint32_t)__bfloat16_as_ushort(a) | (uint32_t)__bfloat16_as_ushort(b) << 16; }
+__device__ __forceinline__ uint32_t pack2(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }       // two upper halves
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
     const int n = there ? 16 : 0;             // the rest is filled with zeros
@@ -114,22 +118,22 @@ constexpr int kFewUnit = 16;
 // is room for two or three pieces on their way (2.6 TB/s).  RB: blocks of 32 values of the rank, 1, 2, 4 or 8.
 __host__ __device__ constexpr int ring_pieces(int rb) { return rb == 8 ? 18 : (rb == 4 ? 15 : 12); }
 // Dynamic shared memory: the rings, this CTA's sums [row][rank], and in one place the warps' parts of them, [k part][row][rank]
-// (8 parts of ranks up to 32, 4 up to 64, 2 up to 128), and afterwards the low-rank rows as hi and lo.
+// (8 parts of ranks up to 32, 4 up to 64, 2 up to 128), and afterwards the low-rank rows as hi, mid and lo: [part][row][rb * 32],
+// in odd rows the pieces of 64 bytes that make up 128 the other way round, so that lanes that read together are in different
+// banks (a padded row would leave no room for two CTAs of a rank of 256).
 struct FewPlan {
-    int pitch, sums_at, part_at, lo_at, bytes;       // pitch: values of a row of hi or lo
+    int sums_at, part_at, bytes;
     __host__ __device__ FewPlan(int rank, int rb) {
-        pitch = rb * 32 + 32;                        // (lanes that read together are in different banks)
         sums_at = kThreads * ring_pieces(rb) * 16;
         part_at = sums_at + kFewUnit * rank * 4;
-        lo_at = part_at + kFewUnit * pitch * 2;
-        const int parts = 8 / rb, a = parts > 1 ? parts * kFewUnit * rank * 4 : 0, b = 2 * kFewUnit * pitch * 2;
+        const int parts = 8 / rb, a = parts > 1 ? parts * kFewUnit * rank * 4 : 0, b = 3 * kFewUnit * rb * 32 * 2;
         bytes = part_at + (a > b ? a : b);
     }
 };
 
 struct FewShared {
     int32_t ids[kFewRows];
-    int32_t same[kFewRows];                   // rows before with the same id
+    uint8_t same[kFewRows];                   // rows before with the same id
     uint32_t leads[kFewRows / 32];            // rows that lead a unit, a bit each
     int32_t rows[kFewUnit];
 };
@@ -155,7 +159,7 @@ __device__ __forceinline__ int find_unit(const LowRankArgs& p, FewShared& s, int
         same += __popc(alike & ((1u << lane) - 1u));
         const unsigned leads = __ballot_sync(0xffffffffu, i < p.n && same % kFewUnit == 0);
         if (lane == 0) s.leads[i >> 5] = leads;
-        s.same[i] = same;
+        s.same[i] = (uint8_t)same;
     }
     __syncthreads();
     int leader = -1, here = unit;
@@ -209,8 +213,7 @@ low_rank_few_kernel(const LowRankArgs p, const int ctas, const int clusters) {
     const FewPlan pl(rank, RB);
     float* sums = reinterpret_cast<float*>(dyn + pl.sums_at);
     float* parts = reinterpret_cast<float*>(dyn + pl.part_at);
-    __nv_bfloat16* hi = reinterpret_cast<__nv_bfloat16*>(dyn + pl.part_at);
-    __nv_bfloat16* lo = reinterpret_cast<__nv_bfloat16*>(dyn + pl.lo_at);
+    __nv_bfloat16* low_rows = reinterpret_cast<__nv_bfloat16*>(dyn + pl.part_at);
     const uint32_t own = smem_addr(dyn) + (uint32_t)tid * 16u;
     const __nv_bfloat16* a = p.a + (size_t)id * rank * p.in;
     const __nv_bfloat16* b = p.b + (size_t)id * p.n_out * rank;
@@ -338,26 +341,27 @@ low_rank_few_kernel(const LowRankArgs p, const int ctas, const int clusters) {
             }
             v *= sc;
         }
-        split2(v, hi[r * pl.pitch + k], lo[r * pl.pitch + k]);
+        uint32_t part[3];
+        split3(v, part);
+#pragma unroll
+        for (int h = 0; h < 3; ++h) low_rows[(h * kFewUnit + r) * RB * 32 + (RB > 1 ? k ^ ((r & 1) * 32) : k)] = __ushort_as_bfloat16((unsigned short)(part[h] >> 16));
     }
     if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");     // this CTA has read the others' sums
     __syncthreads();
 
     // + t . b^T
-    const uint4* h0 = reinterpret_cast<const uint4*>(hi + g * pl.pitch + q * 8);
-    const uint4* h1 = reinterpret_cast<const uint4*>(hi + (g + 8) * pl.pitch + q * 8);
-    const uint4* l0 = reinterpret_cast<const uint4*>(lo + g * pl.pitch + q * 8);
-    const uint4* l1 = reinterpret_cast<const uint4*>(lo + (g + 8) * pl.pitch + q * 8);
+    const uint4* low_even = reinterpret_cast<const uint4*>(low_rows) + g * RB * 4 + (RB > 1 ? (g & 1) * 4 : 0) + q;     // of even blocks, odd ones
+    const uint4* low_odd = low_even - (g & 1) * 8;
+    auto low_at = [&](int kb, int h, int r) { return (kb & 1 ? low_odd : low_even)[(h * kFewUnit + r * 8) * RB * 4 + kb * 4]; };     // hi, mid, lo; rows g and g + 8
     // up to a rank of 128 the low-rank rows stay in registers (read for every tile they cost a rank of 128 half of its time)
     constexpr int kKept = RB <= 4 ? RB : 1;
-    uint4 vh0[kKept], vh1[kKept], vl0[kKept], vl1[kKept];
+    uint4 low[kKept][3][2];
 #pragma unroll
-    for (int kb = 0; kb < kKept; ++kb) {
-        vh0[kb] = h0[kb * 4];
-        vh1[kb] = h1[kb * 4];
-        vl0[kb] = l0[kb * 4];
-        vl1[kb] = l1[kb * 4];
-    }
+    for (int kb = 0; kb < kKept; ++kb)
+#pragma unroll
+        for (int h = 0; h < 3; ++h)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) low[kb][h][r] = low_at(kb, h, r);
     size_t at0 = (size_t)row0 * p.n_out + (t0 + warp) * 8 + 2 * q, at1 = (size_t)row1 * p.n_out + (t0 + warp) * 8 + 2 * q;
     int out_col = (t0 + warp) * 8 + 2 * q;
     uint32_t from = own;
@@ -379,17 +383,20 @@ low_rank_few_kernel(const LowRankArgs p, const int ctas, const int clusters) {
             const uint4 w = ld_shared16(from + (1 + kb) * kPiece);
             const int i0 = kKept == RB ? kb : 0;
             if (kKept != RB) {
-                vh0[0] = h0[kb * 4];
-                vl0[0] = l0[kb * 4];
-                if (more) {
-                    vh1[0] = h1[kb * 4];
-                    vl1[0] = l1[kb * 4];
+#pragma unroll
+                for (int h = 0; h < 3; ++h) {
+                    low[0][h][0] = low_at(kb, h, 0);
+                    if (more) low[0][h][1] = low_at(kb, h, 1);
                 }
             }
-            mma(d, vh0[i0].x, vh1[i0].x, vh0[i0].y, vh1[i0].y, w.x, w.y);
-            mma(e, vl0[i0].x, vl1[i0].x, vl0[i0].y, vl1[i0].y, w.x, w.y);
-            mma(d, vh0[i0].z, vh1[i0].z, vh0[i0].w, vh1[i0].w, w.z, w.w);
-            mma(e, vl0[i0].z, vl1[i0].z, vl0[i0].w, vl1[i0].w, w.z, w.w);
+            // (the small parts in sums of their own)
+#pragma unroll
+            for (int h = 2; h >= 0; --h) {
+                float(&to)[4] = h == 0 ? d : e;
+                const uint4 v0 = low[i0][h][0], v1 = low[i0][h][1];
+                mma(to, v0.x, v1.x, v0.y, v1.y, w.x, w.y);
+                mma(to, v0.z, v1.z, v0.w, v1.w, w.z, w.w);
+            }
         }
         if (out_col < p.n_out) {
             if (has0) write(at0, yv.x, d[0] + e[0], d[1] + e[1]);
@@ -451,17 +458,18 @@ struct TileMaps {
 // product was; beyond 128 they take the stages' place.
 struct TilePlan {
     int r16, blocks;                          // rank rounded up to 16; blocks of 64 of it
-    int stages, stage, sums_at, hi_at, lo_at, bytes;
+    int stages, stage, sums_at, low_at, low_pitch, bytes;  // low_at: the low-rank rows, fp32, low_pitch values apart (no bank twice)
     __host__ __device__ TilePlan(int rank, int nj) {
         r16 = (rank + 15) & ~15;
         blocks = (r16 + 63) / 64;
         stages = nj <= 4 ? 5 : 3;
         const int first = kBlock + r16 * 128, second = blocks * kBlock + kTileRows * 128;
         stage = ((first > second ? first : second) + 1023) & ~1023;
-        hi_at = stages * stage;
-        lo_at = hi_at + blocks * kBlock;
-        sums_at = nj == 4 ? lo_at + blocks * kBlock : 0;
-        bytes = lo_at + blocks * kBlock + (nj == 4 ? kTileRows * r16 * 4 : 0);
+        low_at = stages * stage;
+        low_pitch = r16 + 4;
+        const int end = low_at + kTileRows * low_pitch * 4;
+        sums_at = nj == 4 ? end : 0;
+        bytes = end + (nj == 4 ? kTileRows * r16 * 4 : 0);
     }
 };
 
@@ -506,7 +514,8 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
     const int unit = (int)blockIdx.x >> cut, c = (int)blockIdx.x & (ctas - 1);
     // First of all the tensor memory: an SM starts its second CTA only when the first has given up the permit to allocate (with
     // the allocation behind the ids half of the CTAs of 8192 rows started 6.7 us late, of 777 rows 3.2).
-    constexpr uint32_t kTmem = NJ == 8 ? 256 : 128;        // the first product's sums, in their place two of a stage of the second
+    // The first product's sums; in their place two stages' of the second, and from column 128 on its A, see below.
+    constexpr uint32_t kTmem = NJ <= 4 ? 256 : 512, kLowAt = 128, kLowCols = 16 * NJ;
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&s.tmem_base)), "r"(kTmem) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -721,8 +730,9 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
         else __syncthreads();
         if (ctas > 1) cluster_sync();
         else __syncthreads();
-        const uint64_t hi_desc = tc::smem_desc(base + (uint32_t)pl.hi_at), lo_desc = tc::smem_desc(base + (uint32_t)pl.lo_at);
-        const uint32_t idesc = tc::idesc_for(64, kCols) | (1u << 7) | (1u << 10);
+        asm volatile("bar.sync 1, %0;" ::"n"(kThreads + 32) : "memory");   // ... and in tensor memory
+        tc::tc_fence_after();
+        const uint32_t idesc = tc::idesc_for(128, kCols) | (1u << 7) | (1u << 10);
         const int kks = r16 / 16;
         for (int e = 0; e < total - n_in; ++e) {
             tc::mbar_wait_on(tc::smem_u32(&s.loaded[slot]), ph, flag, p.spin_limit);
@@ -731,13 +741,12 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
             const uint32_t d = tmem + (uint32_t)((e & 1) * 64);
             const uint64_t b_desc = tc::smem_desc(base + (uint32_t)(slot * pl.stage + kBlock));
 #pragma unroll
-            for (int part = 0; part < 2; ++part)
+            for (int part = 1; part >= 0; --part)          // (the small ones first)
 #pragma unroll
                 for (int kk = 0; kk < 2 * NJ; ++kk)
-                    if (kk < kks) {
-                        const uint64_t at = (uint64_t)((kk >> 2) * (kBlock >> 4) + 2 * (kk & 3));
-                        tc::umma_ss_if(me, d, (part ? lo_desc : hi_desc) + at, b_desc + at, idesc, part > 0 || kk > 0 ? 1u : 0u);
-                    }
+                    if (kk < kks)
+                        tc::umma_ts_if(me, d, tmem + kLowAt + (uint32_t)(part * kLowCols + kk * 8),
+                                       b_desc + (uint64_t)((kk >> 2) * (kBlock >> 4) + 2 * (kk & 3)), idesc, part == 0 || kk > 0 ? 1u : 0u);
             tc::umma_commit_if<false>(me, tc::smem_u32(&s.used[slot]));
             tc::umma_commit_if<false>(me, tc::smem_u32(&s.sums_there[e & 1]));
             __syncwarp();
@@ -807,7 +816,7 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
             if (i > 0) wait(s.used[(i - 1) % S], (i - 1) / S);             // the place of the next copy is free
             copy(early);
         }
-        // the low-rank rows: this CTA's part of the sums, then all of them as hi + lo in every CTA
+        // the low-rank rows: this CTA's part of the sums, then all of them in every CTA
         auto sums_of = [&](int cta) {         // their place in a CTA
             return NJ <= 2 ? (((int)((long)ik * (cta + 1) >> shift) - (int)((long)ik * cta >> shift) + S - 1) % S) * pl.stage : pl.sums_at;
         };
@@ -848,19 +857,47 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] += __shfl_xor_sync(0xffffffffu, v[e], d);
             if (!mine) continue;
-            __nv_bfloat16 hi[8], lo[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) split2(j * 8 < rank ? v[e] * sc : 0.f, hi[e], lo[e]);      // (past the rank: another adapter's)
-            const uint4 vh = make_uint4(pack2(hi[0], hi[1]), pack2(hi[2], hi[3]), pack2(hi[4], hi[5]), pack2(hi[6], hi[7]));
-            const uint4 vl = make_uint4(pack2(lo[0], lo[1]), pack2(lo[2], lo[3]), pack2(lo[4], lo[5]), pack2(lo[6], lo[7]));
-            const uint32_t dst0 = base + (uint32_t)((j >> 3) * kBlock + r * 128 + (((j & 7) ^ (r & 7)) * 16));
-            const uint32_t dst = ctas > 1 ? peer_addr(dst0, peer) : dst0;
-            st_peer4(dst + pl.hi_at, vh);
-            st_peer4(dst + pl.lo_at, vl);
+            for (int e = 0; e < 8; ++e) v[e] = j * 8 < rank ? v[e] * sc : 0.f;                     // (past the rank: another adapter's)
+            const uint32_t at = base + (uint32_t)(pl.low_at + (r * pl.low_pitch + j * 8) * 4), dst = ctas > 1 ? peer_addr(at, peer) : at;
+            st_peer4(dst, make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3])));
+            st_peer4(dst + 16, make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7])));
         }
-        asm volatile("fence.proxy.async.shared::cluster;" ::: "memory");   // (what it wrote is read by MMAs, here and in the other CTAs)
+        asm volatile("fence.proxy.async.shared::cluster;" ::: "memory");   // (TMA writes where the sums were)
         if (ctas > 1) cluster_sync();
         else __syncthreads();
+        // The second product's A is the same in every stage and lies in tensor memory, so that its MMAs read b alone from shared
+        // memory, whose bandwidth the copies of y need (a call on 8192 rows of rank 64: 78.4 us, with A there, too, 86 to 91): hi
+        // and mid of a warp's 16 rows in its 32 lanes, and in columns behind them lo and zeros.
+        {
+            const float* row = reinterpret_cast<const float*>(smem + pl.low_at) + (rt * 16 + (lane & 15)) * pl.low_pitch;
+#pragma unroll 1
+            for (int jb = 0; jb < NJ; ++jb) {
+                uint32_t cols[16] = {};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int k = jb * 32 + i * 4;
+                    if (k >= r16) break;
+                    const float4 f = *reinterpret_cast<const float4*>(row + k);
+                    uint32_t p0[3], p1[3], p2[3], p3[3];
+                    split3(f.x, p0);
+                    split3(f.y, p1);
+                    split3(f.z, p2);
+                    split3(f.w, p3);
+                    if (half == 0) {
+                        cols[2 * i] = lane < 16 ? pack2(p0[0], p1[0]) : pack2(p0[1], p1[1]);
+                        cols[2 * i + 1] = lane < 16 ? pack2(p2[0], p3[0]) : pack2(p2[1], p3[1]);
+                    } else if (lane < 16) {
+                        cols[2 * i] = pack2(p0[2], p1[2]);
+                        cols[2 * i + 1] = pack2(p2[2], p3[2]);
+                    }
+                }
+                tc::tmem_st16(tmem + ((uint32_t)(rt * 32) << 16) + kLowAt + (uint32_t)(half * (int)kLowCols + jb * 16), cols);
+            }
+            tc::tmem_st_wait();
+            tc::tc_fence_before();
+            asm volatile("bar.arrive 1, %0;" ::"n"(kThreads + 32) : "memory");
+        }
         if (NJ > 4)
             for (int i = 0; i < S - 1; ++i) copy(total);
         int n = n0 * kCols;                                // first column of the stage
@@ -884,8 +921,10 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
         for (int e = 0; e < total - n_in; ++e) {
             wait(s.sums_there[e & 1], e >> 1);
             tc::tc_fence_after();
-            uint32_t u[16], v[2][4];
-            tmem_ld_16x32(tmem + ((uint32_t)(rt * 32) << 16) + (uint32_t)((e & 1) * 64 + half * 32), u);
+            uint32_t u[16], u_mid[16], v[2][4];
+            const uint32_t sums_at = tmem + ((uint32_t)(rt * 32) << 16) + (uint32_t)((e & 1) * 64 + half * 32);
+            tmem_ld_16x32(sums_at, u);
+            tmem_ld_16x32(sums_at + (16u << 16), u_mid);
             arrived();
             __syncwarp();
             if (WIDE) {
@@ -893,12 +932,13 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
                 for (int h = 0; h < 2; ++h) ld_matrices(y + frag_at + h * 1024, v[h]);
             }
             tmem_wait(u);
+            tmem_wait(u_mid);
             tc::tc_fence_before();
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(tc::smem_u32(&s.sums_free[e & 1]));
             float d[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) d[i] = __uint_as_float(u[i]);
+            for (int i = 0; i < 16; ++i) d[i] = __uint_as_float(u[i]) + __uint_as_float(u_mid[i]);
             if (WIDE) {
                 // added in y's place, which is read and written as 8 x 8 matrices (the sums' layout), out in 16-byte pieces
 #pragma unroll

@@ -170,6 +170,16 @@ __device__ __forceinline__ void umma_ss_if(uint32_t me, uint32_t tmem_d, uint64_
         ::"r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate), "r"(0u), "r"(me)
         : "memory");
 }
+// ... A from tensor memory.
+__device__ __forceinline__ void umma_ts_if(uint32_t me, uint32_t tmem_d, uint32_t tmem_a, uint64_t db, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "setp.ne.b32 q, %6, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "l"(db), "r"(idesc), "r"(accumulate), "r"(0u), "r"(me)
+        : "memory");
+}
 template <bool PAIR>
 __device__ __forceinline__ void umma_commit_if(uint32_t me, uint32_t bar) {
     if (PAIR)

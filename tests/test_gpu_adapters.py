@@ -57,6 +57,27 @@ def test_low_rank_add(cuda, t, k, n, count, rank, order):
     assert ops.low_rank_add(y, p["x"], p["a"], p["b"], ids, p["scale"], out=y) is y and torch.equal(y, out)
 
 
+@pytest.mark.parametrize("t,n,count,rank", [(1, 96, 1, 16), (5, 100, 2, 8), (40, 264, 3, 64), (20, 41, 2, 128), (20, 72, 2, 200), (100, 128, 9, 256),
+                                            (300, 136, 2, 16), (300, 264, 2, 64), (200, 136, 1, 128), (200, 72, 1, 256), (300, 77, 2, 24)])
+def test_whole_numbers_of_24_bits_are_exact(cuda, t, n, count, rank):
+    """Low-rank rows of up to 21 bits, and a y that takes the first eight bits of what is added to it: every sum is a whole
+    number below 2^24, exact in fp32 in any order, so that every output is the one rounding of its sum.  (A low-rank row of 16
+    bits leaves a few units of 2^19, next to outputs whose step is 8 and less.)"""
+    g = gen(t + n + rank)
+
+    def whole(lo, hi, *shape):
+        return torch.randint(lo, hi, shape, generator=g, device="cuda")
+
+    p = dict(x=whole(0, 65, t, 512).bfloat16(), a=whole(0, 65, count, rank, 512).bfloat16(), scale=None,
+             b=((whole(0, rank, count, n, rank) < 4) * (2 * whole(0, 2, count, n, rank) - 1)).bfloat16())
+    ids = whole(0, count, t).int()
+    rows = torch.einsum("tk,trk->tr", p["x"].double(), p["a"].double()[ids.long()])
+    add = torch.einsum("tr,tnr->tn", rows, p["b"].double()[ids.long()])
+    p["y"] = -add.bfloat16()
+    assert rows.max() > 2 ** 18 and torch.einsum("tr,tnr->tn", rows, p["b"].double().abs()[ids.long()]).max() < 2 ** 24
+    assert torch.equal(run(p, ids), (p["y"].double() + add).float().bfloat16())
+
+
 @pytest.mark.parametrize("t", [3, 70, 700])
 def test_ids_without_an_adapter(cuda, t):
     """No row has one; ids far outside; every row the last adapter.  What a row without an adapter holds is left bit for bit,
