@@ -35,7 +35,8 @@ extern "C"
 #endif
 __attribute__((visibility("default"))) void imx_testing_prefill_give_up(int on);
 
-/* The same for imx_mxfp8_matmul: its outputs are NaN, status 4 is recorded. */
+/* The same for imx_mxfp8_matmul: its outputs are NaN, status 4 is recorded.  on = 1: all CTAs; 2 + r: where clusters cut the
+ * reduction CTA r of each alone, which makes all outputs of its cluster NaN. */
 #ifdef __cplusplus
 extern "C"
 #endif

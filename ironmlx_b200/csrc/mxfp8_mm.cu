@@ -48,7 +48,7 @@ constexpr int kMxMaxStages = 10;
 constexpr int kMxGroups = 2;                       // groups of four K steps whose scales are in shared memory
 constexpr int kMxMaxSplits = 8;                    // CTAs of a cluster that cut the K range of a tile
 constexpr int kMxMostRows = 0x7fffff00;            // of either operand: a tile that starts below ends within 31 bits
-std::atomic<int> g_mx_spin_limit{kSpin};
+std::atomic<int> g_mx_give_up{0};                  // see imx_testing_mxfp8_give_up
 
 template <int NT, bool SWAP, bool PAIR>
 struct Plan {
@@ -82,6 +82,7 @@ struct MxBars {
     uint64_t retired;                   // after an expired wait: the MMAs issued before it
     uint32_t tmem_base;
     int abort;
+    int cluster_gave_up;                // K range cut: a CTA of the cluster has (set by that CTA, in all of them)
 };
 
 struct MxArgs {
@@ -96,6 +97,7 @@ struct MxArgs {
     int y_map;                          // y leaves by TMA (rows that start on 16 bytes)
     int piece_p, piece_q;               // bytes on which the scales' rows start: 16 (and no row ends in a group), 4 or 1
     int spin_limit;
+    int give_up;
     int32_t* status;
 };
 struct MxMaps {
@@ -154,6 +156,10 @@ __device__ __forceinline__ void copy_to_peer(uint32_t dst, uint32_t src, uint32_
         "cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [ra], [%1], %2, [rb];\n\t}"
         ::"r"(dst), "r"(src), "r"(bytes), "r"(bar), "r"(rank)
         : "memory");
+}
+// One word of CTA `rank`'s shared memory, at this CTA's offset of it.
+__device__ __forceinline__ void st_cluster_int(uint32_t addr, int v, uint32_t rank) {
+    asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %0, %2;\n\tst.shared::cluster.s32 [ra], %1;\n\t}" ::"r"(addr), "r"(v), "r"(rank) : "memory");
 }
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
@@ -248,7 +254,6 @@ mxfp8_mm_kernel(const MxArgs a, const int lg_splits, const __grid_constant__ MxM
     const uint32_t sbase = smem_u32(base), out_base = sbase + P::kStages * P::kTile, sf_base = out_base + P::kOut;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     volatile int* abort_flag = &bars.abort;
-    const int spin = a.spin_limit;
 
     // Warp 9 prepares the barriers, tells the others so and goes on to the loads, of which a full ring takes microseconds to
     // issue; it needs nothing of what the others prepare.
@@ -268,6 +273,7 @@ mxfp8_mm_kernel(const MxArgs a, const int lg_splits, const __grid_constant__ MxM
             mbar_init(smem_u32(&bars.sums), 1);
             mbar_init(smem_u32(&bars.retired), 1);
             bars.abort = 0;
+            bars.cluster_gave_up = 0;
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -292,6 +298,7 @@ mxfp8_mm_kernel(const MxArgs a, const int lg_splits, const __grid_constant__ MxM
 
     // a cluster a tile when the K range is cut, else every CTA (pair) takes every stride-th tile whole
     const int splits = 1 << lg_splits, rank = PAIR || (SWAP && lg_splits > 0) ? (int)cluster_ctarank() : 0;
+    const int spin = SWAP && a.give_up > 1 && a.give_up - 2 != rank ? kSpin : a.spin_limit;
     const int steps = (a.in + kMxK - 1) / kMxK, lg_cluster = PAIR ? 1 : lg_splits;
     const int k0 = PAIR ? 0 : (steps * rank) >> lg_splits, k1 = PAIR ? steps : (steps * (rank + 1)) >> lg_splits;
     const int first = (int)blockIdx.x >> lg_cluster, stride = (int)gridDim.x >> lg_cluster;
@@ -557,14 +564,15 @@ mxfp8_mm_kernel(const MxArgs a, const int lg_splits, const __grid_constant__ MxM
         }
         if (!SWAP && lane == 0) tma_store_done();
         if (SWAP && lg_splits > 0) {
-            // each CTA's columns to it, [sender][column][lane]; it adds them
+            // each CTA's columns to it, [sender][column][lane]; it adds them.  (All of them send, also a CTA that has given up, so
+            // that what a CTA waits for comes.)
             fence_async_proxy();
             asm volatile("bar.sync 1, 128;" ::: "memory");
             cluster_wait();
             met = true;
             if (warp == 0 && elect_one()) {
                 mbar_expect_tx(smem_u32(&bars.sums), (uint32_t)((sum_cols(rank) * 512) << lg_splits));
-                for (int r = 0; r < splits && done > 0 && *abort_flag == 0; ++r)
+                for (int r = 0; r < splits; ++r)
                     if (sum_cols(r) > 0)
                         copy_to_peer(out_base + (uint32_t)(rank << lg_own) * 512u, sbase + (uint32_t)(r << lg_own) * 512u, (uint32_t)sum_cols(r) * 512u,
                                      smem_u32(&bars.sums), (uint32_t)r);
@@ -615,9 +623,17 @@ mxfp8_mm_kernel(const MxArgs a, const int lg_splits, const __grid_constant__ MxM
     }
     if (SWAP && lg_splits > 0) {
         if (!met) cluster_wait();
-        // nobody leaves while another CTA may copy into its shared memory or out of it
-        asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+        if (gave_up && tid < splits) st_cluster_int(smem_u32(&bars.cluster_gave_up), 1, (uint32_t)tid);
+        // nobody leaves while another CTA may copy into its shared memory or out of it: all copies have been issued here, and a
+        // CTA that has waited for its sums has all that come to it
+        cluster_arrive();
         cluster_wait();
+        if (bars.cluster_gave_up != 0) {                     // (then some may not have waited; the same in all CTAs)
+            if (warp == 0) mbar_drain(smem_u32(&bars.sums), 0u);
+            cluster_arrive();
+            cluster_wait();
+            bad = true;
+        }
     }
     if (bad) {
         if (tid == 0) atomicExch(a.status, 4);
@@ -666,7 +682,8 @@ int launch(const Call& c, int lg_splits, int height = PAIR ? 256 : 128) {
     auto piece = [&](const uint8_t* s) { return (uintptr_t)s % 16 == 0 && c.in % 512 == 0 ? 16 : ((uintptr_t)s % 4 == 0 && c.in % 128 == 0 ? 4 : 1); };
     a.piece_p = piece(a.ps);
     a.piece_q = piece(a.qs);
-    a.spin_limit = g_mx_spin_limit.load();
+    a.give_up = g_mx_give_up.load();
+    a.spin_limit = a.give_up == 0 ? kSpin : 0;
     a.status = c.status;
     // rows of x that do not exist are not brought: what the lanes hold in their place reaches no output
     const int p_box = SWAP ? height : (c.m < 128 ? (c.m + 7) & ~7 : 128);
@@ -748,7 +765,7 @@ int run(const Call& c) {
 }  // namespace
 
 // Test hook (include/ironmlx_b200_testing.h).
-void testing_mxfp8_give_up(int on) { g_mx_spin_limit.store(on ? 0 : kSpin); }
+void testing_mxfp8_give_up(int on) { g_mx_give_up.store(on); }
 
 }  // namespace imx
 

@@ -299,3 +299,25 @@ def test_expired_wait_gives_nan_and_a_status(cuda, m, n_in, n_out):
     assert e.value.code == _lib.ERR_DEVICE
     ops.check_status(cuda)
     assert torch.equal(ops.mxfp8_matmul(rows, *w), want)
+
+
+@pytest.mark.parametrize("m,n_in,n_out", [(1, 2048, 512), (8, 2048, 256), (20, 4096, 300), (64, 4096, 512)])
+@pytest.mark.parametrize("rank", [0, 1])
+def test_one_cta_of_a_cut_reduction_gives_up(cuda, m, n_in, n_out, rank):
+    """Where a cluster cuts the reduction and one CTA of it gives up, no output of the cluster has all its parts: all are NaN,
+    the status is reported once, the next call is right again."""
+    g = gen(15)
+    rows, w = mx(g, m, n_in), mx(g, n_out, n_in, 0.02)
+    want = ops.mxfp8_matmul(rows, *w)
+    for _ in range(5):
+        _lib.lib().imx_testing_mxfp8_give_up(2 + rank)
+        try:
+            y = ops.mxfp8_matmul(rows, *w)
+            torch.cuda.synchronize()
+        finally:
+            _lib.lib().imx_testing_mxfp8_give_up(0)
+        assert y.isnan().all()
+        with pytest.raises(_lib.IronMLXError):
+            ops.check_status(cuda)
+        ops.check_status(cuda)
+        assert torch.equal(ops.mxfp8_matmul(rows, *w), want)
