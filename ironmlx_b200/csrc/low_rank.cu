@@ -1055,11 +1055,11 @@ int launch_low_rank(LowRankArgs p, int sms, cudaStream_t stream) {
         IMX_TRY(encode_tensor_map_2d(p.b, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, (size_t)p.count * p.n_out, (size_t)p.rank, (size_t)p.rank * 2, 64, kCols, 128,
                                      true, &maps.b));
     }
-    for (int r0 = 0; r0 < rows; r0 += step) {   
-        p.n = rows - r0 < step ? rows - r0 : step;
-        p.x = whole.x + (size_t)r0 * p.in;
-        p.y = whole.y + (size_t)r0 * p.n_out;
-        p.out = whole.out + (size_t)r0 * p.n_out;
+    for (size_t r0 = 0; r0 < (size_t)rows; r0 += step) {     // (31 bits do not count the end of the last block of 2^31 - 1 rows)
+        p.n = rows - (int)r0 < step ? rows - (int)r0 : step;
+        p.x = whole.x + r0 * p.in;
+        p.y = whole.y + r0 * p.n_out;
+        p.out = whole.out + r0 * p.n_out;
         p.ids = whole.ids + r0;
         int ctas = 1;
         void* args[] = {&p, &ctas, nullptr, nullptr};

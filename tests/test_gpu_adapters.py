@@ -150,6 +150,26 @@ def test_expired_wait_gives_nan_and_a_status(cuda):
     ops.check_status(cuda)
 
 
+def test_as_many_rows_as_an_int_counts(cuda):
+    """2^31 - 1 rows: the last block of 8192 ends where 31 bits end.  Few rows have an adapter, all others stay as they are."""
+    rows = 2 ** 31 - 1
+    if torch.cuda.mem_get_info()[0] < 64 << 30:
+        pytest.skip("64 GB of memory needed")
+    g = gen(23)
+    p = make(g, 1, 8, 1, 2, 8)
+    x, y = torch.empty(rows, 8, dtype=torch.bfloat16, device=cuda), torch.full((rows, 1), 3.0, dtype=torch.bfloat16, device=cuda)
+    ids = torch.full((rows,), -1, dtype=torch.int32, device=cuda)
+    at = [0, 8191, 8192, 2 ** 30, rows - 8192, rows - 8191, rows - 2, rows - 1]
+    small = {**p, "x": bf16(g, 8, 8), "y": y[:8].clone()}
+    for i, row in enumerate(at):
+        x[row], ids[row] = small["x"][i], i % 2
+    run({**p, "x": x, "y": y}, ids, out=y)
+    check(torch.stack([y[row] for row in at]), small, torch.stack([ids[row] for row in at]))
+    for row in at:
+        y[row] = 3.0
+    assert all((part == 3).all() for part in y.split(1 << 28))
+
+
 def test_adapters_on_streams(cuda):
     g = gen(20)
     p, q = make(g, 300, 512, 512, 6, 16), make(g, 24, 512, 512, 6, 16)
