@@ -184,7 +184,7 @@ int launch_add_rms_norm(const void* x, const void* residual, int n, int H, const
     int nv = threads(4) <= max_threads(4) ? 4 : 8;
     while (nv > 1 && threads(nv / 2) <= max_threads(nv / 2) && (threads(nv / 2) == threads(nv) || (long)n * threads(nv / 2) <= 1024L * di.sms)) nv /= 2;
     const int T = threads(nv), rows = T < 256 ? 256 / T : 1, block = T * rows;
-    const int grid = ceil_div(n, rows);
+    const unsigned grid = (unsigned)(((long)n + rows - 1) / rows);
     auto kernel = nv <= 1 ? add_rms_norm_kernel<1> : (nv <= 2 ? add_rms_norm_kernel<2> : (nv <= 4 ? add_rms_norm_kernel<4> : add_rms_norm_kernel<8>));
     kernel<<<grid, block, 0, stream>>>((const __nv_bfloat16*)x, (const __nv_bfloat16*)residual, n, H, (const __nv_bfloat16*)w, eps,
                                        out, T, 1. / H); IMX_LAUNCHED();

@@ -144,6 +144,26 @@ def test_norm_writes_its_rows_only(cuda):
     assert torch.equal(buf["s"][65:92].view(9, 3), rows.scales)
 
 
+def test_norm_of_as_many_rows_as_an_int_counts(cuda):
+    """2^31 - 1 rows of eight, in place: rows of ones stay ones (the factor of 1e-6 is lost in bf16), those at the ends and around
+    the middle are the norms of what was there."""
+    rows = 2 ** 31 - 1
+    if torch.cuda.mem_get_info()[0] < 48 << 30:
+        pytest.skip("48 GB of memory needed")
+    g = gen(7)
+    x = torch.ones(rows, 8, dtype=torch.bfloat16, device=cuda)
+    at, few = [0, 1, 2 ** 30, rows - 9, rows - 8, rows - 7, rows - 2, rows - 1], bf16(g, 8, 8)
+    for i, row in enumerate(at):
+        x[row] = few[i]
+    want = ops.add_rms_norm(few, None, None, EPS)[1]
+    _lib.check(_lib.lib().imx_add_rms_norm(x.data_ptr(), None, rows, 8, None, EPS, None, x.data_ptr(), None, None,
+                                           torch.cuda.current_stream().cuda_stream))
+    assert torch.equal(torch.stack([x[row] for row in at]), want)
+    for row in at:
+        x[row] = 1.0
+    assert all((part == 1).all() for part in x.split(1 << 26))
+
+
 def test_norm_of_infinities_and_nan(cuda):
     """What is not finite stays in its row: a NaN makes the row NaN, an infinity its own place NaN and the rest zero (its
     factor is zero), in bf16 and in 8 bits alike."""
