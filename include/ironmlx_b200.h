@@ -383,7 +383,7 @@ IMX_API int imx_linear(const void* x, int m, int in, const void* w, int n_out, c
  * values), fp32 accumulation, y bf16: what `QuantizedLinear::forward_with_stream` (mlx/src/nn/linear.rs:51-63) computes
  * for an mxfp8 weight, on rows that imx_add_rms_norm (or imx_quantize) left in 8 bits.  w->biases is NULL, w->global_scale
  * is not read.  in: a multiple of 32; x_q and w->w 16-byte aligned, scales at any byte, y at any bf16 value (rows that
- * start on 16 bytes are written fastest); m and n_out at most 2^31 - 256.  y overlaps no input.  scratch: imx_mxfp8_matmul_scratch_bytes bytes, 256-byte
+ * start on 16 bytes are written fastest); m, n_out and in at most 2^31 - 256.  y overlaps no input.  scratch: imx_mxfp8_matmul_scratch_bytes bytes, 256-byte
  * aligned, zero-filled once; it holds the status word that imx_moe_status() reads and nothing that a call leaves for
  * another, so that calls on several streams may share it.  Should a bounded wait run out, the outputs concerned are NaN. */
 IMX_API int imx_mxfp8_matmul_scratch_bytes(int m, int n_out, int in, size_t* bytes);

@@ -47,7 +47,7 @@ constexpr int kMxK = 128;                          // codes of a row in a stage
 constexpr int kMxMaxStages = 10;
 constexpr int kMxGroups = 2;                       // groups of four K steps whose scales are in shared memory
 constexpr int kMxMaxSplits = 8;                    // CTAs of a cluster that cut the K range of a tile
-constexpr int kMxMostRows = 0x7fffff00;            // of either operand: a tile that starts below ends within 31 bits
+constexpr int kMxMost = 0x7fffff00;                // rows of either operand, and their length: a tile that starts below ends within 31 bits
 std::atomic<int> g_mx_give_up{0};                  // see imx_testing_mxfp8_give_up
 
 template <int NT, bool SWAP, bool PAIR>
@@ -785,7 +785,7 @@ int imx_mxfp8_matmul(const void* x_q, const void* x_scales, int m, const imx_qte
                      void* scratch, size_t scratch_bytes, void* stream) {
     IMX_REQUIRE(m >= 0 && n_out > 0 && in > 0 && in % 32 == 0,
                 "mxfp8_matmul: sizes (%d rows, %d -> %d) must be positive, the input dimension a multiple of 32", m, in, n_out);
-    IMX_REQUIRE(m <= kMxMostRows && n_out <= kMxMostRows, "mxfp8_matmul: at most %d rows and outputs", kMxMostRows);
+    IMX_REQUIRE(m <= kMxMost && n_out <= kMxMost && in <= kMxMost, "mxfp8_matmul: rows, outputs and inputs of at most %d", kMxMost);
     if (m == 0) return IMX_OK;
     IMX_REQUIRE(x_q && x_scales && w && w->w && w->scales && y, "mxfp8_matmul: rows, weight and their scales, and y are required");
     IMX_REQUIRE(w->biases == nullptr, "mxfp8_matmul: an mxfp8 weight has no biases");

@@ -43,6 +43,7 @@ def product(xq=A, xs=B, m=4, w=D, ws=E, biases=None, n_out=64, n_in=64, y=F, scr
 @pytest.mark.parametrize("kw,needle", [
     (dict(m=-1), b"sizes"), (dict(n_out=0), b"sizes"), (dict(n_in=0), b"sizes"), (dict(n_in=48), b"multiple of 32"),
     (dict(m=0x7fffff80), b"at most"), (dict(n_out=0x7fffffff), b"at most"),
+    (dict(n_in=0x7fffffe0), b"at most"), (dict(n_in=0x7fffff20), b"at most"),
     (dict(xq=None), b"required"), (dict(xs=None), b"required"), (dict(w=None), b"required"), (dict(ws=None), b"required"),
     (dict(y=None), b"required"), (dict(biases=A), b"biases"), (dict(xq=A + 4), b"aligned"), (dict(w=D + 8), b"aligned"),
     (dict(y=F + 1), b"aligned"), (dict(y=A + 128), b"overlaps"), (dict(y=B), b"overlaps"), (dict(y=D - 2), b"overlaps"),
