@@ -245,6 +245,13 @@ def _row_count(name: str, x: torch.Tensor, length: int) -> int:
     return n
 
 
+def _count(name: str, what: str, value: int) -> int:
+    """A dimension that the C ABI takes as an int (ctypes would cut off what 31 bits do not hold)."""
+    if value > 0x7fffffff:
+        raise IronMLXError(_lib.ERR_INVALID, f"{name}: {what} of {value}, at most 2^31 - 1")
+    return value
+
+
 def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: Optional[torch.Tensor], eps: float,
                  out: str = "bf16", stream=None):
     """`h = x + residual` and `rms_norm(h)` in one pass, sums in fp32, each output rounded once.
@@ -271,6 +278,7 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: Opti
         with _on(x, stream):
             return add_rms_norm(x, residual, weight, eps, out)
     n = _row_count("add_rms_norm", x, hidden)
+    _count("add_rms_norm", "a row length", hidden)
     h, y, rows = x, None, None
     residual_at = h_at = y_at = q_at = scales_at = None
     if residual is not None:
@@ -334,6 +342,8 @@ def mxfp8_matmul(rows, w: torch.Tensor, scales: torch.Tensor, stream=None) -> to
         with _on(x, stream):
             return mxfp8_matmul(rows, w, scales)
     n = _row_count("mxfp8_matmul", x, words)
+    _count("mxfp8_matmul", "an input dimension", words * 4)
+    _count("mxfp8_matmul", "an output dimension", n_out)
     index = x.get_device()
     y = torch.empty(*lead, n_out, dtype=torch.bfloat16, device=x.device)
     qt = QTensor(w.data_ptr(), scales.data_ptr(), None, 1.0)
@@ -361,6 +371,8 @@ def low_rank_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
         raise IronMLXError(_lib.ERR_INVALID,
                            f"low_rank_add: x {tuple(xshape)} and y {tuple(yshape)} do not match adapters {in_dim} -> {n_out}")
     rows = _row_count("low_rank_add", x, in_dim)
+    for what, value in (("an input dimension", in_dim), ("an output dimension", n_out), ("a rank", rank), ("a number of adapters", count)):
+        _count("low_rank_add", what, value)
     if ids.dtype != torch.int32 or ids.numel() != rows:
         raise IronMLXError(_lib.ERR_INVALID, f"low_rank_add: ids must be int32, one for each of the {rows} rows")
     if scale is not None and (scale.dtype != torch.float32 or scale.numel() != count):

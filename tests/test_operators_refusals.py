@@ -108,6 +108,33 @@ def test_more_rows_than_an_int_counts():
         ops._row_count("op", x.expand(1 << 31, 8), 8)
 
 
+def test_dimensions_that_an_int_does_not_hold(monkeypatch):
+    """The C ABI takes ints, and ctypes would pass 2^32 + 64 on as 64."""
+    monkeypatch.setattr(ops, "_require_same_device", lambda name, *tensors: None)
+    monkeypatch.setattr(ops, "_elsewhere", lambda x, stream: False)
+
+    def meta(dtype, *shape):
+        return torch.empty(1, device="meta", dtype=dtype).expand(*shape)
+
+    bf, i32, u8 = torch.bfloat16, torch.int32, torch.uint8
+    long = 2 ** 32 + 64
+    with pytest.raises(_lib.IronMLXError, match="row length"):
+        ops.add_rms_norm(meta(bf, 1, long), None, None, 1e-6)
+    with pytest.raises(_lib.IronMLXError, match="input dimension"):
+        ops.mxfp8_matmul((meta(i32, 1, long // 4), meta(u8, 1, long // 32)), meta(i32, 8, long // 4), meta(u8, 8, long // 32))
+    with pytest.raises(_lib.IronMLXError, match="output dimension"):
+        ops.mxfp8_matmul((meta(i32, 1, 16), meta(u8, 1, 2)), meta(i32, long, 16), meta(u8, long, 2))
+    ids = meta(i32, 1)
+    with pytest.raises(_lib.IronMLXError, match="input dimension"):
+        ops.low_rank_add(meta(bf, 1, 64), meta(bf, 1, long), meta(bf, 2, 8, long), meta(bf, 2, 64, 8), ids)
+    with pytest.raises(_lib.IronMLXError, match="output dimension"):
+        ops.low_rank_add(meta(bf, 1, long), meta(bf, 1, 64), meta(bf, 2, 8, 64), meta(bf, 2, long, 8), ids)
+    with pytest.raises(_lib.IronMLXError, match="number of adapters"):
+        ops.low_rank_add(meta(bf, 1, 64), meta(bf, 1, 64), meta(bf, long, 8, 64), meta(bf, long, 64, 8), ids)
+    with pytest.raises(_lib.IronMLXError, match="a rank"):
+        ops.low_rank_add(meta(bf, 1, 64), meta(bf, 1, 64), meta(bf, 2, long, 64), meta(bf, 2, 64, long), ids)
+
+
 def build_cpp(out_dir):
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
     exe, cuda, lib_dir = os.path.join(out_dir, "operators_main"), os.environ.get("CUDA_HOME", "/usr/local/cuda"), os.path.dirname(_lib.LIB_PATH)
