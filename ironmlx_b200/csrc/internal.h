@@ -169,6 +169,14 @@ void testing_decode_handoff(int spin_limit, int withhold);
 void testing_route_give_up(int on);
 void testing_prefill_give_up(int on);
 constexpr int kSpin = 1 << 22;               // bound of the waits of the tensor-core kernels
+// A CTA that holds tensor memory while it waits for another CTA of its cluster must find no other kernel's that does so on its
+// SM, or each could hold what the other's partner, on another SM, waits to allocate (tcgen05.alloc waits without a bound).
+// Shared memory keeps them apart: such kernels ask for kClusterSmem at the least, but for the adapters' tiles up to a rank of
+// 64, of which two fit into an SM and its tensor memory (kTileSmem at the least, 256 columns each).
+constexpr size_t kClusterSmem = 144 * 1024, kTileSmem = 86 * 1024;
+constexpr bool never_share_an_sm(size_t a, size_t b) { return a + 1024 + b + 1024 > 228 * 1024; }       // (1 KB of each CTA is the system's)
+static_assert(never_share_an_sm(kClusterSmem, kClusterSmem) && never_share_an_sm(kClusterSmem, kTileSmem), "they could wait for one another");
+static_assert(never_share_an_sm(2 * kTileSmem + 1024, kTileSmem), "three tiles have no room in tensor memory");
 // Decode kernel of the block-scaled float formats (mxfp8, nvfp4).
 bool decode_fp_supported(const ExpertSet& s);
 int launch_decode_fp(const GroupedArgs& a, cudaStream_t stream, cudaEvent_t mid = nullptr);

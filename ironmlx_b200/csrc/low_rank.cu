@@ -459,7 +459,7 @@ struct TileMaps {
 struct TilePlan {
     int r16, blocks;                          // rank rounded up to 16; blocks of 64 of it
     int stages, stage, sums_at, low_at, low_pitch, bytes;  // low_at: the low-rank rows, fp32, low_pitch values apart (no bank twice)
-    __host__ __device__ TilePlan(int rank, int nj) {
+    __host__ __device__ constexpr TilePlan(int rank, int nj) : r16(0), blocks(0), stages(0), stage(0), sums_at(0), low_at(0), low_pitch(0), bytes(0) {
         r16 = (rank + 15) & ~15;
         blocks = (r16 + 63) / 64;
         stages = nj <= 4 ? 5 : 3;
@@ -470,8 +470,11 @@ struct TilePlan {
         const int end = low_at + kTileRows * low_pitch * 4;
         sums_at = nj == 4 ? end : 0;
         bytes = end + (nj == 4 ? kTileRows * r16 * 4 : 0);
+        if (nj > 2 && bytes + 1024 < (int)kClusterSmem) bytes = (int)kClusterSmem - 1024;
     }
+    constexpr size_t smem() const { return (size_t)bytes + 1024; }
 };
+static_assert(TilePlan(8, 1).smem() >= kTileSmem && TilePlan(40, 2).smem() >= kTileSmem, "beside another kernel that waits in a cluster");
 
 // 16 lanes x 8 columns a count: thread t gets of each block of eight columns lane t / 4, columns 2 (t % 4), +1, and the same of
 // lane t / 4 + 8, as an mma.sync leaves its sums.
@@ -515,12 +518,13 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
     // First of all the tensor memory: an SM starts its second CTA only when the first has given up the permit to allocate (with
     // the allocation behind the ids half of the CTAs of 8192 rows started 6.7 us late, of 777 rows 3.2).
     // The first product's sums; in their place two stages' of the second, and from column 128 on its A, see below.
+    static_assert(NJ > 2 || 2 * (128 + 2 * 16 * NJ) <= 512, "two CTAs an SM");
     constexpr uint32_t kTmem = NJ <= 4 ? 256 : 512, kLowAt = 128, kLowCols = 16 * NJ;
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&s.tmem_base)), "r"(kTmem) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    // (No CTA that holds all 512 columns and waits for another SM's is ever beside this one: their shared memories do not fit.)
+    // (Which kernels are beside this one on an SM: internal.h.)
     auto give_back = [&]() {
         if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(s.tmem_base), "r"(kTmem) : "memory");
     };
@@ -1087,7 +1091,7 @@ int launch_low_rank(LowRankArgs p, int sms, cudaStream_t stream) {
         const TileKernel tile = tile_kernel(p.rank, p.wide != 0);
         args[2] = &clusters;
         args[3] = &maps;
-        IMX_TRY(launch_clusters(tile.kernel, (unsigned)(units * ctas * clusters), kTileThreads, ctas, (size_t)TilePlan(p.rank, tile.nj).bytes + 1024, stream, args));
+        IMX_TRY(launch_clusters(tile.kernel, (unsigned)(units * ctas * clusters), kTileThreads, ctas, TilePlan(p.rank, tile.nj).smem(), stream, args));
     }
     return IMX_OK;
 }
@@ -1141,7 +1145,7 @@ extern "C" int imx_low_rank_add(const void* y, const void* x, int n_rows, int in
             IMX_CHECK_CUDA(cudaFuncSetAttribute(few.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FewPlan(rank, few.rb).bytes));
             for (bool wide : {false, true}) {
                 const TileKernel tile = tile_kernel(rank, wide);
-                IMX_CHECK_CUDA(cudaFuncSetAttribute(tile.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TilePlan(rank, tile.nj).bytes + 1024));
+                IMX_CHECK_CUDA(cudaFuncSetAttribute(tile.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)TilePlan(rank, tile.nj).smem()));
             }
         }
         device_mark_setup(di.ordinal, kSetupLowRank);

@@ -67,6 +67,7 @@ struct Plan {
     static constexpr int kAcc1 = NT == 256 ? kSf0 - 256 : NT;            // ... of the second accumulator
     static constexpr int kLag = NT == 256 ? 1 : 2;                       // a tile's MMAs wait for the drain of the kLag-th before
     static constexpr size_t kSmem = (size_t)kStages * kTile + kMxGroups * kGroup + kOut + 2048;
+    static_assert(kSmem >= kClusterSmem, "beside another kernel that waits in a cluster");
     static_assert(kSf0 + kStages * kSfCols <= 512 && (NT < 256 || kAcc1 >= 192), "tensor memory");
 };
 

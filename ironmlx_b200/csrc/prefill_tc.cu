@@ -76,6 +76,7 @@ bool make_plan(const QFormat& f, int fmt, int K_max, int K_min, bool wide, bool 
     out->p.spin_limit = g_spin_limit.load();
     out->p.lg_group = log2_exact(f.group);
     out->smem = fixed + (size_t)st * stage;
+    if (pair && out->smem < kClusterSmem) out->smem = kClusterSmem;          // (two-term weights: four stages are about 100 KB)
     out->wide = wide;
     out->pair = pair;
     out->xr = xr;

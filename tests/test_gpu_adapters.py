@@ -200,6 +200,29 @@ def test_adapters_beside_products(cuda):
     assert all(torch.equal(x, alone[0]) and torch.equal(y, alone[1]) for x, y in got)
 
 
+@pytest.mark.parametrize("rank", [16, 64, 136, 256])
+def test_adapters_beside_pairs_with_two_term_weights(cuda, rank):
+    """Tiles of adapters and the pairs of CTAs of a 6-bit projection (which hold all of tensor memory and need little shared
+    memory) on streams of their own at the same time, and tiles of a small rank beside both: the values of the calls alone."""
+    g = gen(78)
+    p, q = make(g, 700, 1024, 2048, 5, rank), make(g, 600, 512, 1024, 3, 8)
+    ip, iq = (torch.randint(-1, 3, (t,), generator=g, device="cuda", dtype=torch.int32) for t in (700, 600))
+    w = nn.QuantizedLinear.new(*ops.quantize(torch.randn(2048, 1024, generator=g, device="cuda") * 0.05, bits=6, group_size=64), 64, 6)
+    x = bf16(g, 1500, 1024)
+    alone = run(p, ip), run(q, iq), w.forward_with_stream(x)
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+
+    def project():
+        with torch.cuda.stream(streams[2]):
+            return w.forward_with_stream(x)
+
+    got = [(run(p, ip, stream=streams[i % 2]), run(q, iq, stream=streams[1 - i % 2]), project()) for i in range(40)]
+    torch.cuda.synchronize()
+    ops.check_status()
+    assert all(torch.equal(a, b) for three in got for a, b in zip(three, alone))
+
+
 @pytest.mark.parametrize("kind", ["dense", "affine", "mxfp8"])
 def test_projection_with_adapters(cuda, kind):
     g = gen(21)
