@@ -42,7 +42,8 @@ extern "C"
 #endif
 __attribute__((visibility("default"))) void imx_testing_mxfp8_give_up(int on);
 
-/* ... and for imx_low_rank_add's kernel of many rows: status 5. */
+/* ... and for imx_low_rank_add's kernel of many rows: status 5.  2 + r: CTA r of each cluster alone; all outputs of a cluster
+ * with adapters are NaN then too. */
 #ifdef __cplusplus
 extern "C"
 #endif

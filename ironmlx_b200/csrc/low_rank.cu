@@ -31,7 +31,7 @@ constexpr int kMaxRank = 256;
 constexpr int kThreads = 256;
 constexpr size_t kStatusBytes = 256;
 constexpr int kMostColumns = 1 << 30;         // of x and y: columns past the end of a row are counted in 31 bits
-std::atomic<int> g_low_rank_spin_limit{kSpin};
+std::atomic<int> g_low_rank_give_up{0};       // see imx_testing_low_rank_give_up
 
 struct LowRankArgs {
     const __nv_bfloat16* y;
@@ -43,7 +43,7 @@ struct LowRankArgs {
     __nv_bfloat16* out;
     int n, in, n_out, count, rank;
     int wide;                 // y and out: rows of whole 16-byte pieces
-    int spin_limit;
+    int spin_limit, give_up;
     int32_t* status;
 };
 
@@ -515,6 +515,7 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     const int shift = 31 - __clz(ctas), cut = shift + 31 - __clz(clusters);       // (both are powers of two)
     const int unit = (int)blockIdx.x >> cut, c = (int)blockIdx.x & (ctas - 1);
+    const int spin = p.give_up > 1 && p.give_up - 2 != c ? kSpin : p.spin_limit;
     // First of all the tensor memory: an SM starts its second CTA only when the first has given up the permit to allocate (with
     // the allocation behind the ids half of the CTAs of 8192 rows started 6.7 us late, of 777 rows 3.2).
     // The first product's sums; in their place two stages' of the second, and from column 128 on its A, see below.
@@ -680,7 +681,7 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
         bool ok = true;
         auto fill = [&](int upto) {
             for (; issued < upto && ok; ++issued) {
-                ok = tc::mbar_wait(tc::smem_u32(&s.used[slot]), ph, abort_flag, p.spin_limit);
+                ok = tc::mbar_wait(tc::smem_u32(&s.used[slot]), ph, abort_flag, spin);
                 if (!ok) break;
                 if (lane == 0) {
                     const uint32_t to = base + (uint32_t)(slot * pl.stage + kBlock), bar = tc::smem_u32(&s.loaded[slot]);
@@ -718,8 +719,8 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
             }
         };
         for (int i = 0; i < n_in; ++i) {
-            tc::mbar_wait_on(tc::smem_u32(&s.rows_there[slot]), ph, flag, p.spin_limit);
-            tc::mbar_wait_on(tc::smem_u32(&s.loaded[slot]), ph, flag, p.spin_limit);
+            tc::mbar_wait_on(tc::smem_u32(&s.rows_there[slot]), ph, flag, spin);
+            tc::mbar_wait_on(tc::smem_u32(&s.loaded[slot]), ph, flag, spin);
             tc::tc_fence_after();
             const uint32_t st = base + (uint32_t)(slot * pl.stage), idesc = tc::idesc_for(64, r16) | (1u << 7) | (1u << 10);      // bf16
 #pragma unroll
@@ -739,8 +740,8 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
         const uint32_t idesc = tc::idesc_for(128, kCols) | (1u << 7) | (1u << 10);
         const int kks = r16 / 16;
         for (int e = 0; e < total - n_in; ++e) {
-            tc::mbar_wait_on(tc::smem_u32(&s.loaded[slot]), ph, flag, p.spin_limit);
-            if (e >= 2) tc::mbar_wait_on(tc::smem_u32(&s.sums_free[e & 1]), (uint32_t)((e - 2) >> 1) & 1u, flag, p.spin_limit);
+            tc::mbar_wait_on(tc::smem_u32(&s.loaded[slot]), ph, flag, spin);
+            if (e >= 2) tc::mbar_wait_on(tc::smem_u32(&s.sums_free[e & 1]), (uint32_t)((e - 2) >> 1) & 1u, flag, spin);
             tc::tc_fence_after();
             const uint32_t d = tmem + (uint32_t)((e & 1) * 64);
             const uint64_t b_desc = tc::smem_desc(base + (uint32_t)(slot * pl.stage + kBlock));
@@ -758,7 +759,7 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
         }
     } else {
         const int rt = warp & 3, half = warp >> 2, g = lane >> 2, q = lane & 3;    // the warp's 16 rows, and its half of the columns
-        auto wait = [&](uint64_t& bar, int phase) { tc::mbar_wait(tc::smem_u32(&bar), (uint32_t)phase & 1u, abort_flag, p.spin_limit); };
+        auto wait = [&](uint64_t& bar, int phase) { tc::mbar_wait(tc::smem_u32(&bar), (uint32_t)phase & 1u, abort_flag, spin); };
         const float sc = p.scale != nullptr ? p.scale[id] : 1.f;
         // What a thread copies is the same in every stage but for the columns: a piece of two rows of x, or of y.
         const int cr = tid >> 3, cc = (tid & 7) * 8;
@@ -827,12 +828,16 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
         float* sums = reinterpret_cast<float*>(smem + sums_of(c));
         if (n_in > 0) wait(s.used[(n_in - 1) % S], (n_in - 1) / S);
         tc::tc_fence_after();
+        const bool gave_up = *abort_flag != 0;             // a CTA that has makes the low-rank rows NaN, and so all outputs of the cluster
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
             const int t = half + 2 * j;
             if (t * 16 >= r16) break;
             float v[8] = {};
             if (n_in > 0) tmem_ld_16x16(tmem + ((uint32_t)(rt * 32) << 16) + (uint32_t)(t * 16), v);
+            if (gave_up)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(0x7fc00000u);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 float* d = sums + (rt * 16 + g) * r16 + t * 16 + h * 8 + 2 * q;
@@ -999,7 +1004,7 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
         copies_wait<0>();
     }
     __syncthreads();
-    if (s.abort != 0) {                                    // a wait ran out: NaN in this CTA's columns
+    if (s.abort != 0) {                                    // a wait ran out: NaN in this CTA's columns (after the exchange in these alone)
         if (warp == 8) {
             if (tc::elect_one()) tc::umma_commit(tc::smem_u32(&s.retired));
             __syncwarp();
@@ -1099,7 +1104,7 @@ int launch_low_rank(LowRankArgs p, int sms, cudaStream_t stream) {
 }  // namespace
 
 // Test hook (include/ironmlx_b200_testing.h).
-void testing_low_rank_give_up(int on) { g_low_rank_spin_limit.store(on ? 0 : kSpin); }
+void testing_low_rank_give_up(int on) { g_low_rank_give_up.store(on); }
 
 }  // namespace imx
 
@@ -1150,9 +1155,10 @@ extern "C" int imx_low_rank_add(const void* y, const void* x, int n_rows, int in
         }
         device_mark_setup(di.ordinal, kSetupLowRank);
     }
+    const int give_up = g_low_rank_give_up.load();
     const int wide = n_out % 8 == 0 && (((uintptr_t)y | (uintptr_t)out) % 16) == 0;
     return launch_low_rank(LowRankArgs{(const __nv_bfloat16*)y, (const __nv_bfloat16*)x, (const __nv_bfloat16*)ad->a, (const __nv_bfloat16*)ad->b,
                                        ad->scale, ids, (__nv_bfloat16*)out, n_rows, in, n_out, ad->count, ad->rank, wide,
-                                       g_low_rank_spin_limit.load(), (int32_t*)scratch},
+                                       give_up == 0 ? kSpin : 0, give_up, (int32_t*)scratch},
                            di.sms, (cudaStream_t)stream);
 }

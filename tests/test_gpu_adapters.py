@@ -150,6 +150,28 @@ def test_expired_wait_gives_nan_and_a_status(cuda):
     ops.check_status(cuda)
 
 
+@pytest.mark.parametrize("rank", [16, 64, 128, 256])
+@pytest.mark.parametrize("cta", [0, 1, 7])
+def test_one_cta_of_a_cluster_gives_up(cuda, rank, cta):
+    """A CTA that gives up in the first product has a part of its rows' sums that all CTAs of its cluster need: no output of
+    theirs is a number, the status is reported once, the next call is right again."""
+    g = gen(24)
+    p = make(g, 400, 512, 1040, 3, rank)
+    ids = torch.randint(-1, 3, (400,), generator=g, device="cuda", dtype=torch.int32)
+    want = run(p, ids)
+    _lib.lib().imx_testing_low_rank_give_up(2 + cta)
+    try:
+        out = run(p, ids)
+        torch.cuda.synchronize()
+    finally:
+        _lib.lib().imx_testing_low_rank_give_up(0)
+    assert out[ids >= 0].isnan().all() and torch.equal(out[ids < 0], p["y"][ids < 0])
+    with pytest.raises(_lib.IronMLXError):
+        ops.check_status(cuda)
+    ops.check_status(cuda)
+    assert torch.equal(run(p, ids), want)
+
+
 def test_as_many_rows_as_an_int_counts(cuda):
     """2^31 - 1 rows: the last block of 8192 ends where 31 bits end.  Few rows have an adapter, all others stay as they are."""
     rows = 2 ** 31 - 1
