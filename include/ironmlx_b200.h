@@ -189,6 +189,11 @@ IMX_API int imx_moe_forward_host(const imx_moe_config* cfg, const imx_moe_weight
  * ran out: the call's output is incomplete). */
 IMX_API int imx_moe_status(void* workspace, void* stream);
 
+/* A status block of the library's own on the current device: 256 bytes, zero when the library is loaded, there until the process
+ * ends.  For the calls whose scratch is a status word alone (imx_mxfp8_matmul, imx_low_rank_add); nothing is allocated or
+ * launched, so that it may be asked for, first of all, while a stream is captured. */
+IMX_API int imx_status_block(void** block);
+
 /* The expert kernels carry their intermediate rows in fp16 (SwiGLU outputs; on the tensor-core path also
  * the expert rows) and clamp what exceeds its range (+-65504).  A clamp changes the result, so it is counted in
  * the workspace (per value on the decode paths, per thread and tile on the tensor-core path): this reads the

@@ -77,6 +77,7 @@ SIGNATURES = {
     "imx_testing_prefill_give_up": (None, [_i]),
     "imx_testing_mxfp8_give_up": (None, [_i]),
     "imx_testing_low_rank_give_up": (None, [_i]),
+    "imx_status_block": (_i, [C.POINTER(_vp)]),
     "imx_moe_saturations": (_i, [_vp, _vp, C.POINTER(C.c_longlong)]),
     "imx_moe_route": (_i, [_vp, _i, _i, _vp, _vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
     "imx_moe_route_scratch_bytes": (_i, [_i, _i, _i, C.POINTER(_sz)]),

@@ -2,6 +2,7 @@
 // workspace carving and stage orchestration.  No device allocation happens
 // here; every scratch byte comes from the caller's workspace.
 #include <cstring>
+#include <mutex>
 
 #include "internal.h"
 #include "../../include/ironmlx_b200_testing.h"
@@ -9,6 +10,9 @@
 namespace imx {
 
 static thread_local std::string g_error;
+
+// imx_status_block's: in the library's device image, one for each GPU.
+static __device__ __align__(256) int32_t g_status_block[64];
 
 void set_error(const char* fmt, ...) {
     char buf[1024];
@@ -537,6 +541,23 @@ int imx_moe_status(void* workspace, void* stream_) {
         IMX_CHECK_CUDA(cudaMemsetAsync(workspace, 0, sizeof(host), stream));
         return IMX_ERR_DEVICE;
     }
+    return IMX_OK;
+}
+
+int imx_status_block(void** block) {
+    IMX_REQUIRE(block != nullptr, "status_block: nowhere to put the address");
+    static std::mutex mu;
+    static void* addr[64] = {};
+    int dev = 0;
+    IMX_CHECK_CUDA(cudaGetDevice(&dev));
+    IMX_REQUIRE(dev >= 0 && dev < 64, "status_block: device ordinal %d not supported", dev);
+    std::lock_guard<std::mutex> lock(mu);
+    if (addr[dev] == nullptr) {
+        void* p = nullptr;
+        IMX_CHECK_CUDA(cudaGetSymbolAddress(&p, g_status_block));
+        addr[dev] = p;
+    }
+    *block = addr[dev];
     return IMX_OK;
 }
 

@@ -301,25 +301,28 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: Opti
 _STATUS = {}
 
 
-def _status_block(index: int) -> torch.Tensor:
-    """The status block of a device's `mxfp8_matmul` and `low_rank_add` calls: zero-filled once, kernels only ever set its first word."""
-    buf = _STATUS.get(index)
-    if buf is None:
-        buf = torch.zeros(256, dtype=torch.uint8, device=torch.device("cuda", index))
-        if not torch.cuda.is_current_stream_capturing():             # in a capture: one for this call
-            torch.cuda.current_stream(index).synchronize()           # other streams see the zeros
-            _STATUS[index] = buf
-    return buf
+def _status_block(index: int) -> int:
+    """The address of the status block that the `mxfp8_matmul` and `low_rank_add` calls of a device, the current one, share: the
+    library's own, which kernels only ever set, so that a captured call's replays are reported like any call."""
+    at = _STATUS.get(index)
+    if at is None:
+        block = C.c_void_p()
+        check(lib().imx_status_block(C.byref(block)))
+        at = _STATUS[index] = block.value
+    return at
 
 
 def check_status(device=None, stream=None) -> None:
-    """Raises if a bounded wait ran out in an `mxfp8_matmul` or `low_rank_add` call on the device (default: the current one) since the last
-    check; synchronises the stream."""
+    """Raises if a bounded wait ran out in an `mxfp8_matmul` or `low_rank_add` call on the device (default: the current one),
+    replayed ones among them, since the last check; synchronises the stream."""
     index = torch.device("cuda" if device is None else device).index
-    buf = _STATUS.get(torch.cuda.current_device() if index is None else index)
-    if buf is not None:
-        with _on(buf, stream):
-            check(lib().imx_moe_status(buf.data_ptr(), stream_ptr()))
+    index = torch.cuda.current_device() if index is None else index
+    if index not in _STATUS:                     # no such call yet
+        return
+    if stream is not None and stream.device_index != index:
+        raise IronMLXError(_lib.ERR_INVALID, f"a stream of device {stream.device_index} cannot take work on cuda:{index}")
+    with torch.cuda.device(index) if stream is None else torch.cuda.stream(stream):
+        check(lib().imx_moe_status(_STATUS[index], stream_ptr()))
 
 
 def mxfp8_matmul(rows, w: torch.Tensor, scales: torch.Tensor, stream=None) -> torch.Tensor:
@@ -348,7 +351,7 @@ def mxfp8_matmul(rows, w: torch.Tensor, scales: torch.Tensor, stream=None) -> to
     y = torch.empty(*lead, n_out, dtype=torch.bfloat16, device=x.device)
     qt = QTensor(w.data_ptr(), scales.data_ptr(), None, 1.0)
     check(lib().imx_mxfp8_matmul(x.data_ptr(), xs.data_ptr(), n, C.byref(qt), n_out, words * 4, y.data_ptr(),
-                                 _status_block(index).data_ptr(), 256, _raw_stream(index)))
+                                 _status_block(index), 256, _raw_stream(index)))
     return y
 
 
@@ -387,5 +390,5 @@ def low_rank_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
     ad = _lib.Adapters(a.data_ptr(), b.data_ptr(), None if scale is None else scale.data_ptr(), count, rank)
     index = x.get_device()
     check(lib().imx_low_rank_add(y.data_ptr(), x.data_ptr(), rows, in_dim, C.byref(ad), ids.data_ptr(), n_out, out.data_ptr(),
-                                 _status_block(index).data_ptr(), 256, _raw_stream(index)))
+                                 _status_block(index), 256, _raw_stream(index)))
     return out

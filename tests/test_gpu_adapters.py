@@ -5,6 +5,9 @@ Tolerances: one rounding to bf16 is 2^-8 of the value; the low-rank row and the 
 their sums in fp32: 2^-15 of the sum of magnitudes |scale| (|x| |a|^T) |b|^T covers 2^-16 for the low-rank row's rounding and
 fp32 sums of up to 8192 and 256 terms in 32 or more parts (2^-17)."""
 import ctypes as C
+import os
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -148,6 +151,49 @@ def test_expired_wait_gives_nan_and_a_status(cuda):
         ops.check_status(cuda)
     assert torch.equal(run(p, ids), want)
     ops.check_status(cuda)
+
+
+FIRST_CALL_IN_A_CAPTURE = """
+import torch
+from ironmlx_b200 import IronMLXError, _lib, ops
+t, k, n = 300, 512, 512
+y, x, ids = torch.zeros(t, n, device="cuda").bfloat16(), torch.ones(t, k, device="cuda").bfloat16(), torch.zeros(t, dtype=torch.int32, device="cuda")
+a, b = torch.ones(1, 16, k, device="cuda").bfloat16(), torch.ones(1, n, 16, device="cuda").bfloat16()
+packed, scales = torch.full((t, k // 4), 0x38383838, dtype=torch.int32, device="cuda"), torch.full((t, k // 32), 127, dtype=torch.uint8, device="cuda")
+hooks = dict(adapters=_lib.lib().imx_testing_low_rank_give_up, product=_lib.lib().imx_testing_mxfp8_give_up)
+calls = dict(adapters=lambda: ops.low_rank_add(y, x, a, b, ids), product=lambda: ops.mxfp8_matmul((packed, scales), packed, scales))
+values = dict(adapters=16.0 * k, product=float(k))
+for which in (FIRST, "adapters", "product"):
+    for give_up in (1, 0):
+        hooks[which](give_up)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out, after = calls[which](), torch.ones(4096, device="cuda")
+        hooks[which](0)
+        for _ in range(2):
+            graph.replay()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert (after == 1).all()
+            if give_up:
+                assert out.isnan().all()
+                try:
+                    ops.check_status()
+                    raise SystemExit("not reported")
+                except IronMLXError as e:
+                    assert e.code == _lib.ERR_DEVICE
+            else:
+                assert (out == values[which]).all()
+            ops.check_status()
+"""
+
+
+@pytest.mark.parametrize("first", ["adapters", "product"])
+def test_first_call_in_a_capture_reports_its_replays(cuda, first):
+    """In a process of its own, whose first call of the operators is captured: every replay whose waits run out is reported."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", FIRST_CALL_IN_A_CAPTURE.replace("FIRST", repr(first))], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stdout + done.stderr
 
 
 @pytest.mark.parametrize("rank", [16, 64, 128, 256])

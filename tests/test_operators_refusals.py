@@ -90,6 +90,10 @@ def test_no_rows_are_no_work():
     assert low_rank(n=0, y=None, x=None, ids=None, out=None) == 0
 
 
+def test_status_block_refuses_no_address():
+    refused(_lib.lib().imx_status_block(None), b"nowhere")
+
+
 def test_scratch_sizes():
     nb = C.c_size_t(0)
     lib = _lib.lib()
