@@ -245,11 +245,10 @@ def _row_count(name: str, x: torch.Tensor, length: int) -> int:
     return n
 
 
-def _count(name: str, what: str, value: int) -> int:
-    """A dimension that the C ABI takes as an int (ctypes would cut off what 31 bits do not hold)."""
+def _count(name: str, what: str, value: int) -> None:
+    """Refuses a dimension that the C ABI's int does not hold (ctypes would cut it off)."""
     if value > 0x7fffffff:
         raise IronMLXError(_lib.ERR_INVALID, f"{name}: {what} of {value}, at most 2^31 - 1")
-    return value
 
 
 def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor], weight: Optional[torch.Tensor], eps: float,
@@ -345,8 +344,9 @@ def mxfp8_matmul(rows, w: torch.Tensor, scales: torch.Tensor, stream=None) -> to
         with _on(x, stream):
             return mxfp8_matmul(rows, w, scales)
     n = _row_count("mxfp8_matmul", x, words)
-    _count("mxfp8_matmul", "an input dimension", words * 4)
-    _count("mxfp8_matmul", "an output dimension", n_out)
+    if max(words * 4, n_out) > 0x7fffffff:
+        _count("mxfp8_matmul", "an input dimension", words * 4)
+        _count("mxfp8_matmul", "an output dimension", n_out)
     index = x.get_device()
     y = torch.empty(*lead, n_out, dtype=torch.bfloat16, device=x.device)
     qt = QTensor(w.data_ptr(), scales.data_ptr(), None, 1.0)
@@ -374,8 +374,9 @@ def low_rank_add(y: torch.Tensor, x: torch.Tensor, a: torch.Tensor, b: torch.Ten
         raise IronMLXError(_lib.ERR_INVALID,
                            f"low_rank_add: x {tuple(xshape)} and y {tuple(yshape)} do not match adapters {in_dim} -> {n_out}")
     rows = _row_count("low_rank_add", x, in_dim)
-    for what, value in (("an input dimension", in_dim), ("an output dimension", n_out), ("a rank", rank), ("a number of adapters", count)):
-        _count("low_rank_add", what, value)
+    if max(in_dim, n_out, rank, count) > 0x7fffffff:
+        for what, value in (("an input dimension", in_dim), ("an output dimension", n_out), ("a rank", rank), ("a number of adapters", count)):
+            _count("low_rank_add", what, value)
     if ids.dtype != torch.int32 or ids.numel() != rows:
         raise IronMLXError(_lib.ERR_INVALID, f"low_rank_add: ids must be int32, one for each of the {rows} rows")
     if scale is not None and (scale.dtype != torch.float32 or scale.numel() != count):
