@@ -114,6 +114,13 @@ private:
     size_t bytes_ = 0;
 };
 
+// The library's status block of the current device.
+inline void* status_block() {
+    void* block = nullptr;
+    check(imx_status_block(&block));
+    return block;
+}
+
 namespace ops {
 
 // x [M, in] (bf16) times a packed weight [out, in] (transpose = true) or [in, out] (false).
@@ -142,8 +149,8 @@ inline void dequantize(const Array& w, const Array& scales, const Array* biases,
                          stream));
 }
 
-// Rows in mxfp8 (packed [M, in/4], scales [M, in/32]) times an mxfp8 weight.  The scratch is zero-filled when it is made and
-// only ever holds the status word.
+// Rows in mxfp8 (packed [M, in/4], scales [M, in/32]) times an mxfp8 weight.  Nothing is allocated, so that the first call may
+// be captured; an expired wait is reported by check_status().
 inline void mxfp8_matmul(const Array& rows, const Array& row_scales, const Array& w, const Array& scales, Array& y,
                          cudaStream_t stream = nullptr) {
     imx_qtensor q{w.ptr, scales.ptr, nullptr, 1.f};
@@ -151,12 +158,11 @@ inline void mxfp8_matmul(const Array& rows, const Array& row_scales, const Array
     if (in <= 0 || n_out <= 0 || rows.dim(-1) * 4 != in || w.dim(-1) * 4 != in || scales.dim(-1) * 32 != in || w.dim(0) != n_out || scales.dim(0) != n_out ||
         rows.size() / (in / 4) != m || y.size() / n_out != m)
         throw Error(IMX_ERR_INVALID, "mxfp8_matmul: rows [M, in/4], weight [out, in/4], their scales [.., in/32] and y [M, out] do not match");
-    size_t need = 0;
-    check(imx_mxfp8_matmul_scratch_bytes(m, n_out, in, &need));
-    Scratch& sc = Scratch::local();
-    void* ws = sc.get(need);
-    check(imx_mxfp8_matmul(rows.ptr, row_scales.ptr, m, &q, n_out, in, y.ptr, ws, sc.bytes(), stream));
+    check(imx_mxfp8_matmul(rows.ptr, row_scales.ptr, m, &q, n_out, in, y.ptr, status_block(), 256, stream));
 }
+// Throws if a bounded wait ran out in a call (or a replay) of mxfp8_matmul or LowRankAdapters::add on the current device since
+// the last check; synchronises the stream.
+inline void check_status(cudaStream_t stream = nullptr) { check(imx_moe_status(status_block(), stream)); }
 
 }  // namespace ops
 
@@ -171,11 +177,7 @@ struct LowRankAdapters {
         if (in <= 0 || n_out <= 0 || x.dim(-1) != in || y.dim(-1) != n_out || ids.size() != rows || y.size() / n_out != rows || b.dim(0) != a.dim(0) ||
             b.dim(2) != a.dim(1) || (scale && scale->size() != a.dim(0)))
             throw Error(IMX_ERR_INVALID, "LowRankAdapters: shapes do not match the adapters");
-        size_t need = 0;
-        check(imx_low_rank_scratch_bytes(rows, in, n_out, ad.count, ad.rank, &need));
-        Scratch& sc = Scratch::local();
-        void* ws = sc.get(need);
-        check(imx_low_rank_add(y.ptr, x.ptr, rows, in, &ad, (const int32_t*)ids.ptr, n_out, y.ptr, ws, sc.bytes(), stream));
+        check(imx_low_rank_add(y.ptr, x.ptr, rows, in, &ad, (const int32_t*)ids.ptr, n_out, y.ptr, status_block(), 256, stream));
     }
 };
 

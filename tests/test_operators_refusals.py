@@ -139,11 +139,11 @@ def test_dimensions_that_an_int_does_not_hold(monkeypatch):
         ops.low_rank_add(meta(bf, 1, 64), meta(bf, 1, 64), meta(bf, 2, long, 64), meta(bf, 2, 64, long), ids)
 
 
-def build_cpp(out_dir):
+def build_cpp(out_dir, name="operators_main"):
     root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
-    exe, cuda, lib_dir = os.path.join(out_dir, "operators_main"), os.environ.get("CUDA_HOME", "/usr/local/cuda"), os.path.dirname(_lib.LIB_PATH)
+    exe, cuda, lib_dir = os.path.join(out_dir, name), os.environ.get("CUDA_HOME", "/usr/local/cuda"), os.path.dirname(_lib.LIB_PATH)
     subprocess.run(["g++", "-std=c++17", "-O1", "-I", os.path.join(root, "include"), "-I", os.path.join(cuda, "include"),
-                    os.path.join(root, "tests", "cpp", "operators_main.cpp"), "-o", exe, "-L", lib_dir, "-l:libironmlx_b200.so",
+                    os.path.join(root, "tests", "cpp", name + ".cpp"), "-o", exe, "-L", lib_dir, "-l:libironmlx_b200.so",
                     "-L", os.path.join(cuda, "lib64"), "-lcudart", f"-Wl,-rpath,{lib_dir}", f"-Wl,-rpath,{os.path.join(cuda, 'lib64')}"],
                    check=True, capture_output=True, text=True)
     return exe
@@ -159,6 +159,12 @@ def test_cpp_mirror_refuses_shapes(tmp_path):
 @pytest.mark.gpu
 def test_cpp_mirror_runs_the_operators(cuda, tmp_path):
     done = subprocess.run([build_cpp(str(tmp_path)), "run"], capture_output=True, text=True)
+    assert done.returncode == 0, done.stdout + done.stderr
+
+
+@pytest.mark.gpu
+def test_cpp_mirror_captures_first_calls(cuda, tmp_path):
+    done = subprocess.run([build_cpp(str(tmp_path), "operators_capture_main")], capture_output=True, text=True)
     assert done.returncode == 0, done.stdout + done.stderr
 
 
