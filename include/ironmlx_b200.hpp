@@ -75,6 +75,12 @@ struct Array {
     size_t nbytes() const { return (size_t)size() * dtype_size(dtype); }
 };
 
+// A dimension as the C ABI takes it.
+inline int as_int(int64_t n) {
+    if (n < 0 || n > INT32_MAX) throw Error(IMX_ERR_INVALID, "a dimension of " + std::to_string(n) + ", at most 2^31 - 1");
+    return (int)n;
+}
+
 inline int mode_id(const std::string& mode) {
     if (mode == "affine") return IMX_MODE_AFFINE;
     if (mode == "mxfp8") return IMX_MODE_MXFP8;
@@ -154,7 +160,7 @@ inline void dequantize(const Array& w, const Array& scales, const Array* biases,
 inline void mxfp8_matmul(const Array& rows, const Array& row_scales, const Array& w, const Array& scales, Array& y,
                          cudaStream_t stream = nullptr) {
     imx_qtensor q{w.ptr, scales.ptr, nullptr, 1.f};
-    const int in = (int)row_scales.dim(-1) * 32, n_out = (int)y.dim(-1), m = in > 0 ? (int)(row_scales.size() / (in / 32)) : 0;
+    const int in = as_int(row_scales.dim(-1) * 32), n_out = as_int(y.dim(-1)), m = in > 0 ? as_int(row_scales.size() / (in / 32)) : 0;
     if (in <= 0 || n_out <= 0 || rows.dim(-1) * 4 != in || w.dim(-1) * 4 != in || scales.dim(-1) * 32 != in || w.dim(0) != n_out || scales.dim(0) != n_out ||
         rows.size() / (in / 4) != m || y.size() / n_out != m)
         throw Error(IMX_ERR_INVALID, "mxfp8_matmul: rows [M, in/4], weight [out, in/4], their scales [.., in/32] and y [M, out] do not match");
@@ -172,8 +178,8 @@ struct LowRankAdapters {
     std::optional<Array> scale;
     // y += scale[j] * (x a[j]^T) b[j]^T with j = ids[t] for each row t (none where it is negative)
     void add(Array& y, const Array& x, const Array& ids, cudaStream_t stream = nullptr) const {
-        const imx_adapters ad{a.ptr, b.ptr, scale ? (const float*)scale->ptr : nullptr, (int)a.dim(0), (int)a.dim(1)};
-        const int in = (int)a.dim(2), n_out = (int)b.dim(1), rows = in > 0 ? (int)(x.size() / in) : 0;
+        const imx_adapters ad{a.ptr, b.ptr, scale ? (const float*)scale->ptr : nullptr, as_int(a.dim(0)), as_int(a.dim(1))};
+        const int in = as_int(a.dim(2)), n_out = as_int(b.dim(1)), rows = in > 0 ? as_int(x.size() / in) : 0;
         if (in <= 0 || n_out <= 0 || x.dim(-1) != in || y.dim(-1) != n_out || ids.size() != rows || y.size() / n_out != rows || b.dim(0) != a.dim(0) ||
             b.dim(2) != a.dim(1) || (scale && scale->size() != a.dim(0)))
             throw Error(IMX_ERR_INVALID, "LowRankAdapters: shapes do not match the adapters");
@@ -248,11 +254,11 @@ struct RMSNorm {
     // h = x + residual and its norm in one pass: y bf16 and / or rows in mxfp8 (rows and row_scales), whichever is given
     void forward_residual(const Array& x, const Array* residual, Array* h, Array* y, Array* rows, Array* row_scales,
                           cudaStream_t stream = nullptr) const {
-        const int n = (int)x.dim(-1);
+        const int n = as_int(x.dim(-1));
         if (n <= 0 || weight.size() != n || (residual && residual->size() != x.size()) || (h && h->size() != x.size()) || (y && y->size() != x.size()) ||
             (rows && rows->size() * 4 != x.size()) || (row_scales && row_scales->size() * 32 != x.size()))
             throw Error(IMX_ERR_INVALID, "RMSNorm::forward_residual: shapes do not match x");
-        check(imx_add_rms_norm(x.ptr, residual ? residual->ptr : nullptr, (int)(x.size() / n), n, weight.ptr, eps, h ? h->ptr : nullptr,
+        check(imx_add_rms_norm(x.ptr, residual ? residual->ptr : nullptr, as_int(x.size() / n), n, weight.ptr, eps, h ? h->ptr : nullptr,
                                y ? y->ptr : nullptr, rows ? rows->ptr : nullptr, row_scales ? row_scales->ptr : nullptr, stream));
     }
 };

@@ -156,6 +156,13 @@ def test_cpp_mirror_refuses_shapes(tmp_path):
     assert done.returncode == 0, done.stdout + done.stderr
 
 
+def test_cpp_mirror_refuses_sizes_that_an_int_does_not_hold(tmp_path):
+    if shutil.which("g++") is None or not os.path.exists(_lib.LIB_PATH):
+        pytest.skip("g++ or the library is missing")
+    done = subprocess.run([build_cpp(str(tmp_path), "operators_sizes_main")], capture_output=True, text=True)
+    assert done.returncode == 0, done.stdout + done.stderr
+
+
 @pytest.mark.gpu
 def test_cpp_mirror_runs_the_operators(cuda, tmp_path):
     done = subprocess.run([build_cpp(str(tmp_path)), "run"], capture_output=True, text=True)
