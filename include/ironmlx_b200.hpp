@@ -235,7 +235,7 @@ struct QuantizedLinear {
     }
     // The projection of rows that RMSNorm::forward_residual left in 8 bits (mxfp8 weights only).
     void forward_rows(const Array& rows, const Array& row_scales, Array& y, cudaStream_t stream = nullptr) const {
-        if (mode != "mxfp8") throw Error(IMX_ERR_INVALID, "forward_rows: 8-bit rows need an mxfp8 weight, not " + mode);
+        if (mode != "mxfp8" || biases) throw Error(IMX_ERR_INVALID, "forward_rows: 8-bit rows need an mxfp8 weight, not " + mode + (biases ? " with biases" : ""));
         ops::mxfp8_matmul(rows, row_scales, weight, scales, y, stream);
     }
     imx_qtensor qtensor() const {

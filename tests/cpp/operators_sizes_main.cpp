@@ -29,5 +29,11 @@ int main() {
     refused("a product over 2^32 values", [&] { Array few = bf16({4, 64}); ops::mxfp8_matmul(bf16({4, wrap / 4 + 16}), bf16({4, wrap / 32 + 2}), bf16({64, wrap / 4 + 16}), bf16({64, wrap / 32 + 2}), few); });
     refused("adapters beside 2^32 rows", [&] { LowRankAdapters{bf16({2, 8, 64}), bf16({2, 64, 8}), std::nullopt}.add(y, bf16({wrap, 64}), bf16({wrap})); });
     refused("adapters of a rank above 2^32", [&] { Array few = bf16({0, 64}); LowRankAdapters{bf16({2, wrap + 8, 64}), bf16({2, 64, wrap + 8}), std::nullopt}.add(few, bf16({0, 64}), bf16({0})); });
+    QuantizedLinear proj{};
+    proj.weight = bf16({64, 16});
+    proj.scales = bf16({64, 2});
+    proj.biases = bf16({64, 2});
+    proj.mode = "mxfp8";
+    refused("8-bit rows and a weight with biases", [&] { Array none = bf16({0, 64}); proj.forward_rows(bf16({0, 16}), bf16({0, 2}), none); });
     return wrong;
 }
