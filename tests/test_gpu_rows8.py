@@ -117,6 +117,22 @@ def test_codes_next_to_the_middle_of_two(cuda, rows, hidden):
     assert (scaled.abs() > 2.0 ** -6).all() and torch.equal(got.packed.view(torch.float8_e4m3fn).double(), want)
 
 
+@pytest.mark.parametrize("rows,hidden", [(8192, 2048), (8192, 1024), (2048, 8192), (512, 32768)])
+def test_codes_of_normal_rows(cuda, rows, hidden):
+    """Rows with a residual, whose sums of squares fp32 rounds: v in fp32, all that follows in 64 bits, and all codes above the
+    smallest normal number are the formula's."""
+    g = gen(rows + hidden)
+    x, r, w = bf16(g, rows, hidden, std=0.5), bf16(g, rows, hidden, std=2.0), bf16(g, hidden, std=0.1) + 1
+    _, _, got = ops.add_rms_norm(x, r, w, EPS, "mxfp8")
+    v = (x.float() + r.float()).double()
+    u = v / torch.sqrt((v * v).mean(-1, keepdim=True) + EPS) * w.double()
+    scaled = u / torch.exp2(got.scales.double() - 127).repeat_interleave(32, -1)
+    step = torch.exp2(torch.floor(torch.log2(scaled.abs().clamp(min=2.0 ** -6))) - 3)
+    want = (torch.round(scaled / step) * step).clamp(-448, 448)
+    normal = scaled.abs() > 2.0 ** -6
+    assert torch.equal(got.packed.view(torch.float8_e4m3fn).double()[normal], want[normal])
+
+
 def test_norm_in_place_and_leading_dimensions(cuda):
     g = gen(4)
     x, r, w = bf16(g, 2, 37, 1056), bf16(g, 2, 37, 1056), bf16(g, 1056)
