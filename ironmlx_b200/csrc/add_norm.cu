@@ -44,19 +44,19 @@ __device__ __forceinline__ void inverse_root(double a, float& hi, float& lo) {
     hi = r;
     lo = f > 0.f && f < INFINITY ? 0.5f * r * e : 0.f;
 }
-// The middle between two codes has the mantissa's last 20 bits 0x80000: a distance from it, in units of the last place, the
-// middle being kNearTie / 2.  What is nearer than fp32's roundings reach (two of v * inv * w and rsqrtf's, 3.5 units) is decided
-// with what they left out: one value in 60000, so that it costs next to nothing, and with fp32 alone 10 of the 17 million codes
-// of 8192 rows of 2048 are not the formula's.
-constexpr unsigned kNearTie = 16u << 12;
-__device__ __forceinline__ unsigned from_tie(float v) { return (__float_as_uint(v) << 12) + (0x80000000u + kNearTie / 2); }
-__device__ __forceinline__ float off_tie(float v, float inv, float inv_lo, float w, float up) {
-    const float a = v * inv, b = a * w;
-    const float rest = fmaf(a, w, -b) + (fmaf(v, inv, -a) + v * inv_lo) * w;
-    const float s = b + rest, left = rest - (s - b);
-    const uint32_t bits = __float_as_uint(s * up);
-    if ((bits & 0xfffffu) != 0x80000u || !(fabsf(left) > 0x1p-42f * fabsf(s))) return s * up;   // (rest is right to 2^-46 of s: the middle itself)
-    return __uint_as_float((left > 0.f) == (s > 0.f) ? bits + 1 : bits - 1);
+// Codes of values that fp32's roundings (two of v * inv * w, a's and rsqrtf's: under 2^-21) could have put on the other side of the
+// middle between two codes, normal numbers or not: those of the value a little larger and a little smaller differ.  They are
+// decided with what the roundings left out: one value in 50000, so that it costs next to nothing.  (Told by the mantissa's bits,
+// and below 2^-6 by the value, 8192 rows of 2048 took 27.0 us, so 25.5.)
+constexpr float kAround = 0x1p-20f;
+__device__ __forceinline__ uint32_t codes2(float a, float b) { return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3); }     // NaN stays NaN
+// v * inv * w * up for the conversion: what 64 bits round is 2^-45 of it, and so it is the middle itself if it is that near;
+// else cut off to fp32 with a last bit that keeps it off the middle (whose bit is 0) on its side.
+__device__ __forceinline__ float decided(float v, float inv, float inv_lo, float w, float up) {
+    const double d = (double)v * ((double)inv + (double)inv_lo) * (double)w * (double)up;
+    const float f = (float)d;
+    if (fabs(d - (double)f) <= fabs(d) * 0x1p-42) return f;
+    return __uint_as_float(__float_as_uint(__double2float_rz(d)) | 1u);
 }
 
 // T threads a row (a multiple of 32), blockDim.x / T rows a CTA.
@@ -165,23 +165,22 @@ add_rms_norm_kernel(const __nv_bfloat16* x, const __nv_bfloat16* residual, int n
             amax = fmaxf(amax, __shfl_xor_sync(active, amax, 2));
             const uint32_t code = scale_code(amax);
             const float up = __uint_as_float((254u - code) << 23);         // 2^-e
-            unsigned near = ~0u;
+            const float above = up * (1.f + kAround), below = up * (1.f - kAround);
+            uint32_t c[4], differ = 0;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                u[j] *= up;
-                near = min(near, from_tie(u[j]));
+            for (int j = 0; j < 4; ++j) {
+                c[j] = codes2(u[2 * j] * above, u[2 * j + 1] * above);
+                differ |= c[j] ^ codes2(u[2 * j] * below, u[2 * j + 1] * below);
             }
-            if (near <= kNearTie) {
+            if (differ != 0) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (from_tie(u[j]) <= kNearTie)
-                        u[j] = off_tie(v[i][j], inv, inv_lo, w == nullptr ? 1.f : __bfloat162float(w[(size_t)p * 8 + j]), up);
+                for (int j = 0; j < 4; ++j) {
+                    const size_t k = (size_t)p * 8 + 2 * j;
+                    const float w0 = w == nullptr ? 1.f : __bfloat162float(w[k]), w1 = w == nullptr ? 1.f : __bfloat162float(w[k + 1]);
+                    c[j] = codes2(decided(v[i][2 * j], inv, inv_lo, w0, up), decided(v[i][2 * j + 1], inv, inv_lo, w1, up));
+                }
             }
-            uint16_t c[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j)                                    // NaN stays NaN
-                c[j] = __nv_cvt_float2_to_fp8x2(make_float2(u[2 * j], u[2 * j + 1]), __NV_SATFINITE, __NV_E4M3);
-            *reinterpret_cast<uint2*>(out.q + at) = make_uint2(c[0] | (uint32_t)c[1] << 16, c[2] | (uint32_t)c[3] << 16);
+            *reinterpret_cast<uint2*>(out.q + at) = make_uint2(c[0] | c[1] << 16, c[2] | c[3] << 16);
             if ((p & 3) == 0) out.scales[at / 32] = (uint8_t)code;
         }
     }

@@ -133,6 +133,33 @@ def test_codes_of_normal_rows(cuda, rows, hidden):
     assert torch.equal(got.packed.view(torch.float8_e4m3fn).double()[normal], want[normal])
 
 
+@pytest.mark.parametrize("rows,hidden", [(2048, 8192), (4096, 2048)])
+@pytest.mark.parametrize("residual", [False, True])
+def test_small_codes_next_to_the_middle_of_two(cuda, rows, hidden, residual):
+    """A large value in every 32, so that the others are below the smallest normal number of e4m3 or around it, where codes are
+    steps of 2^-9 of the scale: they are the formula's, all of them.  (Rows of 2 and -1 whose mean square is a square, 2401 / 1024,
+    have values on the middle itself, which 64 bits miss by 2^-52.  Nothing else is nearer than 2^-48 to it there: a value in
+    steps is the root of v^2 w^2 hidden 2^c / M with whole M <= 2^15 and an 8-bit w, the middle's square a quarter of a whole
+    number, so that they are equal or 2^-30 apart.)"""
+    g = gen(rows + residual)
+    if residual:
+        x, r = bf16(g, rows, hidden, std=0.5), bf16(g, rows, hidden, std=2.0)
+    else:
+        x, r = torch.where(torch.rand(rows, hidden, generator=g, device="cuda") < torch.rand(rows, 1, generator=g, device="cuda"), 2.0, -1.0).bfloat16(), None
+    w = torch.exp2(-16 + 3 * torch.rand(hidden, generator=g, device="cuda")).bfloat16()
+    w[::32] = 1.0
+    _, _, got = ops.add_rms_norm(x, r, w, 0.0, "mxfp8")
+    v = (x.float() + r.float()).double() if residual else x.double()
+    u = v / torch.sqrt((v * v).mean(-1, keepdim=True)) * w.double()
+    scaled = u / torch.exp2(got.scales.double() - 127).repeat_interleave(32, -1)
+    step = torch.exp2(torch.floor(torch.log2(scaled.abs().clamp(min=2.0 ** -6))) - 3)
+    steps = scaled / step
+    middle = torch.floor(steps) + 0.5
+    steps = torch.where((steps - middle).abs() < 2.0 ** -48, middle, steps)
+    want = (torch.round(steps) * step).clamp(-448, 448)
+    assert (scaled.abs() < 2.0 ** -6).double().mean() > 0.5 and torch.equal(got.packed.view(torch.float8_e4m3fn).double(), want)
+
+
 def test_norm_in_place_and_leading_dimensions(cuda):
     g = gen(4)
     x, r, w = bf16(g, 2, 37, 1056), bf16(g, 2, 37, 1056), bf16(g, 1056)
