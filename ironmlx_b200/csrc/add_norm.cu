@@ -163,16 +163,28 @@ add_rms_norm_kernel(const __nv_bfloat16* x, const __nv_bfloat16* residual, int n
             for (int j = 0; j < 8; ++j) amax = fmaxf(amax, fabsf(u[j]));
             amax = fmaxf(amax, __shfl_xor_sync(active, amax, 1));
             amax = fmaxf(amax, __shfl_xor_sync(active, amax, 2));
-            const uint32_t code = scale_code(amax);
-            const float up = __uint_as_float((254u - code) << 23);         // 2^-e
+            uint32_t code = scale_code(amax);
+            float up = __uint_as_float((254u - code) << 23);               // 2^-e
             const float above = up * (1.f + kAround), below = up * (1.f - kAround);
-            uint32_t c[4], differ = 0;
+            // (amax next to 448, 1.75 * 2^8, times a power of two, by eight units of the last place: its scale is uncertain too)
+            const bool at_border = (__float_as_uint(amax) & 0x7fffffu) - 0x5ffff8u <= 16u;
+            uint32_t c[4], differ = at_border;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 c[j] = codes2(u[2 * j] * above, u[2 * j + 1] * above);
                 differ |= c[j] ^ codes2(u[2 * j] * below, u[2 * j + 1] * below);
             }
             if (differ != 0) {
+                if (at_border) {                                           // (the same in the quad)
+                    const float border = __uint_as_float((__float_as_uint(amax) & 0x7f800000u) | 0x600000u);
+                    const double root = (double)inv + (double)inv_lo, most = (double)border * (1. + 0x1p-42);      // (nearer it is the border itself)
+                    bool over = false;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        over = over || fabs((double)v[i][j] * (w == nullptr ? 1. : (double)__bfloat162float(w[(size_t)p * 8 + j]))) * root > most;
+                    code = scale_code(border) + (__any_sync(0xfu << (threadIdx.x & 28), over) ? 1u : 0u);
+                    up = __uint_as_float((254u - code) << 23);
+                }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const size_t k = (size_t)p * 8 + 2 * j;

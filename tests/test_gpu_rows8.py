@@ -160,6 +160,45 @@ def test_small_codes_next_to_the_middle_of_two(cuda, rows, hidden, residual):
     assert (scaled.abs() < 2.0 ** -6).double().mean() > 0.5 and torch.equal(got.packed.view(torch.float8_e4m3fn).double(), want)
 
 
+def four_squares(n, most):
+    """Whole numbers of at most `most` whose squares add up to n."""
+    for a in range(min(most, int(n ** 0.5)), -1, -1):
+        for b in range(min(a, int((n - a * a) ** 0.5)), -1, -1):
+            left = n - a * a - b * b
+            for c in range(min(b, int(left ** 0.5)), -1, -1):
+                d = round((left - c * c) ** 0.5)
+                if d <= c and d * d == left - c * c:
+                    return a, b, c, d
+    return None
+
+
+def test_scales_next_to_their_border(cuda):
+    """Rows of whole numbers whose largest, 7 m, has the squares' sum 2^14 m^2 + d: the norm of the largest is 7 m sqrt(4096 / sum),
+    for d = 0 exactly 3.5 = 448 * 2^-7, the largest value of the scale 2^-7; a d of one is 2^-25 of it.  The scale is the
+    formula's, which whole numbers tell: 2^-7 for d >= 0, 2^-6 for d < 0."""
+    r = np.random.default_rng(5)
+    rows, want = [], []
+    for m in range(20, 37):
+        for d in (-3, -1, 0, 0, 1, 2):
+            v = r.integers(-int(3.4 * m), int(3.4 * m) + 1, 4096)
+            v[0], v[5:9] = 7 * m * (1 if d % 2 else -1), 0
+            total, i = 2 ** 14 * m * m + d, 4095
+            while not 0 <= total - int((v * v).sum()) <= 90 * m * m:                       # (four squares below 6 m hold it)
+                v[i], i = (0 if (v * v).sum() > total else 5 * m), i - 1
+            v[5:9] = four_squares(total - int((v * v).sum()), 7 * m - 1)
+            assert (v * v).sum() == total and i > 64 and (abs(v[1:]) < 7 * m).all()
+            rows.append(v)
+            want.append(120 if d >= 0 else 121)
+    x = torch.tensor(np.array(rows), device=cuda).bfloat16()
+    assert (x.cpu().double().numpy() == np.array(rows)).all()
+    _, _, got = ops.add_rms_norm(x, None, None, 0.0, "mxfp8")
+    assert got.scales[:, 0].tolist() == want
+    _, _, got = ops.add_rms_norm(x * 0.5, (x * 0.5), None, 0.0, "both")                    # the same sum, from two halves
+    assert got.scales[:, 0].tolist() == want
+    u = x.double() / torch.sqrt((x.double() ** 2).mean(-1, keepdim=True))
+    check_rows(got, u)
+
+
 def test_norm_in_place_and_leading_dimensions(cuda):
     g = gen(4)
     x, r, w = bf16(g, 2, 37, 1056), bf16(g, 2, 37, 1056), bf16(g, 1056)
