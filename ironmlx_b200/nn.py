@@ -39,6 +39,8 @@ class LowRankAdapters:
 class _WithAdapters:
     def forward_with_adapters(self, x: torch.Tensor, adapters: LowRankAdapters, ids: torch.Tensor, stream=None) -> torch.Tensor:
         """The shared projection of all rows and the low-rank adapter ids[t] of each (int32, negative: none)."""
+        if not x.is_cuda:
+            raise IronMLXError(_lib.ERR_INVALID, "forward_with_adapters: tensors must be contiguous CUDA tensors")
         if ops._elsewhere(x, stream):
             with ops._on(x, stream):
                 return self.forward_with_adapters(x, adapters, ids)

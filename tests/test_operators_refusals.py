@@ -201,3 +201,12 @@ def test_python_layer_refuses_host_tensors_and_other_formats():
         ops.mxfp8_matmul((w, s), w, s)
     with pytest.raises(_lib.IronMLXError):
         nn.QuantizedLinear(w, s, None, 64, 4, "affine").forward_rows((w, s))
+
+
+def test_projection_with_adapters_refuses_host_tensors():
+    x, ids = torch.zeros(2, 64, dtype=torch.bfloat16), torch.zeros(2, dtype=torch.int32)
+    adapters = nn.LowRankAdapters(torch.zeros(1, 8, 64, dtype=torch.bfloat16), torch.zeros(1, 16, 8, dtype=torch.bfloat16))
+    for layer in (nn.Linear(torch.zeros(16, 64, dtype=torch.bfloat16)),
+                  nn.QuantizedLinear(torch.zeros(16, 16, dtype=torch.int32), torch.zeros(16, 2, dtype=torch.uint8), None, 32, 8, "mxfp8")):
+        with pytest.raises(_lib.IronMLXError, match="CUDA"):
+            layer.forward_with_adapters(x, adapters, ids)
