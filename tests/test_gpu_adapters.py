@@ -81,6 +81,19 @@ def test_whole_numbers_of_24_bits_are_exact(cuda, t, n, count, rank):
     assert torch.equal(run(p, ids), (p["y"].double() + add).float().bfloat16())
 
 
+@pytest.mark.parametrize("t,count,rank", [(129, 129, 16), (200, 150, 64), (256, 200, 16), (256, 2100, 8), (384, 300, 128), (512, 400, 16), (512, 512, 64)])
+def test_more_rows_than_128_with_nearly_as_many_adapters(cuda, t, count, rank):
+    """A decode batch above the size of the kernel for few rows, most of whose rows are alone with their adapter."""
+    g = gen(t + count)
+    p = make(g, t, 1024, 520, count, rank)
+    ids = torch.randperm(count, generator=g, device="cuda")[torch.arange(t, device="cuda") % count].int()
+    ids[::17] = -1
+    ids[1] = ids[t - 1]
+    out = run(p, ids)
+    check(out, p, ids)
+    assert torch.equal(out, run(p, ids))
+
+
 @pytest.mark.parametrize("t", [3, 70, 700])
 def test_ids_without_an_adapter(cuda, t):
     """No row has one; ids far outside; every row the last adapter.  What a row without an adapter holds is left bit for bit,
