@@ -74,17 +74,14 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// v = hi + mid + lo (parts 0, 1, 2), each the next 8 of its 24 bits: bf16 numbers in the upper halves of 32 bits.  (Cut off, not
-// rounded: hi is finite where v is; what is not finite stays in hi.)
-__device__ __forceinline__ uint32_t upper(float v) { return __float_as_uint(v) & 0xffff0000u; }
-__device__ __forceinline__ void split3(float v, uint32_t (&part)[3]) {
-    const bool finite = fabsf(v) < INFINITY;
-    part[0] = finite ? upper(v) : __float_as_uint(v) | (v == v ? 0u : 0x400000u);
-    const float left = finite ? v - __uint_as_float(part[0]) : 0.f;
-    part[1] = upper(left);
-    part[2] = __float_as_uint(left - __uint_as_float(part[1]));
+// v = hi + mid + lo, each the next 8 of its 24 bits: bf16 numbers in the upper halves of 32 bits.  (Cut off, not rounded: hi is
+// finite where v is; what is not finite stays in hi.)
+__device__ __forceinline__ float upper(float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
+__device__ __forceinline__ float after_upper(float v) {
+    const float left = v - upper(v);
+    return left == left ? left : 0.f;
 }
-__device__ __forceinline__ uint32_t pack2(uint32_t a, uint32_t b) { return __byte_perm(a, b, 0x7632); }       // two upper halves
+__device__ __forceinline__ uint32_t pack2(float a, float b) { return __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632); }       // two upper halves
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
     const int n = there ? 16 : 0;             // the rest is filled with zeros
@@ -182,8 +179,11 @@ __device__ __forceinline__ int find_unit(const LowRankArgs& p, FewShared& s, int
 
 // `clusters` clusters of `ctas` CTAs a unit: each cluster multiplies x . a^T for itself and takes a part of the columns.
 // TP: tiles of eight values of the rank that a warp multiplies (1, 2 or 4; RB > 1: 4).
+// Two CTAs an SM above a rank of 32: three would leave 80 registers (rank 64, 128 rows of 16 and 120 adapters 15.4 and 32.9 us,
+// with two 13.7 and 27.7; 48 rows of 40 adapters, which fill three, 16.4 and 17.3).
+constexpr int few_ctas(int rb) { return rb <= 1 ? 3 : 2; }
 template <int RB, int TP>
-__global__ void __launch_bounds__(kThreads, RB <= 2 ? 3 : 2)
+__global__ void __launch_bounds__(kThreads, few_ctas(RB))
 low_rank_few_kernel(const LowRankArgs p, const int ctas, const int clusters) {
     __shared__ __align__(16) FewShared s;
     extern __shared__ __align__(16) unsigned char dyn[];
@@ -341,10 +341,10 @@ low_rank_few_kernel(const LowRankArgs p, const int ctas, const int clusters) {
             }
             v *= sc;
         }
-        uint32_t part[3];
-        split3(v, part);
+        const float left = after_upper(v), part[3] = {v, left, left - upper(left)};
 #pragma unroll
-        for (int h = 0; h < 3; ++h) low_rows[(h * kFewUnit + r) * RB * 32 + (RB > 1 ? k ^ ((r & 1) * 32) : k)] = __ushort_as_bfloat16((unsigned short)(part[h] >> 16));
+        for (int h = 0; h < 3; ++h)
+            low_rows[(h * kFewUnit + r) * RB * 32 + (RB > 1 ? k ^ ((r & 1) * 32) : k)] = __ushort_as_bfloat16((unsigned short)(__float_as_uint(part[h]) >> 16));
     }
     if (ctas > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");     // this CTA has read the others' sums
     __syncthreads();
@@ -353,13 +353,14 @@ low_rank_few_kernel(const LowRankArgs p, const int ctas, const int clusters) {
     const uint4* low_even = reinterpret_cast<const uint4*>(low_rows) + g * RB * 4 + (RB > 1 ? (g & 1) * 4 : 0) + q;     // of even blocks, odd ones
     const uint4* low_odd = low_even - (g & 1) * 8;
     auto low_at = [&](int kb, int h, int r) { return (kb & 1 ? low_odd : low_even)[(h * kFewUnit + r * 8) * RB * 4 + kb * 4]; };     // hi, mid, lo; rows g and g + 8
-    // up to a rank of 128 the low-rank rows stay in registers (read for every tile they cost a rank of 128 half of its time)
-    constexpr int kKept = RB <= 4 ? RB : 1;
-    uint4 low[kKept][3][2];
+    // Up to a rank of 128 the low-rank rows stay in registers (read for every tile they cost a rank of 128 half of its time), of
+    // ranks above 64 hi and mid alone (lo from shared memory: 128 rows of 2 adapters 17.3 us, all three, with spills, 18.1).
+    constexpr int kKept = RB <= 4 ? RB : 1, kParts = RB == 4 ? 2 : 3;
+    uint4 low[kKept][kParts][2];
 #pragma unroll
     for (int kb = 0; kb < kKept; ++kb)
 #pragma unroll
-        for (int h = 0; h < 3; ++h)
+        for (int h = 0; h < kParts; ++h)
 #pragma unroll
             for (int r = 0; r < 2; ++r) low[kb][h][r] = low_at(kb, h, r);
     size_t at0 = (size_t)row0 * p.n_out + (t0 + warp) * 8 + 2 * q, at1 = (size_t)row1 * p.n_out + (t0 + warp) * 8 + 2 * q;
@@ -384,19 +385,20 @@ low_rank_few_kernel(const LowRankArgs p, const int ctas, const int clusters) {
             const int i0 = kKept == RB ? kb : 0;
             if (kKept != RB) {
 #pragma unroll
-                for (int h = 0; h < 3; ++h) {
+                for (int h = 0; h < kParts; ++h) {
                     low[0][h][0] = low_at(kb, h, 0);
                     if (more) low[0][h][1] = low_at(kb, h, 1);
                 }
             }
-            // (the small parts in sums of their own)
-#pragma unroll
-            for (int h = 2; h >= 0; --h) {
-                float(&to)[4] = h == 0 ? d : e;
-                const uint4 v0 = low[i0][h][0], v1 = low[i0][h][1];
-                mma(to, v0.x, v1.x, v0.y, v1.y, w.x, w.y);
-                mma(to, v0.z, v1.z, v0.w, v1.w, w.z, w.w);
-            }
+            // (two sums, lo in both by turns: one for mid and lo would make the chain of MMAs twice as long)
+            const uint4 h0 = low[i0][0][0], h1 = low[i0][0][1], m0 = low[i0][1][0], m1 = low[i0][1][1];
+            const uint4 l0 = kParts == 3 ? low[i0][kParts - 1][0] : low_at(kb, 2, 0), l1 = kParts == 3 ? low[i0][kParts - 1][1] : low_at(kb, 2, 1);
+            mma(e, l0.x, l1.x, l0.y, l1.y, w.x, w.y);
+            mma(d, l0.z, l1.z, l0.w, l1.w, w.z, w.w);
+            mma(e, m0.x, m1.x, m0.y, m1.y, w.x, w.y);
+            mma(d, h0.x, h1.x, h0.y, h1.y, w.x, w.y);
+            mma(e, m0.z, m1.z, m0.w, m1.w, w.z, w.w);
+            mma(d, h0.z, h1.z, h0.w, h1.w, w.z, w.w);
         }
         if (out_col < p.n_out) {
             if (has0) write(at0, yv.x, d[0] + e[0], d[1] + e[1]);
@@ -880,6 +882,7 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
         // and mid of a warp's 16 rows in its 32 lanes, and in columns behind them lo and zeros.
         {
             const float* row = reinterpret_cast<const float*>(smem + pl.low_at) + (rt * 16 + (lane & 15)) * pl.low_pitch;
+            const uint32_t keep = lane < 16 ? 0xffffffffu : 0u;
 #pragma unroll 1
             for (int jb = 0; jb < NJ; ++jb) {
                 uint32_t cols[16] = {};
@@ -888,17 +891,13 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
                     const int k = jb * 32 + i * 4;
                     if (k >= r16) break;
                     const float4 f = *reinterpret_cast<const float4*>(row + k);
-                    uint32_t p0[3], p1[3], p2[3], p3[3];
-                    split3(f.x, p0);
-                    split3(f.y, p1);
-                    split3(f.z, p2);
-                    split3(f.w, p3);
+                    const float l0 = after_upper(f.x), l1 = after_upper(f.y), l2 = after_upper(f.z), l3 = after_upper(f.w);
                     if (half == 0) {
-                        cols[2 * i] = lane < 16 ? pack2(p0[0], p1[0]) : pack2(p0[1], p1[1]);
-                        cols[2 * i + 1] = lane < 16 ? pack2(p2[0], p3[0]) : pack2(p2[1], p3[1]);
-                    } else if (lane < 16) {
-                        cols[2 * i] = pack2(p0[2], p1[2]);
-                        cols[2 * i + 1] = pack2(p2[2], p3[2]);
+                        cols[2 * i] = pack2(lane < 16 ? f.x : l0, lane < 16 ? f.y : l1);
+                        cols[2 * i + 1] = pack2(lane < 16 ? f.z : l2, lane < 16 ? f.w : l3);
+                    } else {
+                        cols[2 * i] = pack2(l0 - upper(l0), l1 - upper(l1)) & keep;
+                        cols[2 * i + 1] = pack2(l2 - upper(l2), l3 - upper(l3)) & keep;
                     }
                 }
                 tc::tmem_st16(tmem + ((uint32_t)(rt * 32) << 16) + kLowAt + (uint32_t)(half * (int)kLowCols + jb * 16), cols);
@@ -1050,8 +1049,8 @@ int launch_clusters(const void* kernel, unsigned grid, int threads, int ctas, si
     return IMX_OK;
 }
 
-// 128 rows, 2048 -> 4096, by the two kernels, in us: 16 adapters of rank 16, 64, 128  9.0, 13.9, 19.9 and (tiles) 18.3, 19.3, 30.0;
-// 120 adapters  16.8, 27.1, 46.0 and 38.5, 42.7, 67.2; 2 adapters  8.2, 11.2, 16.0 and 11.0, 13.1, 17.0.  So up to 128 rows are
+// 128 rows, 2048 -> 4096, by the two kernels, in us: 16 adapters of rank 16, 64, 128  9.5, 13.9, 21.4 and (tiles) 12.9, 15.8, 29.5;
+// 120 adapters  17.6, 28.5, 53.2 and 29.5, 35.8, 65.4; 2 adapters  8.8, 12.1, 17.5 and 9.2, 12.0, 16.1.  So up to 128 rows are
 // few; so are, 128 at a time, more of them where the tile kernel cannot count the adapters or name b's rows in 31 bits.
 int launch_low_rank(LowRankArgs p, int sms, cudaStream_t stream) {
     const int rows = p.n, step = rows <= kFewRows || p.count >= kMaxBins || (long)p.count * p.n_out > 0x7fffffffL ? kFewRows : kBlockRows;
@@ -1074,12 +1073,12 @@ int launch_low_rank(LowRankArgs p, int sms, cudaStream_t stream) {
         void* args[] = {&p, &ctas, nullptr, nullptr};
         if (step == kFewRows) {
             // Units: no more than every 16th row leads because 16 have gone before, and one of every id.  A cluster up to
-            // CTAs for three on every SM (two, where the rings leave room for no more): 48 rows of 40 adapters with two 12.4
+            // CTAs for three on every SM (two, where registers or rings leave room for no more): 48 rows of 40 adapters with two 12.4
             // us, with one 14.0, with three 11.7.  More clusters of a unit repeat x . a^T and pay while SMs are idle: one row,
             // 2048 -> 8192, 5.5 us, in one cluster 8.1.
             const FewKernel few = few_kernel(p.rank);
             const int ids = p.count < p.n ? p.count + 1 : p.n, bound = p.n / kFewUnit + ids, units = bound < p.n ? bound : p.n;
-            while (ctas < 8 && units * ctas * 2 <= (few.rb <= 2 ? 3 : 2) * sms) ctas *= 2;
+            while (ctas < 8 && units * ctas * 2 <= few_ctas(few.rb) * sms) ctas *= 2;
             int clusters = 1;
             while (clusters < 16 && units * ctas * clusters * 2 <= sms && p.n_out >= 128 * ctas * clusters) clusters *= 2;
             args[2] = &clusters;
