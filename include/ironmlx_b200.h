@@ -159,8 +159,9 @@ IMX_API int imx_rms_norm(const void* x, int n_rows, int hidden, const void* weig
  * (mlx/src/model/qwen35.rs:262-273 around fast::rms_norm):
  *   v = x + residual (fp32), h = bf16(v), u = v * rsqrt(mean(v^2) + eps) * weight (fp32)
  *   y = bf16(u);  y_q, y_scales = u as mxfp8 rows (imx_quantize's layout and rule), which imx_mxfp8_matmul reads
- * Sums and products stay in fp32 and every output is rounded once: y may differ from imx_rms_norm's of h, which
- * rounds in between, by a step of bf16.
+ * Sums and products are held in fp32 or more and every output is rounded once: y may differ from imx_rms_norm's of h, which
+ * rounds in between, by a step of bf16.  Codes and scales are the formula's for v, evaluated in 64 bits (next to the middle of two
+ * codes by 2^-42 of the value: the middle itself).
  * x, residual, h, y: bf16 [n_rows, hidden]; residual may be NULL (v = x); weight: bf16 [hidden] or NULL; y_q: e4m3
  * [n_rows, hidden], y_scales: ue8m0 [n_rows, hidden / 32].  h, y and the pair y_q, y_scales may each be NULL, not all.
  * hidden: a multiple of 8 (of 32 with y_q), at most 32768; arrays 16-byte aligned (y_scales: any).  h or y may be x's or
@@ -407,7 +408,7 @@ typedef struct imx_adapters {
 /* The adapters of many requests beside a shared projection (no counterpart in the reference): row t of the batch has
  * the adapter j = ids[t],
  *   out[t] = bf16( y[t] + scale[j] * (x[t] . a[j]^T) . b[j]^T )
- * with y[t] the projection's row, x[t] its input, sums in fp32.  A row whose id is outside [0, count) -- -1 by convention --
+ * with y[t] the projection's row, x[t] its input, sums, and the low-rank row between the two products, in fp32.  A row whose id is outside [0, count) -- -1 by convention --
  * has no adapter: out[t] = y[t].  Ids may come in any order.
  * x: bf16 [n_rows, in], in a multiple of 8; in and n_out at most 2^30; y, out: bf16 [n_rows, n_out]; out may be y itself, any other overlap is refused.
  * x, a and b 16-byte aligned; y and out at any bf16 value (16 bytes and n_out a multiple of 8 are fastest).

@@ -4,11 +4,12 @@
 //   u = v * inv * w               fp32, inv = rsqrt(mean(v^2) + eps); y = bf16(u)
 //   q = e4m3(u / 2^e)             e per 32 values: the smallest power of two with amax / 2^e <= 448 (imx_quantize's rule)
 //
-// Bound by memory for many rows, by latency for few: 8192 rows of 2048 with a residual and all outputs take 27.1 us (152 MB at
-// 5.6 TB/s, 85% of the copy bandwidth), 777 rows of 5120 5.3 us, 64 rows of 2048 2.5 us.  A row's values stay in the registers of its threads between the
-// sum of squares and the outputs (NV pieces of eight values a thread), so that everything is read and written once.
-// Four neighbouring lanes hold the 32 values of a scale: two shuffles give the maximum.  Dividing by a power of two is
-// exact, so that the 8-bit conversion is the only rounding there.
+// Bound by memory for many rows, by latency for few: 8192 rows of 2048 with a residual and all outputs take 29 us (152 MB at
+// 5.2 TB/s, 80% of the copy bandwidth), 777 rows of 5120 in bf16 5.6 us, 64 rows of 2048 2.6 us.  A row's values stay in the
+// registers of its threads between the sum of squares and the outputs (NV pieces of eight values a thread), so that everything is
+// read and written once.  Four neighbouring lanes hold the 32 values of a scale: two shuffles give the maximum.  Codes and scales
+// are those that the formula has for v: squares are summed in 64 bits where codes leave, and what fp32 leaves uncertain after that
+// is computed in 64 bits (1.5 of the 29 us).
 #include <cuda_fp8.h>
 
 #include "internal.h"

@@ -12,12 +12,13 @@
 // Two kernels (times on a B200, of the kernels alone):
 //   few rows (at most 128): a and b are read once and go straight into the fragments of mma.sync, whose k order is permuted so
 //     that a lane's 16 bytes are four k pairs.  Bound by latency, of memory (each lane brings what it alone reads, through a
-//     ring of cp.async) and of the cluster's two meetings: one row of rank 16, 2048 -> 8192, takes 5.2 us; 48 rows of 40
-//     adapters of rank 32, 4096 -> 2048 (16 MB: 2.5 us at the copy bandwidth), 11.2 us.
+//     ring of cp.async) and of the cluster's two meetings: one row of rank 16, 2048 -> 8192, takes 5.0 us; 48 rows of 40
+//     adapters of rank 32, 4096 -> 2048 (16 MB: 2.5 us at the copy bandwidth), 11.6 us.
 //   many rows: tiles of 64 rows by tcgen05.mma, x and y gathered by cp.async, a and b brought by TMA.  8192 rows of rank 64,
-//     2048 -> 8192, take 71 us, 318 MB at 4.5 TB/s: y comes and leaves at 6.2 TB/s, close to the copy bandwidth, but the ids
-//     (5 us), x . a^T (7 us) and the cluster's exchange (5 us) come before it, for all CTAs at the same time.  With mma.sync by
-//     the warps that copy it was 113 us; rank 128 takes 93 us (229).  777 rows of rank 16 take 16 us, each phase a latency or two.
+//     2048 -> 8192, take 69 us, 318 MB at 4.6 TB/s: y comes and leaves in 37 us (268 MB; a third of the writes is left in L2),
+//     but the ids (4.6 us), x . a^T (6.1 us), the cluster's exchange and the low-rank rows' way into tensor memory (5.4 us) come
+//     before it, for all CTAs at the same time.  With mma.sync by the warps that copy it was 113 us; rank 128, one CTA an SM,
+//     takes 108 us (229).  777 rows of rank 16 take 16 us, each phase a latency or two.
 #include <atomic>
 
 #include "tcgen05.cuh"
@@ -912,7 +913,7 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
         uint32_t y = base + (uint32_t)((n_in % S) * pl.stage);                   // ... and its place
         const uint32_t frag_at = (uint32_t)((rt * 16 + (lane & 7)) * 128 + (((half * 4 + (lane >> 3)) ^ (lane & 7)) * 16));
         // Rows that start on 4 bytes, not on 16: a lane's own values two at a time, a stage ahead (5034 outputs, 2579 rows of rank
-        // 128: 66 us, one by one when they are needed 171).  Rows of an odd number are left at that.
+        // 128: 74 us; 5033 outputs, one by one when they are needed, 186).  Rows of an odd number are left at that.
         const bool pairs = !WIDE && p.n_out % 2 == 0 && (((uintptr_t)p.y | (uintptr_t)p.out) % 4) == 0;
         const size_t row_at[2] = {(size_t)s.rows[has_own[0] ? rt * 16 + g : 0] * p.n_out, (size_t)s.rows[has_own[1] ? rt * 16 + g + 8 : 0] * p.n_out};
         uint32_t ahead[2][4];

@@ -26,7 +26,7 @@
 // the tiles concerned are NaN.
 //
 // On a B200, the kernel alone: 8192 rows, 2048 -> 8192, 102 us, 2.7 PFLOP/s, 81% of twice cuBLAS' bf16 rate (in a loop of
-// seconds the power limit makes it 122 to 125 us); 777 rows, 4096 -> 2048, 12.2 us; 64 rows, 2048 -> 152064, 55 us, 6.2 TB/s; one row,
+// seconds the power limit makes it 122 to 125 us); 777 rows, 4096 -> 2048, 12.2 us; 64 rows, 2048 -> 152064, 55 to 59 us, 6.2 to 5.8 TB/s; one row,
 // 2048 -> 8192, 7 us, of which 4 are a launch's and the ring's filling.  What a K step of 128 costs beside its MMAs bounds all that
 // is not large: 340 cycles for the warp that issues them, before it issued by predicates and looked ahead 600.
 #include <atomic>
@@ -718,7 +718,7 @@ int launch(const Call& c, int lg_splits, int height = PAIR ? 256 : 128) {
 //   64 rows   S64 9.5 (9.4), S64 cut in 2 10.2 (9.8), N64 7.7 (7.7);   4096 -> 2048  S64 cut in 4 8.5 (8.8), N64 9.6 (10.6)
 //   256 rows  N64 11.1 (10.6), N128 9.1 (9.0), P128 9.7 (9.5), P256 11.9 (12.1)
 //   777 rows 4096 -> 2048  N64 16.7 (16.5), N128 12.6 (12.6), P128 12.8 (12.8), P256 17.4 (17.8)
-//   1024 rows N128 20.8 (19.8), P128 19.4 (19.5), P256 18.2 (17.8);   8192 rows  N128 130, P128 115, P256 99
+//   1024 rows N128 20.8 (19.8), P128 19.4 (19.5), P256 17.4 (17.8);   8192 rows  N128 130, P128 115, P256 99
 //   64 rows 2048 -> 152064  S64 55, N64 63, N128 58, P128 70, P256 68 (memory: 52)
 // Clusters of eight that fill the GPU find no place together: 4096 -> 2048, 1 row, cut in 8 (128 CTAs) 11.3, in 4 6.7.
 int run(const Call& c) {
