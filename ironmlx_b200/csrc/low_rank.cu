@@ -479,18 +479,17 @@ struct TilePlan {
 };
 static_assert(TilePlan(8, 1).smem() >= kTileSmem && TilePlan(40, 2).smem() >= kTileSmem, "beside another kernel that waits in a cluster");
 
-// 16 lanes x 8 columns a count: thread t gets of each block of eight columns lane t / 4, columns 2 (t % 4), +1, and the same of
+// (On their way until tmem_wait.)  16 lanes x 8 columns a count: thread t gets of each block of eight columns lane t / 4, columns 2 (t % 4), +1, and the same of
 // lane t / 4 + 8, as an mma.sync leaves its sums.
 __device__ __forceinline__ void tmem_ld_16x16(uint32_t taddr, float (&v)[8]) {
-    uint32_t u[8];
     asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-                 : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7])
+                 : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
                  : "r"(taddr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(u[i]);
 }
-// (On its way until tmem_wait.)
+__device__ __forceinline__ void tmem_wait(float (&v)[8]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7])::"memory");
+}
 __device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t (&u)[16]) {
     asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
                  : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]), "=r"(u[9]),
@@ -523,7 +522,11 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
     // the allocation behind the ids half of the CTAs of 8192 rows started 6.7 us late, of 777 rows 3.2).
     // The first product's sums; in their place two stages' of the second, and from column 128 on its A, see below.
     static_assert(NJ > 2 || 2 * (128 + 2 * 16 * NJ) <= 512, "two CTAs an SM");
-    constexpr uint32_t kTmem = NJ <= 4 ? 256 : 512, kLowAt = 128, kLowCols = 16 * NJ;
+    // (The tensor cores cut each addition off, not round it: a sum of 172 K steps is off by up to 2^-18, as much as 16 bits of the
+    // low-rank row.  So the first product has several sums, a stage each in turn, which are added in the end.)
+    constexpr uint32_t kTmem = NJ <= 2 ? 256 : 512, kLowAt = 128, kLowCols = 16 * NJ;
+    constexpr int kSums = NJ <= 4 ? 4 : 2;
+    static_assert(kSums * NJ * 32 <= (int)kTmem && kLowAt + 2 * kLowCols <= kTmem, "tensor memory");
     if (warp == 9) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(&s.tmem_base)), "r"(kTmem) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
@@ -728,7 +731,8 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
             const uint32_t st = base + (uint32_t)(slot * pl.stage), idesc = tc::idesc_for(64, r16) | (1u << 7) | (1u << 10);      // bf16
 #pragma unroll
             for (int kk = 0; kk < kCols / 16; ++kk)
-                tc::umma_ss_if(me, tmem, tc::smem_desc(st) + 2 * kk, tc::smem_desc(st + kBlock) + 2 * kk, idesc, i > 0 || kk > 0 ? 1u : 0u);
+                tc::umma_ss_if(me, tmem + (uint32_t)((i % kSums) * NJ * 32), tc::smem_desc(st) + 2 * kk, tc::smem_desc(st + kBlock) + 2 * kk, idesc,
+                               i >= kSums || kk > 0 ? 1u : 0u);
             tc::umma_commit_if<false>(me, tc::smem_u32(&s.used[slot]));
             __syncwarp();
             next_stage();
@@ -836,8 +840,17 @@ low_rank_tile_kernel(const LowRankArgs p, const int ctas, const int clusters, co
         for (int j = 0; j < NJ; ++j) {
             const int t = half + 2 * j;
             if (t * 16 >= r16) break;
-            float v[8] = {};
-            if (n_in > 0) tmem_ld_16x16(tmem + ((uint32_t)(rt * 32) << 16) + (uint32_t)(t * 16), v);
+            float v[8] = {}, u[kSums][8];
+#pragma unroll
+            for (int k = 0; k < kSums; ++k)
+                if (k < n_in) tmem_ld_16x16(tmem + ((uint32_t)(rt * 32) << 16) + (uint32_t)(k * NJ * 32 + t * 16), u[k]);
+#pragma unroll
+            for (int k = 0; k < kSums; ++k) {
+                if (k >= n_in) break;
+                tmem_wait(u[k]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[i] += u[k][i];
+            }
             if (gave_up)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(0x7fc00000u);

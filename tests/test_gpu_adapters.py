@@ -81,6 +81,24 @@ def test_whole_numbers_of_24_bits_are_exact(cuda, t, n, count, rank):
     assert torch.equal(run(p, ids), (p["y"].double() + add).float().bfloat16())
 
 
+@pytest.mark.parametrize("rank,steps", [(16, 32), (64, 32), (128, 32), (256, 64)])
+def test_long_sums_are_not_cut_off_too_often(cuda, rank, steps):
+    """Sums of 4096 positive products, of which y takes the first eight bits.  The tensor cores cut a sum off at each addition, by
+    half a unit of its last place on average, which at a share f of the whole is at most f 2^-23 of it: `steps` additions to one
+    sum make it steps 2^-25 too small on average (roundings of the outputs have no such mean).  A CTA of two has 2048 of the
+    values, 128 K steps, as four sums (two above a rank of 128)."""
+    g = gen(rank)
+    t, n = 8192, 64
+    x, a = ((1 + torch.rand(*shape, generator=g, device="cuda")).bfloat16() for shape in ((t, 4096), (1, rank, 4096)))
+    b = torch.zeros(1, n, rank, dtype=torch.bfloat16, device=cuda)
+    b[0, torch.arange(n, device=cuda), torch.arange(n, device=cuda) % rank] = 1.0
+    add = (x.double() @ a[0].double().T) @ b[0].double().T
+    y = -add.bfloat16()
+    out = ops.low_rank_add(y, x, a, b, torch.zeros(t, dtype=torch.int32, device=cuda))
+    off = ((out.double() - (y.double() + add)) / add).mean().item()
+    assert abs(off) <= steps * 2.0 ** -25, (off, steps * 2.0 ** -25)
+
+
 @pytest.mark.parametrize("t,count,rank", [(129, 129, 16), (200, 150, 64), (256, 200, 16), (256, 2100, 8), (384, 300, 128), (512, 400, 16), (512, 512, 64)])
 def test_more_rows_than_128_with_nearly_as_many_adapters(cuda, t, count, rank):
     """A decode batch above the size of the kernel for few rows, most of whose rows are alone with their adapter."""
